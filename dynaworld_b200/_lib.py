@@ -101,6 +101,26 @@ class Splats2DGrads(C.Structure):
     _fields_ = [("means", vp), ("conics", vp), ("opacities", vp), ("packed", vp), ("colors", vp)]
 
 
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class Norm(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("dim", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("x", vp), ("x_stride", C.c_int64), ("residual", vp), ("residual_stride", C.c_int64), ("weight", vp),
+    ]
+
+
+class Linear(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
+        ("activation", C.c_int32), ("reserved", C.c_int32), ("x", vp), ("x_stride", C.c_int64), ("weight", vp),
+        ("weight_stride", C.c_int64), ("bias", vp), ("residual", vp), ("residual_stride", C.c_int64),
+        ("x_scale", vp), ("weight_scale", vp),
+    ]
+
+
 P = C.POINTER
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -135,6 +155,15 @@ SIGNATURES = {
     "gsb_splats2d_preprocess": (C.c_int, [P(Splats2D), C.c_int32, C.c_int32, P(Options), vp, vp, vp, vp, vp,
                                           C.c_size_t, vp]),
     "gsb_splats2d_preprocess_bwd": (C.c_int, [P(Splats2D), vp, vp, P(Splats2DGrads), vp]),
+    "gsb_rms_norm_fwd": (C.c_int, [P(Norm), vp, vp, vp, vp]),
+    "gsb_rms_norm_bwd_workspace": (C.c_size_t, [P(Norm)]),
+    "gsb_rms_norm_bwd": (C.c_int, [P(Norm), vp, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, C.c_size_t, vp]),
+    "gsb_rms_norm_fp8": (C.c_int, [P(Norm), vp, vp, vp, vp]),
+    "gsb_quantize_rows_fp8": (C.c_int, [P(Norm), vp, vp, vp]),
+    "gsb_linear_fwd_workspace": (C.c_size_t, [P(Linear)]),
+    "gsb_linear_fwd": (C.c_int, [P(Linear), vp, vp, vp, C.c_size_t, vp]),
+    "gsb_linear_bwd_workspace": (C.c_size_t, [P(Linear)]),
+    "gsb_linear_bwd": (C.c_int, [P(Linear), vp, vp, C.c_int64, vp, vp, vp, vp, C.c_size_t, vp]),
     "gsb_radix_sort_workspace": (C.c_size_t, [C.c_uint32, C.c_int, C.c_int]),
     "gsb_radix_sort": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),
     "gsb_debug_sort_lookback_timeout": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, vp, C.c_size_t, vp]),

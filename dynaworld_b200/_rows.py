@@ -1,0 +1,53 @@
+"""Argument handling shared by the token-side operators (linear, norm)."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib
+
+TYPE_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+E4M3 = torch.float8_e4m3fn
+_NOTHING = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` current for the launches inside (nothing to do when it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(device)
+
+
+def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
+    """[..., width] as [rows, width] with adjacent row elements: a view where the strides allow it
+    (any positive row stride), else a copy."""
+    if t.ndim != 2:
+        t = t.reshape(-1, width)
+    if (t.stride(1) != 1 and width > 1) or (t.shape[0] > 1 and t.stride(0) < 1):
+        t = t.contiguous()
+    return t
+
+
+def check_input(what: str, x: torch.Tensor) -> int:
+    """The element-type code of x, or the error that refuses it."""
+    code = TYPE_CODES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"{what} takes float32, bfloat16 or float16 tensors, got {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what} needs rows of at least one element, got shape {tuple(x.shape)}")
+    return code
+
+
+def check_device(what: str, x: torch.Tensor) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"the b200 {what} runs on CUDA devices only (got a tensor on {x.device})")
+
+
+def check_like(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, the input on {device}")

@@ -584,4 +584,43 @@ GSB_API gsb_status gsb_debug_sort_lookback_timeout(const uint32_t* keys_in, uint
                                      workspace_bytes - align_up(sizeof(WorkspaceHeader)), st, status);
 }
 
+
+// ---- token side ------------------------------------------------------------------------------
+
+GSB_API gsb_status gsb_rms_norm_fwd(const gsb_norm* norm, void* y, void* summed, float* rstd, void* stream) {
+  return rms_norm_fwd(norm, y, summed, rstd, as_stream(stream));
+}
+
+GSB_API size_t gsb_rms_norm_bwd_workspace(const gsb_norm* norm) { return rms_norm_bwd_workspace(norm); }
+
+GSB_API gsb_status gsb_rms_norm_bwd(const gsb_norm* norm, const float* rstd, const void* dy, int64_t dy_stride,
+                                    const void* dsummed, int64_t dsummed_stride, void* dx, void* dweight,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  return rms_norm_bwd(norm, rstd, dy, dy_stride, dsummed, dsummed_stride, dx, dweight, workspace, workspace_bytes,
+                      as_stream(stream));
+}
+
+GSB_API gsb_status gsb_rms_norm_fp8(const gsb_norm* norm, void* codes, float* scales, void* summed, void* stream) {
+  return rms_norm_fp8(norm, codes, scales, summed, as_stream(stream));
+}
+
+GSB_API gsb_status gsb_quantize_rows_fp8(const gsb_norm* rows, void* codes, float* scales, void* stream) {
+  return quantize_rows_fp8(rows, codes, scales, as_stream(stream));
+}
+
+GSB_API size_t gsb_linear_fwd_workspace(const gsb_linear* linear) { return linear_fwd_workspace(linear); }
+
+GSB_API gsb_status gsb_linear_fwd(const gsb_linear* linear, void* y, void* preact, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  return linear_fwd(linear, y, preact, workspace, workspace_bytes, as_stream(stream));
+}
+
+GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear) { return linear_bwd_workspace(linear); }
+
+GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, const void* dy, int64_t dy_stride,
+                                  void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  return linear_bwd(linear, preact, dy, dy_stride, dx, dweight, dbias, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // extern "C"

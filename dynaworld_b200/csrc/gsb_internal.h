@@ -160,4 +160,19 @@ gsb_status loss_fwd_bwd(const gsb_loss_options& o, int32_t B, int32_t C, int32_t
                         const float* target, float* loss, float* dpred, void* ws, size_t ws_bytes, cudaStream_t st);
 gsb_status scale_planes(const float* in, const float* scale, float* out, int32_t B, int64_t per, cudaStream_t st);
 
+// Root-mean-square norm, its backward and e4m3 forms (norm.cu).
+gsb_status rms_norm_fwd(const gsb_norm* n, void* y, void* summed, float* rstd, cudaStream_t st);
+gsb_status rms_norm_fp8(const gsb_norm* n, void* codes, float* scales, void* summed, cudaStream_t st);
+gsb_status quantize_rows_fp8(const gsb_norm* n, void* codes, float* scales, cudaStream_t st);
+size_t rms_norm_bwd_workspace(const gsb_norm* n);
+gsb_status rms_norm_bwd(const gsb_norm* n, const float* rstd, const void* dy, int64_t dy_stride, const void* dsummed,
+                        int64_t dsummed_stride, void* dx, void* dweight, void* ws, size_t ws_bytes, cudaStream_t st);
+
+// Matrix product with bias, activation and residual (linear.cu).
+size_t linear_fwd_workspace(const gsb_linear* p);
+gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size_t ws_bytes, cudaStream_t st);
+size_t linear_bwd_workspace(const gsb_linear* p);
+gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, int64_t dy_stride, void* dx,
+                      void* dweight, void* dbias, void* ws, size_t ws_bytes, cudaStream_t st);
+
 }  // namespace gsb

@@ -1,0 +1,149 @@
+"""Matrix product with bias, activation and residual: the layers of the decoder's heads and
+feed-forward blocks.
+
+    y = act(x weight^T + bias) + residual
+
+``linear`` takes float32, bfloat16 or float16 operands and is differentiable; ``linear_fp8`` takes
+e4m3 codes with per-row scales (``rms_norm_fp8``, ``quantize_rows_fp8``) and serves only.  The
+reference's heads (GaussianParameterHeads, src/train/gs_models/blocks.py:84-186) are torch layers;
+these are the B200 kernels for them.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._rows import E4M3, TYPE_CODES, check_device, check_input, check_like, on_device, rows_of
+from .norm import _refuse_grad
+from .render import _stage, _stream
+
+
+def _activation(name: str) -> int:
+    code = _lib.ACTIVATIONS.get(name)
+    if code is None:
+        raise ValueError(f"Unknown activation: {name!r} (one of {', '.join(_lib.ACTIVATIONS)})")
+    return code
+
+
+def _spec(x, weight, bias, residual, act, code, out_code, x_scale=None, weight_scale=None):
+    return _lib.Linear(x.shape[0], weight.shape[0], weight.shape[1], code, out_code, act, 0, x.data_ptr(), x.stride(0),
+                       weight.data_ptr(), weight.stride(0), _lib.ptr(bias), _lib.ptr(residual),
+                       0 if residual is None else residual.stride(0), _lib.ptr(x_scale), _lib.ptr(weight_scale))
+
+
+def _run_forward(spec, rows: int, n: int, dtype, dev, preact) -> torch.Tensor:
+    L = _lib.lib()
+    y = torch.empty((rows, n), dtype=dtype, device=dev)
+    p = ctypes.byref(spec)
+    with on_device(dev), _stage("linear"):
+        ws = torch.empty(L.gsb_linear_fwd_workspace(p), dtype=torch.uint8, device=dev)
+        _lib.check("gsb_linear_fwd", L.gsb_linear_fwd(p, y.data_ptr(), _lib.ptr(preact), ws.data_ptr(), ws.numel(),
+                                                      _stream(dev)))
+    return y
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, code):
+        dev = x.device
+        preact = None
+        if act and any(ctx.needs_input_grad[:3]):
+            preact = torch.empty((x.shape[0], weight.shape[0]), device=dev,
+                                 dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
+        y = _run_forward(_spec(x, weight, bias, residual, act, code, code), x.shape[0], weight.shape[0], x.dtype, dev,
+                         preact)
+        ctx.act, ctx.code = act, code
+        ctx.save_for_backward(x, weight, preact)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, preact = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        if not (need_x or need_w or need_b):
+            return None, None, None, dy if need_r else None, None, None
+        L = _lib.lib()
+        dev = x.device
+        n, k = weight.shape
+        g = rows_of(dy, n)
+        dx = torch.empty((x.shape[0], k), dtype=x.dtype, device=dev) if need_x else None
+        dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need_w else None
+        db = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
+        p = ctypes.byref(_spec(x, weight, None, None, ctx.act, ctx.code, ctx.code))
+        with on_device(dev), _stage("linear_bwd"):
+            ws = torch.empty(L.gsb_linear_bwd_workspace(p), dtype=torch.uint8, device=dev)
+            _lib.check("gsb_linear_bwd", L.gsb_linear_bwd(
+                p, _lib.ptr(preact), g.data_ptr(), g.stride(0), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
+                ws.data_ptr(), ws.numel(), _stream(dev)))
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+def _check_shapes(what, x, weight, bias, residual, dtype):
+    if weight.ndim != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1:
+        raise ValueError(f"{what}: weight must be [n, {x.shape[-1]}], got {tuple(weight.shape)}")
+    n = weight.shape[0]
+    if weight.dtype != x.dtype:
+        raise TypeError(f"{what}: weight must be {x.dtype}, got {weight.dtype}")
+    if weight.device != x.device:
+        raise RuntimeError(f"{what}: weight is on {weight.device}, the input on {x.device}")
+    if bias is not None:
+        check_like(what, "bias", bias, (n,), dtype, x.device)
+    if residual is not None:
+        check_like(what, "residual", residual, (*x.shape[:-1], n), dtype, x.device)
+    return n
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y = act(x weight^T + bias) + residual, x [..., k], weight [n, k], bias [n], residual and y
+    [..., n]; all float32, bfloat16 or float16 of one type.  ``activation``: "none", "relu",
+    "gelu", "gelu_tanh" (its tanh form) or "silu".
+
+    Sums, bias, activation and residual are formed in float and rounded once.  Differentiable once
+    in x, weight, bias and residual.  With an activation the forward keeps x weight^T + bias for the
+    backward (float beside float32 operands, else float16), and the backward rounds
+    dy act'(z) to the operands' type before its two products.  The same inputs give the same bits."""
+    code = check_input("linear", x)
+    act = _activation(activation)
+    n = _check_shapes("linear", x, weight, bias, residual, x.dtype)
+    check_device("linear", x)
+    x2, w2 = rows_of(x, x.shape[-1]), rows_of(weight, weight.shape[1])
+    r2 = None if residual is None else rows_of(residual, n)
+    b = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (b is not None and b.requires_grad)
+                                    or (r2 is not None and r2.requires_grad)):
+        y = _Linear.apply(x2, w2, b, r2, act, code)
+    else:
+        y = _run_forward(_spec(x2, w2, b, r2, act, code, code), x2.shape[0], n, x.dtype, x.device, None)
+    return y.view(*x.shape[:-1], n)
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, *, activation: str = "none", residual: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``linear`` on e4m3 codes: x [..., k] with x_scale [...], weight [n, k] with weight_scale [n]
+    (float32; a value is its code times its row's scale).  bias, residual and y are of ``dtype``.
+    Not differentiable."""
+    if x.dtype != E4M3:
+        raise TypeError(f"linear_fp8 takes {E4M3} codes, got {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError(f"linear_fp8 needs rows of at least one element, got shape {tuple(x.shape)}")
+    out_code = TYPE_CODES.get(dtype)
+    if out_code is None:
+        raise TypeError(f"linear_fp8 gives float32, bfloat16 or float16, not {dtype}")
+    act = _activation(activation)
+    n = _check_shapes("linear_fp8", x, weight, bias, residual, dtype)
+    check_like("linear_fp8", "x_scale", x_scale, x.shape[:-1], torch.float32, x.device)
+    check_like("linear_fp8", "weight_scale", weight_scale, (n,), torch.float32, x.device)
+    check_device("linear_fp8", x)
+    _refuse_grad("linear_fp8", x_scale, weight_scale, bias, residual)
+    x2, w2 = rows_of(x, x.shape[-1]), rows_of(weight, weight.shape[1])
+    r2 = None if residual is None else rows_of(residual, n)
+    b = None if bias is None else bias.contiguous()
+    y = _run_forward(_spec(x2, w2, b, r2, act, _lib.E4M3, out_code, x_scale.contiguous(), weight_scale.contiguous()),
+                     x2.shape[0], n, dtype, x.device, None)
+    return y.view(*x.shape[:-1], n)

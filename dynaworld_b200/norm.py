@@ -1,0 +1,148 @@
+"""Root-mean-square norm of the decoder's token stream, with the residual's addition and an 8-bit
+output, and row-wise 8-bit quantisation.
+
+    h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
+
+The layers in front of the decoder heads (GaussianParameterHeads, src/train/gs_models/blocks.py)
+are torch modules in the reference; these are the B200 kernels for them, next to ``linear``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._rows import E4M3, check_device, check_input, check_like, on_device, rows_of
+from .render import _stage, _stream
+
+
+def _norm(x: torch.Tensor, code: int, eps: float, residual: torch.Tensor | None, weight: torch.Tensor | None):
+    return _lib.Norm(x.shape[0], x.shape[1], code, eps, 0, x.data_ptr(), x.stride(0), _lib.ptr(residual),
+                     0 if residual is None else residual.stride(0), _lib.ptr(weight))
+
+
+def _forward(x, weight, residual, eps, code, need_rstd):
+    """x [rows, dim] -> y, summed (None without a residual), rstd (None unless needed)."""
+    L = _lib.lib()
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    summed = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(x.shape[0], dtype=torch.float32, device=dev) if need_rstd else None
+    with on_device(dev), _stage("rms_norm"):
+        _lib.check("gsb_rms_norm_fwd", L.gsb_rms_norm_fwd(
+            ctypes.byref(_norm(x, code, eps, residual, weight)), y.data_ptr(), _lib.ptr(summed), _lib.ptr(rstd),
+            _stream(dev)))
+    return y, summed, rstd
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, code):
+        y, summed, rstd = _forward(x, weight, residual, eps, code, True)
+        ctx.eps, ctx.code = eps, code
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if summed is None else summed, weight, rstd)
+        return y, summed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dsummed):
+        h, weight, rstd = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:  # only the stream was used
+            return (dsummed if need_x else None, None if not need_w else torch.zeros_like(weight),
+                    dsummed if need_r else None, None, None)
+        L = _lib.lib()
+        dev = h.device
+        dim = h.shape[1]
+        dy = rows_of(dy, dim)
+        dsummed = None if dsummed is None else rows_of(dsummed, dim)
+        dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
+        dw = torch.empty(dim, dtype=weight.dtype, device=dev) if need_w else None
+        norm = _norm(h, ctx.code, ctx.eps, None, weight)
+        with on_device(dev), _stage("rms_norm_bwd"):
+            ws = torch.empty(L.gsb_rms_norm_bwd_workspace(ctypes.byref(norm)), dtype=torch.uint8, device=dev)
+            _lib.check("gsb_rms_norm_bwd", L.gsb_rms_norm_bwd(
+                ctypes.byref(norm), rstd.data_ptr(), dy.data_ptr(), dy.stride(0), _lib.ptr(dsummed),
+                0 if dsummed is None else dsummed.stride(0), dx.data_ptr(), _lib.ptr(dw), ws.data_ptr(), ws.numel(),
+                _stream(dev)))
+        return dx if need_x else None, dw, dx if need_r else None, None, None
+
+
+def _check(what, x, weight, residual, eps):
+    code = check_input(what, x)
+    if weight is not None:
+        check_like(what, "weight", weight, (x.shape[-1],), x.dtype, x.device)
+    if residual is not None:
+        check_like(what, "residual", residual, x.shape, x.dtype, x.device)
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    check_device(what, x)
+    return code
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x + residual.
+
+    x and residual [..., D], weight [D], all float32, bfloat16 or float16 of one type.  Returns y,
+    or with a residual the pair (y, h): h is the new residual stream.  The sum, the statistics and
+    the product are formed in float; y and h are rounded once.  Differentiable in x, weight and
+    residual (once; the backward uses h as returned); the weight gradient is the same on every run."""
+    code = _check("rms_norm", x, weight, residual, eps)
+    dim = x.shape[-1]
+    x2 = rows_of(x, dim)
+    r2 = None if residual is None else rows_of(residual, dim)
+    w = weight.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (residual is not None and residual.requires_grad)):
+        y, h = _RmsNorm.apply(x2, w, r2, float(eps), code)
+    else:
+        y, h, _ = _forward(x2, w, r2, float(eps), code, False)
+    y = y.view(x.shape)
+    return y if residual is None else (y, h.view(x.shape))
+
+
+def _refuse_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what} is not differentiable; call it under torch.no_grad() or detach its inputs.")
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """``rms_norm`` with y in 8 bits for ``linear_fp8``: (codes [..., D] float8_e4m3fn, scale [...]
+    float32), and h as the third value with a residual.  Per row top = max(max |y|, 1e-30),
+    scale = top / 448 and code = e4m3(y * (448 / top)), from y in float.  A row with a NaN or an
+    infinity stands for NaN.  Not differentiable."""
+    code = _check("rms_norm_fp8", x, weight, residual, eps)
+    _refuse_grad("rms_norm_fp8", x, weight, residual)
+    L = _lib.lib()
+    dev, dim = x.device, x.shape[-1]
+    x2 = rows_of(x, dim)
+    r2 = None if residual is None else rows_of(residual, dim)
+    w = weight.contiguous()
+    q = torch.empty(x.shape, dtype=E4M3, device=dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    with on_device(dev), _stage("rms_norm_fp8"):
+        _lib.check("gsb_rms_norm_fp8", L.gsb_rms_norm_fp8(
+            ctypes.byref(_norm(x2, code, float(eps), r2, w)), q.data_ptr(), scale.data_ptr(), _lib.ptr(h),
+            _stream(dev)))
+    return (q, scale) if residual is None else (q, scale, h)
+
+
+def quantize_rows_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., D] in 8 bits with one scale per row: (codes float8_e4m3fn, scale [...] float32), as
+    ``rms_norm_fp8`` quantises its y.  For ``linear_fp8``: weights once, the activations between two
+    8-bit products every step.  Not differentiable."""
+    code = _check("quantize_rows_fp8", x, None, None, 0.0)
+    _refuse_grad("quantize_rows_fp8", x)
+    L = _lib.lib()
+    dev, dim = x.device, x.shape[-1]
+    x2 = rows_of(x, dim)
+    q = torch.empty(x.shape, dtype=E4M3, device=dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    with on_device(dev), _stage("quantize_rows_fp8"):
+        _lib.check("gsb_quantize_rows_fp8", L.gsb_quantize_rows_fp8(
+            ctypes.byref(_norm(x2, code, 0.0, None, None)), q.data_ptr(), scale.data_ptr(), _stream(dev)))
+    return q, scale

@@ -383,6 +383,94 @@ GSB_API gsb_status gsb_splats2d_preprocess_bwd(const gsb_splats2d* splats, const
                                                const float* grad2d, gsb_splats2d_grads* grads,
                                                void* stream);
 
+/* ---- token side: the operators that turn decoder tokens into raw head outputs -------------- */
+/* No counterpart among the reference's kernels: its heads (GaussianParameterHeads,
+   gs_models/blocks.py:84-186) are torch layers.  Element types: */
+#define GSB_F32 0
+#define GSB_BF16 1
+#define GSB_F16 2
+#define GSB_E4M3 3 /* 8-bit codes: a value is code * scale of its row */
+
+/* Rows [rows, dim] of `dtype` (F32, BF16 or F16).  Strides count elements between rows; a row's
+   elements are adjacent.  Outputs are contiguous.  0 <= rows <= 2^31 - 1. */
+typedef struct gsb_norm {
+  int64_t rows;
+  int32_t dim;
+  int32_t dtype;
+  float eps;
+  int32_t reserved;
+  const void* x;
+  int64_t x_stride;
+  const void* residual; /* added to x first; or NULL */
+  int64_t residual_stride;
+  const void* weight;   /* [dim] */
+} gsb_norm;
+
+/* h = x + residual, rstd = 1 / sqrt(mean(h^2) + eps), y = h rstd weight.  h is formed and
+   normalised in float; `summed` (or NULL; written only with a residual) gets it in `dtype`, `rstd`
+   (or NULL) [rows] is what the backward reads. */
+GSB_API gsb_status gsb_rms_norm_fwd(const gsb_norm* norm, void* y, void* summed, float* rstd,
+                                    void* stream);
+GSB_API size_t gsb_rms_norm_bwd_workspace(const gsb_norm* norm);
+/* norm->x is h (x, or `summed` where there was a residual); dy and dsummed (or NULL) the gradients
+   of y and summed.  dx is the gradient of x and of the residual.  dweight may be NULL.  The same
+   inputs give the same bits. */
+GSB_API gsb_status gsb_rms_norm_bwd(const gsb_norm* norm, const float* rstd, const void* dy,
+                                    int64_t dy_stride, const void* dsummed, int64_t dsummed_stride,
+                                    void* dx, void* dweight, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+/* The norm with y as e4m3 codes and one scale per row: top = max(max |y|, 1e-30),
+   scale = top / 448, code = e4m3(y * (448 / top)), y in float.  A row with a NaN or infinity
+   stands for NaN throughout. */
+GSB_API gsb_status gsb_rms_norm_fp8(const gsb_norm* norm, void* codes, float* scales, void* summed,
+                                    void* stream);
+/* The same quantisation of x itself (weight, residual and eps are not read). */
+GSB_API gsb_status gsb_quantize_rows_fp8(const gsb_norm* rows, void* codes, float* scales,
+                                         void* stream);
+
+#define GSB_ACT_NONE 0
+#define GSB_ACT_RELU 1
+#define GSB_ACT_GELU 2      /* z Phi(z) */
+#define GSB_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+#define GSB_ACT_SILU 4      /* z / (1 + exp(-z)) */
+
+/* y = act(x weight^T + bias) + residual, x [m,k], weight [n,k], y [m,n], sums in float.
+   dtype is the type of x and weight; y, bias and residual are of out_dtype, which equals dtype
+   except for E4M3 operands (then F32, BF16 or F16, and x_scale [m] and weight_scale [n] multiply
+   the product).  Strides as in gsb_norm.  0 <= m <= 2^31 - 1; 1 <= n, k <= 2^24. */
+typedef struct gsb_linear {
+  int64_t m;
+  int32_t n;
+  int32_t k;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t activation; /* GSB_ACT_* */
+  int32_t reserved;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;     /* [n] or NULL */
+  const void* residual; /* [m,n] or NULL */
+  int64_t residual_stride;
+  const float* x_scale;
+  const float* weight_scale;
+} gsb_linear;
+
+GSB_API size_t gsb_linear_fwd_workspace(const gsb_linear* linear);
+/* preact (or NULL) [m,n] keeps z = x weight^T + bias for the backward: float for F32 operands, fp16
+   saturated at its largest value for 16-bit ones (every activation is flat or linear there). */
+GSB_API gsb_status gsb_linear_fwd(const gsb_linear* linear, void* y, void* preact, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear);
+/* dz = dy act'(z), dx = dz weight, dweight = dz^T x, dbias = the column sums of dz; outputs that
+   are NULL are not computed, all are contiguous and of dtype (not E4M3).  preact is read unless
+   the activation is NONE.  dz is rounded to dtype before the two products (dbias sums it in
+   float).  The residual's gradient is dy.  The same inputs give the same bits. */
+GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, const void* dy,
+                                  int64_t dy_stride, void* dx, void* dweight, void* dbias,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- utility: the library's radix sort on its own (tests, benchmarks) --------------------- */
 GSB_API size_t gsb_radix_sort_workspace(uint32_t n, int key_bytes, int with_values);
 /* Stable LSD sort of n keys by bits [bit_lo, bit_hi); keys are uint32 (key_bytes 4) or uint64

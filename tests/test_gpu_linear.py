@@ -1,0 +1,366 @@
+"""linear and linear_fp8 on the GPU against their formulas in 64 bits.
+
+Bounds.  half(t) is half a relative step of the type t.  A product's sum over K float terms, added in
+any order with additions that truncate (an error of at most 2^-23 of the partial sum each), is within
+K 2^-23 sum |x w|.  float32 operands of the tensor-core path are split into three bf16 parts; the
+parts that it does not multiply are below 2^-25 |x w| each, which the same bound's first term covers.
+The activations' slopes are at most 1.13 and their second derivatives at most 1.13, |z act''| at most
+1.1; the functions themselves are evaluated within 2^-20 |z| (+ 2^-24).  The kept z has half(float16)
+relative error beside 16-bit operands; dz is rounded to the operands' type.  Within its error of 0 the
+slope of relu is either side's."""
+import math
+
+import pytest
+import torch
+
+from dynaworld_b200 import _lib
+from dynaworld_b200.linear import linear, linear_fp8
+from dynaworld_b200.norm import quantize_rows_fp8
+from gpu_helpers import DEV
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -23
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = list(_lib.ACTIVATIONS)
+E4M3 = torch.float8_e4m3fn
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def act64(z, kind):
+    if kind == "relu":
+        return z.clamp_min(0), (z > 0).double()
+    if kind == "gelu":
+        c = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if kind == "gelu_tanh":
+        s = torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+        return z * s, s + z * s * (1 - s) * 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    return z, torch.ones_like(z)
+
+
+def make(m, k, n, t, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (scale * torch.randn(m, k, generator=g)).to(t)
+    w = (torch.randn(n, k, generator=g) / math.sqrt(k)).to(t)
+    b = (0.5 * torch.randn(n, generator=g)).to(t)
+    r = torch.randn(m, n, generator=g).to(t)
+    dy = torch.randn(m, n, generator=g).to(t)
+    return [v.to(DEV) for v in (x, w, b, r, dy)]
+
+
+def within(got, ref, bound, what=""):
+    assert got.shape == ref.shape
+    over = (got.double() - ref).abs() - bound
+    assert bool((over <= 0).all()), f"{what}: {over.max().item():.3e} past the bound"
+
+
+def check(x, w, b, r, dy, act, grads=True):
+    t = x.dtype
+    n, k = w.shape
+    X, W = x.detach().double().reshape(-1, k), w.detach().double()
+    leaves = [None if v is None else v.detach().clone().requires_grad_(grads) for v in (x, w, b, r)]
+    y = linear(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3])
+    z = X @ W.T
+    mag = X.abs() @ W.abs().T
+    if b is not None:
+        z = z + b.double()
+        mag = mag + b.double().abs()
+    dz_fwd = (k + 2) * U * mag
+    a, slope = act64(z, act)
+    ref = a if r is None else a + r.double().reshape(-1, n)
+    eval_err = z.abs() * 2.0 ** -20 + 2.0 ** -24
+    bound = ref.abs() * half(t) * (1 + 1e-3) + 1.13 * dz_fwd + eval_err + tiny(t)
+    if r is not None:
+        bound = bound + r.double().reshape(-1, n).abs() * U
+    within(y.reshape(-1, n), ref, bound, "y")
+    if not grads:
+        return y
+    used = [v for v in leaves if v is not None]
+    got = dict(zip([i for i, v in enumerate(leaves) if v is not None], torch.autograd.grad(y, used, dy)))
+    G = dy.double().reshape(-1, n)
+    m = G.shape[0]
+    dz = G * slope
+    err = dz.abs() * half(t) + tiny(t)
+    if act != "none":
+        kept = 0.0 if t == torch.float32 else 1.1 * half(torch.float16) + 2.0 ** -24
+        err = err + G.abs() * (1.13 * dz_fwd + kept + 2.0 ** -20)
+        if act == "relu":
+            near = z.abs() <= dz_fwd + z.abs() * half(torch.float16) + 2.0 ** -24
+            err = torch.where(near, G.abs() * (1 + half(t)), dz.abs() * half(t) + tiny(t))
+    else:
+        err = torch.zeros_like(dz)
+    whole = dz.abs() + err
+    dx = dz @ W
+    within(got[0].reshape(-1, k), dx, dx.abs() * half(t) + err @ W.abs() + (n + 2) * U * (whole @ W.abs()) + tiny(t),
+           "dx")
+    dw = dz.T @ X
+    within(got[1], dw, dw.abs() * half(t) + err.T @ X.abs() + (m + 2) * U * (whole.T @ X.abs()) + tiny(t), "dw")
+    if b is not None:
+        db = dz.sum(0)
+        within(got[2], db, db.abs() * half(t) + err.sum(0) + (m + 2) * U * whole.sum(0) + tiny(t), "db")
+    if r is not None:
+        assert torch.equal(got[3].reshape(-1, n), dy.reshape(-1, n))
+    return y
+
+
+# one token, few tokens, tile edges and one past them, odd widths, long sums, widths below a vector
+SHAPES = [(1, 1, 1), (1, 64, 128), (1, 1000, 77), (2, 515, 24), (8, 256, 513), (9, 64, 40), (16, 2048, 96),
+          (63, 100, 300), (64, 64, 64), (127, 129, 255), (128, 128, 256), (129, 136, 264), (300, 771, 1285),
+          (513, 72, 56), (1025, 512, 130), (2500, 40, 3), (5, 4096, 16), (257, 1037, 9), (700, 520, 1032)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_linear_and_gradients(m, k, n, t):
+    x, w, b, r, dy = make(m, k, n, t, seed=m + n)
+    act = ACTS[(m + k + n) % len(ACTS)]
+    check(x, w, b if (m + n) % 3 else None, r if m % 2 else None, dy, act)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [3, 200])
+def test_activations(m, act, t):
+    """Pre-activations over the whole range of the functions, small and saturated."""
+    x, w, b, r, dy = make(m, 96, 160, t, seed=5, scale=4.0)
+    check(x, w, b, None, dy, act)
+    check(x, w, None, r, dy, act)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_strides_and_leading_dimensions(t):
+    """Rows of wider tensors whose starts are aligned to 16 bytes or not, leading dimensions, a
+    transposed input and weight, an expanded gradient."""
+    x, w, b, r, dy = make(130, 64, 72, t)
+    for first, width in ((0, 80), (16, 96), (1, 67)):
+        wide_x = torch.full((130, width), float("nan"), dtype=t, device=DEV)
+        wide_x[:, first:first + 64] = x
+        wide_w = torch.full((72, width), float("nan"), dtype=t, device=DEV)
+        wide_w[:, first:first + 64] = w
+        wide_r = torch.full((130, width + 72), float("nan"), dtype=t, device=DEV)
+        wide_r[:, first:first + 72] = r
+        got = linear(wide_x[:, first:first + 64], wide_w[:, first:first + 64], b, activation="silu",
+                     residual=wide_r[:, first:first + 72])
+        X, W = x.double(), w.double()
+        z = X @ W.T + b.double()
+        ref = act64(z, "silu")[0] + r.double()
+        mag = X.abs() @ W.abs().T + b.double().abs()
+        within(got, ref, ref.abs() * half(t) * 1.001 + 70 * U * mag + z.abs() * 2.0 ** -20 + 2.0 ** -22)
+        leaf = wide_x.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(linear(leaf[:, first:first + 64], w), leaf, dy)
+        ref = dy.double() @ W
+        within(g[:, first:first + 64], ref, ref.abs() * half(t) + 74 * U * (dy.double().abs() @ W.abs()) + tiny(t))
+        assert bool((g[:, :first] == 0).all()) and bool((g[:, first + 64:] == 0).all())
+    y = linear(x, w, b)
+    assert torch.equal(linear(x.view(2, 65, 64), w, b).view(130, 72), y)
+    assert torch.equal(linear(x.t().contiguous().t(), w.t().contiguous().t(), b), y)
+    one = linear(x[7], w, b)
+    assert one.shape == (72,)
+    leaf, leaf2 = (x.clone().requires_grad_(True) for _ in range(2))
+    linear(leaf, w, b, activation="gelu").sum().backward()
+    linear(leaf2, w, b, activation="gelu").backward(torch.ones_like(y))
+    assert torch.equal(leaf.grad, leaf2.grad)
+    # rows that are one row repeated
+    rep = x[:1].expand(130, 64)
+    assert torch.equal(linear(rep, w, b)[5], linear(rep, w, b)[77])
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_nothing_to_do(t):
+    w = torch.ones(24, 16, dtype=t, device=DEV, requires_grad=True)
+    b = torch.ones(24, dtype=t, device=DEV, requires_grad=True)
+    x = torch.empty(0, 16, dtype=t, device=DEV, requires_grad=True)
+    y = linear(x, w, b, activation="gelu")
+    assert y.shape == (0, 24)
+    y.sum().backward()
+    assert x.grad.shape == (0, 16) and bool((w.grad == 0).all()) and bool((b.grad == 0).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_only_some_gradients(t):
+    x, w, b, r, dy = make(200, 72, 88, t)
+    full = [v.clone().requires_grad_(True) for v in (x, w, b, r)]
+    ref = torch.autograd.grad(linear(full[0], full[1], full[2], activation="silu", residual=full[3]), full, dy)
+    for i in range(4):
+        part = [v.clone().requires_grad_(j == i) for j, v in enumerate((x, w, b, r))]
+        (g,) = torch.autograd.grad(linear(part[0], part[1], part[2], activation="silu", residual=part[3]), part[i], dy)
+        assert torch.equal(g, ref[i])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [4, 300])
+def test_nonfinite_rows_stay_in_their_row(m, t):
+    x, w, b, r, dy = make(m, 128, 96, t)
+    y = linear(x, w, b, activation="silu")
+    x2 = x.clone()
+    x2[2, 5] = float("nan")
+    x2[3, 6] = float("inf")
+    y2 = linear(x2, w, b, activation="silu")
+    assert bool(y2[2].isnan().all()) and not bool(torch.isfinite(y2[3]).all())
+    keep = [i for i in range(m) if i not in (2, 3)]
+    assert torch.equal(y2[keep], y[keep])
+
+
+def test_large_values_in_float32():
+    """Values near the type's largest, whose bf16 rounding would overflow."""
+    x = torch.full((130, 64), 0.0, device=DEV)
+    x[:, 0] = torch.finfo(torch.float32).max
+    w = torch.zeros(70, 64, device=DEV)
+    w[:, 0] = 0.5
+    y = linear(x, w)
+    ref = x.double() @ w.double().T
+    within(y, ref, ref * 66 * U)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_saturated_preactivations(t):
+    """z beyond fp16's range: the kept z saturates and the slope there is 1 or 0."""
+    x = torch.full((140, 64), 200.0, dtype=t, device=DEV)
+    x[70:] = -200.0
+    w = torch.full((32, 64), 60.0 if t == torch.float16 else 100.0, dtype=t, device=DEV)
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        leaf = (x / 64).requires_grad_(True) if t == torch.float16 else x.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(linear(leaf, w, activation=act).float().sum(), leaf)
+        assert bool((g[70:] == 0).all())
+        assert bool((g[:70].float() == 32 * float(w[0, 0])).all())
+
+
+def test_same_bits_every_run():
+    for t in TYPES:
+        x, w, b, r, dy = make(3000, 136, 72, t)
+
+        def once():
+            leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+            y = linear(leaves[0], leaves[1], leaves[2], activation="gelu")
+            return [y, *torch.autograd.grad(y, leaves, dy)]
+        for a, c in zip(once(), once()):
+            assert torch.equal(a, c)
+
+
+def test_gradient_against_differences():
+    """Central differences in 64 bits of the formula against the kernels' 32-bit gradients."""
+    x, w, b, r, dy = make(3, 24, 10, torch.float32, seed=9)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        got = torch.autograd.grad(linear(leaves[0], leaves[1], leaves[2], activation=act), leaves, dy)
+
+        def f(parts):
+            return (act64(parts[0] @ parts[1].T + parts[2], act)[0] * dy.double()).sum()
+
+        base = [v.double() for v in (x, w, b)]
+        step = 1e-4
+        for i, idx in ((0, (1, 5)), (0, (2, 23)), (1, (9, 0)), (1, (4, 13)), (2, (7,))):
+            plus, minus = [v.clone() for v in base], [v.clone() for v in base]
+            plus[i][idx] += step
+            minus[i][idx] -= step
+            assert abs(float((f(plus) - f(minus)) / (2 * step)) - float(got[i][idx])) < 2e-5
+
+
+# ---- 8-bit operands ----
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_fp8(m, k, n, t):
+    x, w, b, r, _ = make(m, k, n, torch.float32, seed=m + k)
+    b, r = b.to(t), r.to(t)
+    xq, xs = quantize_rows_fp8(x)
+    wq, ws = quantize_rows_fp8(w)
+    act = ACTS[(m + n) % len(ACTS)]
+    y = linear_fp8(xq, xs, wq, ws, b, activation=act, residual=r, dtype=t)
+    X, W = xq.double() * xs.double()[:, None], wq.double() * ws.double()[:, None]
+    z = X @ W.T + b.double()
+    mag = X.abs() @ W.abs().T + b.double().abs()
+    ref = act64(z, act)[0] + r.double()
+    within(y, ref, ref.abs() * half(t) * 1.001 + 1.13 * (k + 4) * U * mag + z.abs() * 2.0 ** -20 + 2.0 ** -24 +
+           r.double().abs() * U + tiny(t))
+
+
+def test_fp8_strides_and_dimensions():
+    x, w, b, r, _ = make(130, 128, 96, torch.float32)
+    xq, xs = quantize_rows_fp8(x)
+    wq, ws = quantize_rows_fp8(w)
+    ref = linear_fp8(xq, xs, wq, ws)
+    assert ref.dtype == torch.bfloat16
+    assert torch.equal(linear_fp8(xq.view(2, 65, 128), xs.view(2, 65), wq, ws).view(130, 96), ref)
+    for first, width in ((16, 160), (3, 135)):
+        wide = torch.zeros(130, width, dtype=torch.uint8, device=DEV)
+        wide[:, first:first + 128] = xq.view(torch.uint8)
+        got = linear_fp8(wide.view(E4M3)[:, first:first + 128], xs, wq, ws)
+        assert torch.equal(got, ref)
+    one = linear_fp8(xq[3], xs[3], wq, ws)
+    assert one.shape == (96,)
+    assert linear_fp8(xq[:0], xs[:0], wq, ws).shape == (0, 96)
+
+
+def test_refusals_on_the_gpu():
+    x, w, b, r, dy = make(4, 16, 8, torch.float32)
+    xq, xs = quantize_rows_fp8(x)
+    wq, ws = quantize_rows_fp8(w)
+    with pytest.raises(NotImplementedError, match="not differentiable"):
+        linear_fp8(xq, xs, wq, ws, b.requires_grad_(True), dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="weight is on cpu"):
+        linear(x, w.cpu())
+    with pytest.raises(RuntimeError, match="bias is on cpu"):
+        linear(x, w, b.detach().cpu())
+    leaf = x.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(linear(leaf, w, activation="gelu").sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+# ---- streams and graphs ----
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_other_stream(t):
+    x, w, b, r, dy = make(260, 200, 136, t)
+    ref = linear(x, w, b, activation="gelu", residual=r)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        y = linear(x, w, b, activation="gelu", residual=r)
+    side.synchronize()
+    assert torch.equal(y, ref)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [1, 300])
+def test_two_captured_graphs_replayed_together(m, t):
+    """Two graphs of the forward and backward with workspaces of their own, replayed on two streams."""
+    sets = [make(m, 264, 144, t, seed=s) for s in (1, 2)]
+    graphs, outs, refs, kept = [], [], [], []
+    for x, w, b, r, dy in sets:
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        kept.append(leaves)  # a graph reads its inputs where they were
+
+        def step(leaves=leaves, dy=dy):
+            y = linear(leaves[0], leaves[1], leaves[2], activation="silu")
+            return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+        refs.append([v.clone() for v in step()])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, refs):
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)

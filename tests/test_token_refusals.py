@@ -1,0 +1,107 @@
+"""What the token-side operators refuse, before any kernel: on the host, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from dynaworld_b200 import _lib, build
+from dynaworld_b200.linear import linear, linear_fp8
+from dynaworld_b200.norm import quantize_rows_fp8, rms_norm, rms_norm_fp8
+
+E4M3 = torch.float8_e4m3fn
+F = torch.zeros
+
+
+@pytest.mark.parametrize("error, match, call", [
+    (TypeError, "float32, bfloat16 or float16", lambda: linear(F(2, 4, dtype=torch.float64), F(3, 4))),
+    (TypeError, "float32, bfloat16 or float16", lambda: linear(F(2, 4, dtype=torch.int32), F(3, 4))),
+    (ValueError, "at least one element", lambda: linear(F(2, 0), F(3, 0))),
+    (ValueError, "at least one element", lambda: linear(torch.tensor(1.0), F(3, 1))),
+    (ValueError, "weight must be", lambda: linear(F(2, 4), F(3, 5))),
+    (ValueError, "weight must be", lambda: linear(F(2, 4), F(4))),
+    (ValueError, "weight must be", lambda: linear(F(2, 4), F(0, 4))),
+    (TypeError, "weight must be", lambda: linear(F(2, 4), F(3, 4, dtype=torch.bfloat16))),
+    (ValueError, "bias must have shape", lambda: linear(F(2, 4), F(3, 4), F(4))),
+    (TypeError, "bias must be", lambda: linear(F(2, 4), F(3, 4), F(3, dtype=torch.float16))),
+    (ValueError, "residual must have shape", lambda: linear(F(2, 4), F(3, 4), residual=F(3))),
+    (ValueError, "Unknown activation", lambda: linear(F(2, 4), F(3, 4), activation="swish")),
+    (RuntimeError, "CUDA devices only", lambda: linear(F(2, 4), F(3, 4))),
+    (TypeError, "takes torch.float8_e4m3fn", lambda: linear_fp8(F(2, 4), F(2), F(3, 4), F(3))),
+    (TypeError, "weight must be", lambda: linear_fp8(F(2, 4, dtype=E4M3), F(2), F(3, 4), F(3))),
+    (ValueError, "x_scale must have shape",
+     lambda: linear_fp8(F(2, 4, dtype=E4M3), F(3), F(3, 4, dtype=E4M3), F(3))),
+    (TypeError, "weight_scale must be",
+     lambda: linear_fp8(F(2, 4, dtype=E4M3), F(2), F(3, 4, dtype=E4M3), F(3, dtype=torch.float16))),
+    (TypeError, "gives float32, bfloat16 or float16",
+     lambda: linear_fp8(F(2, 4, dtype=E4M3), F(2), F(3, 4, dtype=E4M3), F(3), dtype=torch.float64)),
+    (TypeError, "bias must be torch.bfloat16",
+     lambda: linear_fp8(F(2, 4, dtype=E4M3), F(2), F(3, 4, dtype=E4M3), F(3), F(3))),
+    (RuntimeError, "CUDA devices only", lambda: linear_fp8(F(2, 4, dtype=E4M3), F(2), F(3, 4, dtype=E4M3), F(3))),
+    (TypeError, "float32, bfloat16 or float16", lambda: rms_norm(F(2, 4, dtype=E4M3), F(4))),
+    (ValueError, "weight must have shape", lambda: rms_norm(F(2, 4), F(5))),
+    (TypeError, "weight must be", lambda: rms_norm(F(2, 4), F(4, dtype=torch.bfloat16))),
+    (ValueError, "residual must have shape", lambda: rms_norm(F(2, 4), F(4), residual=F(4))),
+    (ValueError, "eps must not be negative", lambda: rms_norm(F(2, 4), F(4), eps=-1.0)),
+    (ValueError, "eps must not be negative", lambda: rms_norm(F(2, 4), F(4), eps=float("nan"))),
+    (RuntimeError, "CUDA devices only", lambda: rms_norm(F(2, 4), F(4))),
+    (RuntimeError, "CUDA devices only", lambda: rms_norm_fp8(F(2, 4), F(4))),
+    (ValueError, "at least one element", lambda: quantize_rows_fp8(F(2, 0))),
+    (RuntimeError, "CUDA devices only", lambda: quantize_rows_fp8(F(2, 4))),
+])
+def test_refused(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
+
+
+def test_struct_sizes_match_header():
+    assert ctypes.sizeof(_lib.Norm) == 8 + 4 * 4 + 5 * 8
+    assert ctypes.sizeof(_lib.Linear) == 8 + 6 * 4 + 9 * 8
+
+
+def test_entry_points_refuse_before_a_launch(lib):
+    """Bad sizes, types and missing pointers give a status on the host; no rows are no work."""
+    n = _lib.Norm(rows=4, dim=8, dtype=_lib.F32, eps=1e-6, x=256, x_stride=8, weight=256)
+    b = ctypes.byref(n)
+    assert lib.gsb_rms_norm_fwd(None, 256, None, None, None) == 7
+    assert lib.gsb_rms_norm_fwd(b, None, None, None, None) == 7
+    assert lib.gsb_rms_norm_fp8(b, 256, None, None, None) == 7
+    assert lib.gsb_quantize_rows_fp8(b, None, 256, None) == 7
+    assert lib.gsb_rms_norm_bwd(b, 256, 256, 8, None, 0, 256, None, 256, 16, None) == 2
+    assert lib.gsb_rms_norm_bwd(b, None, 256, 8, None, 0, 256, None, 256, 1 << 20, None) == 7
+    for field, bad, status in (("dim", 0, 1), ("rows", -1, 1), ("rows", 1 << 31, 1), ("dtype", _lib.E4M3, 7),
+                               ("eps", -1.0, 7), ("weight", None, 7), ("x", None, 7)):
+        keep = getattr(n, field)
+        setattr(n, field, bad)
+        assert lib.gsb_rms_norm_fwd(b, 256, None, None, None) == status, field
+        setattr(n, field, keep)
+    n.rows = 0
+    assert lib.gsb_rms_norm_fwd(b, 256, None, None, None) == 0
+
+    p = _lib.Linear(m=4, n=8, k=8, dtype=_lib.BF16, out_dtype=_lib.BF16, x=256, x_stride=8, weight=256,
+                    weight_stride=8)
+    b = ctypes.byref(p)
+    big = 1 << 30
+    assert lib.gsb_linear_fwd(None, 256, None, 256, big, None) == 7
+    assert lib.gsb_linear_fwd(b, None, None, 256, big, None) == 7
+    for field, bad, status in (("n", 0, 1), ("k", 0, 1), ("m", -1, 1), ("m", 1 << 31, 1), ("n", (1 << 24) + 1, 1),
+                               ("dtype", 4, 7), ("dtype", _lib.F16, 7), ("dtype", _lib.E4M3, 7),
+                               ("out_dtype", _lib.E4M3, 7), ("activation", 5, 7), ("activation", -1, 7),
+                               ("weight", None, 7), ("x", None, 7)):
+        keep = getattr(p, field)
+        setattr(p, field, bad)
+        assert lib.gsb_linear_fwd(b, 256, None, 256, big, None) == status, field
+        setattr(p, field, keep)
+    assert lib.gsb_linear_bwd(b, None, None, 8, 256, 256, 256, 256, big, None) == 7
+    assert lib.gsb_linear_bwd(b, None, 256, 8, 256, 256, 256, 256, 16, None) == 2
+    p.activation = 2
+    assert lib.gsb_linear_bwd(b, None, 256, 8, 256, 256, 256, 256, big, None) == 7  # no pre-activation
+    p.dtype = _lib.E4M3
+    assert lib.gsb_linear_bwd(b, 256, 256, 8, 256, 256, 256, 256, big, None) == 7  # serving only
+    p.m, p.dtype, p.x = 0, _lib.BF16, None
+    assert lib.gsb_linear_fwd(b, 256, None, 256, big, None) == 0
