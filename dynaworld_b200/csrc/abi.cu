@@ -615,12 +615,16 @@ GSB_API gsb_status gsb_linear_fwd(const gsb_linear* linear, void* y, void* preac
   return linear_fwd(linear, y, preact, workspace, workspace_bytes, as_stream(stream));
 }
 
-GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear) { return linear_bwd_workspace(linear); }
+GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear, const void* dy, int64_t dy_stride) {
+  return linear_bwd_workspace(linear, dy, dy_stride);
+}
 
 GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, const void* dy, int64_t dy_stride,
                                   void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
                                   void* stream) {
   return linear_bwd(linear, preact, dy, dy_stride, dx, dweight, dbias, workspace, workspace_bytes, as_stream(stream));
 }
+
+GSB_API gsb_status gsb_linear_status(void) { return linear_status(); }
 
 }  // extern "C"

@@ -1,208 +1,402 @@
 // y = act(x w^T + b) + r and its backward.
-#include "activation.cuh"
-#include "gsb_common.cuh"
-#include "gsb_internal.h"
-#include "token_types.cuh"
+#include "linear_parts.cuh"
 
 namespace gsb {
 
 namespace {
 
-// C(i, j) = sum_k A(i, k) B(j, k) with any strides, A(i, k) = a[i a_i + k a_k].
-struct Operands {
-  const void* a;
-  int64_t a_i, a_k;
-  const void* b;
-  int64_t b_j, b_k;
-  int64_t m, n, k;
-};
+constexpr int64_t kFewRows = 8;
 
-struct Epilogue {
-  const float* row_scale;
-  const float* col_scale;
-  const void* bias;
-  const void* res;
-  int64_t res_stride;
-  void* preact;
-  void* out;
-  int64_t out_stride;
-};
-
-constexpr float kHalfMax = 65504.0f;
-
-// The pre-activation kept for the backward: float beside float operands, else fp16 saturated at
-// its largest value.  fp16 and not bf16: its 11 bits keep the slope's error (at most 2^-11 |z|
-// act'') an eighth of the rounding that dz gets, and beyond +-65504 every slope is constant.
-__device__ __forceinline__ void put_preact(float* p, float z) { *p = z; }
-__device__ __forceinline__ void put_preact(f16* p, float z) {
-  *p = __float2half_rn(z != z ? z : fminf(fmaxf(z, -kHalfMax), kHalfMax));
-}
-
-template <typename T>
-struct PreactOf { using type = f16; };
-template <>
-struct PreactOf<float> { using type = float; };
-
-constexpr int kTile = 64, kDepth = 16;
-
-template <typename T, typename O, int ACT>
-__global__ void __launch_bounds__(256) product_kernel(Operands p, Epilogue e) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int64_t i0 = int64_t(blockIdx.x) * kTile;
-  const int64_t j0 = int64_t(blockIdx.y) * kTile;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
-    for (int s = threadIdx.x; s < kTile * kDepth; s += 256) {
-      // the unit-stride index runs fastest over the threads
-      const int ai = p.a_k == 1 ? s / kDepth : s % kTile, ak = p.a_k == 1 ? s % kDepth : s / kTile;
-      const bool a_in = i0 + ai < p.m && k0 + ak < p.k;
-      sa[ak][ai] = a_in ? to_f32(a[(i0 + ai) * p.a_i + (k0 + ak) * p.a_k]) : 0.0f;
-      const int bj = p.b_k == 1 ? s / kDepth : s % kTile, bk = p.b_k == 1 ? s % kDepth : s / kTile;
-      const bool b_in = j0 + bj < p.n && k0 + bk < p.k;
-      sb[bk][bj] = b_in ? to_f32(b[(j0 + bj) * p.b_j + (k0 + bk) * p.b_k]) : 0.0f;
+// ---- few rows: bound by the weights' bytes ----------------------------------------------------
+// A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
+// that the weights are read once; the tokens come from L1.  Float operands stay float.
+template <typename T, typename O, int V, int ROWS, int C>
+__global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, int m,
+                                                       int n, int k, Epilogue e) {
+  const int lane = threadIdx.x & 31;
+  const int j0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * C;
+  if (j0 >= n) return;
+  float acc[ROWS][C];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[r][c] = 0.0f;
+  const T* wr[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) wr[c] = w + int64_t(min(j0 + c, n - 1)) * w_stride;
+#pragma unroll(C* ROWS <= 4 ? 4 : 2)
+  for (int i = lane * V; i < k; i += 32 * V) {
+    float wv[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c) load_f32<T, V>(wr[c] + i, wv[c]);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      float xv[V];
+      load_f32<T, V>(x + int64_t(min(r, m - 1)) * x_stride + i, xv);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int u = 0; u < V; ++u) acc[r][c] = fmaf(xv[u], wv[c][u], acc[r][c]);
     }
-    __syncthreads();
+  }
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-      float av[4], bv[4];
+  for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        av[u] = sa[k][ty + 16 * u];
-        bv[u] = sb[k][tx + 16 * u];
+    for (int c = 0; c < C; ++c) {
+      const float s = warp_sum(acc[r][c]);
+      if (lane == r * C + c && r < m && j0 + c < n) {
+        float z[1] = {s};
+        finish<O, 1>(e, n, r, j0 + c, z);
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(av[u], bv[v], acc[u][v]);
     }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = i0 + ty + 16 * u;
-    if (i >= p.m) continue;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int64_t j = j0 + tx + 16 * v;
-      if (j >= p.n) continue;
-      float z = acc[u][v];
-      if (e.row_scale) z *= e.row_scale[i] * e.col_scale[j];
-      if (e.bias) z += to_f32(static_cast<const O*>(e.bias)[j]);
-      if (e.preact) put_preact(static_cast<typename PreactOf<O>::type*>(e.preact) + i * p.n + j, z);
-      float y = act_value<ACT>(z);
-      if (e.res) y += to_f32(static_cast<const O*>(e.res)[i * e.res_stride + j]);
-      static_cast<O*>(e.out)[i * e.out_stride + j] = from_f32<O>(y);
-    }
-  }
 }
 
-template <typename T, typename O, int ACT>
-void product(const Operands& p, const Epilogue& e, cudaStream_t st) {
-  product_kernel<T, O, ACT><<<dim3(unsigned((p.m + kTile - 1) / kTile), unsigned((p.n + kTile - 1) / kTile)), 256, 0,
-                             st>>>(p, e);
-  note_launch();
+template <typename T, typename O, int V>
+void few_rows_v(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
+  const auto run = [&](auto kernel, int cols) {
+    kernel<<<(p.n + 4 * cols - 1) / (4 * cols), 128, 0, st>>>(static_cast<const T*>(p.x), p.x_stride,
+                                                              static_cast<const T*>(p.weight), p.weight_stride,
+                                                              int(p.m), p.n, p.k, e);
+    note_launch();
+  };
+  if (p.m == 1) return run(few_rows_kernel<T, O, V, 1, 2>, 2);
+  if (p.m == 2) return run(few_rows_kernel<T, O, V, 2, 2>, 2);
+  if (p.m <= 4) return run(few_rows_kernel<T, O, V, 4, 4>, 4);
+  return run(few_rows_kernel<T, O, V, 8, 4>, 4);
 }
 
 template <typename T, typename O>
-void product_act(int act, const Operands& p, const Epilogue& e, cudaStream_t st) {
-  switch (act) {
-    case GSB_ACT_RELU: return product<T, O, GSB_ACT_RELU>(p, e, st);
-    case GSB_ACT_GELU: return product<T, O, GSB_ACT_GELU>(p, e, st);
-    case GSB_ACT_GELU_TANH: return product<T, O, GSB_ACT_GELU_TANH>(p, e, st);
-    case GSB_ACT_SILU: return product<T, O, GSB_ACT_SILU>(p, e, st);
-    default: return product<T, O, GSB_ACT_NONE>(p, e, st);
+void few_rows(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
+  constexpr int E = sizeof(T);
+  if (p.k % (16 / E) == 0 && vec_ok(p.x, p.x_stride, E, 16) && vec_ok(p.weight, p.weight_stride, E, 16))
+    return few_rows_v<T, O, 16 / E>(p, e, st);
+  few_rows_v<T, O, 1>(p, e, st);
+}
+
+// ---- operands for the tensor cores ------------------------------------------------------------
+
+// The next multiple of 16 bytes of a row of `cols` values (float operands: of their bf16 parts).
+int64_t pitch_of(int64_t cols, int dtype) {
+  const int64_t per = dtype == GSB_E4M3 ? 16 : 8;
+  return (cols + per - 1) / per * per;
+}
+
+bool fits_tma(const void* p, int64_t stride, int dtype) {
+  const int e = dtype == GSB_E4M3 ? 1 : 2;
+  return dtype != GSB_F32 && stride > 0 && vec_ok(p, stride, e, 16);
+}
+
+size_t copy_bytes(int64_t rows, int64_t cols, int dtype) {
+  return size_t(rows) * size_t(pitch_of(cols, dtype)) * (dtype == GSB_F32 ? 6 : dtype == GSB_E4M3 ? 1 : 2);
+}
+
+// v as a sum of three bf16 values, each the rounding of what the ones before leave: 3 x 8 bits and
+// signs hold all 24 of a float's.  A first part that would round to infinity is truncated
+// instead; infinities and NaN go to the first part alone.
+struct Parts { bf16 p[3]; };
+__device__ __forceinline__ Parts split3(float v) {
+  Parts s;
+  s.p[0] = __float2bfloat16_rn(v);
+  const float top = __bfloat162float(s.p[0]);
+  const bool finite = fabsf(v) <= 3.402823466e38f;
+  if (finite && fabsf(top) > 3.402823466e38f) s.p[0] = __float2bfloat16_rz(v);
+  const float rest = finite ? v - __bfloat162float(s.p[0]) : 0.0f;
+  s.p[1] = __float2bfloat16_rn(rest);
+  s.p[2] = __float2bfloat16_rn(rest - __bfloat162float(s.p[1]));
+  return s;
+}
+
+struct CopyJob {
+  const void* in;
+  int64_t stride, rows, cols, pitch;
+  void* out;
+};
+
+// Rows copied to a pitch that TMA takes (16-bit and 8-bit values), one value per thread and step.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(CopyJob a) {
+  const int64_t total = a.rows * a.cols;
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
+    const int64_t i = t / a.cols, j = t - i * a.cols;
+    static_cast<T*>(a.out)[i * a.pitch + j] = static_cast<const T*>(a.in)[i * a.stride + j];
   }
 }
 
-// dz = dy act'(z) in the operands' type (dz NULL: only the column sums), and per block of rows the
-// float column sums of the unrounded dz.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t dy_stride, const typename PreactOf<T>::type* z,
-                                                 T* dz, float* part, int64_t m, int n, int64_t rows_per_part) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
-  const int64_t lo = blockIdx.y * rows_per_part, hi = min(m, lo + rows_per_part);
-  float s = 0.0f;
-  for (int64_t i = lo; i < hi; ++i) {
-    float v = to_f32(dy[i * dy_stride + j]);
-    if constexpr (ACT != GSB_ACT_NONE) v *= act_slope<ACT>(to_f32(z[i * n + j]));
-    if (dz) dz[i * n + j] = from_f32<T>(v);
-    s += v;
+// Two float matrices (the second may be empty) as three bf16 planes each.
+__global__ void __launch_bounds__(256) split_kernel(CopyJob a, CopyJob b, int a_blocks) {
+  const bool second = blockIdx.x >= a_blocks;
+  const CopyJob& s = second ? b : a;
+  const int64_t block = second ? blockIdx.x - a_blocks : blockIdx.x;
+  const int64_t blocks = second ? gridDim.x - a_blocks : a_blocks;
+  const int64_t plane = s.rows * s.pitch;
+  bf16* out = static_cast<bf16*>(s.out);
+  const int64_t quads = s.pitch / 4, total = s.rows * quads;
+  const bool vec = (reinterpret_cast<uintptr_t>(s.in) & 15) == 0 && (s.stride & 3) == 0 && (s.cols & 3) == 0;
+  for (int64_t t = block * 256 + threadIdx.x; t < total; t += blocks * 256) {
+    const int64_t i = t / quads, j = (t - i * quads) * 4;
+    const float* in = static_cast<const float*>(s.in) + i * s.stride + j;
+    float v[4] = {};
+    if (vec && j < s.cols) {
+      load_f32<float, 4>(in, v);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u < s.cols) v[u] = in[u];
+    }
+    Vec<bf16, 4> o[3];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const Parts q = split3(v[u]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) o[k].v[u] = q.p[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, 4>*>(out + k * plane + i * s.pitch + j) = o[k];
   }
-  if (part) part[int64_t(blockIdx.y) * n + j] = s;
 }
 
-constexpr int kDzParts = 128;
+int copy_blocks(int64_t steps) { return int(std::min<int64_t>((steps + 255) / 256, int64_t(sm_count()) * 8)); }
 
-template <typename T, int ACT>
-void launch_dz(const void* dy, int64_t dy_stride, const void* z, void* dz, float* part, int64_t m, int n,
-               int64_t per, int parts, cudaStream_t st) {
-  using Z = typename PreactOf<T>::type;
-  dz_kernel<T, ACT><<<dim3((n + 255) / 256, parts), 256, 0, st>>>(static_cast<const T*>(dy), dy_stride,
-                                                                static_cast<const Z*>(z), static_cast<T*>(dz), part, m,
-                                                                n, per);
+CopyJob job_of(const void* in, int64_t stride, int64_t rows, int64_t cols, int dtype, void* out) {
+  return {in, stride, rows, cols, pitch_of(cols, dtype), out};
+}
+
+void split(const CopyJob& a, const CopyJob& b, cudaStream_t st) {
+  const int na = copy_blocks(a.rows * (a.pitch / 4)), nb = b.rows ? copy_blocks(b.rows * (b.pitch / 4)) : 0;
+  split_kernel<<<na + nb, 256, 0, st>>>(a, b, na);
   note_launch();
 }
 
-struct BwdSpace {
+void pack(const CopyJob& a, int dtype, cudaStream_t st) {
+  const int blocks = copy_blocks(a.rows * a.cols);
+  if (dtype == GSB_E4M3) pack_kernel<uint8_t><<<blocks, 256, 0, st>>>(a);
+  else pack_kernel<uint16_t><<<blocks, 256, 0, st>>>(a);
+  note_launch();
+}
+
+// One operand as the tensor-core kernel reads it.
+struct Ready {
+  const void* p;
+  int64_t ld, plane;
+};
+
+// Two operands at once: in place where their rows are aligned, else copied (split) to the space given.
+void ready_pair(const CopyJob& a, const CopyJob& b, int dtype, Ready& ra, Ready& rb, cudaStream_t st) {
+  const CopyJob* jobs[2] = {&a, &b};
+  Ready* outs[2] = {&ra, &rb};
+  if (dtype == GSB_F32) split(a, b, st);
+  for (int i = 0; i < 2; ++i) {
+    const CopyJob& s = *jobs[i];
+    if (fits_tma(s.in, s.stride, dtype)) {
+      *outs[i] = {s.in, s.stride, 0};
+      continue;
+    }
+    if (dtype != GSB_F32 && s.rows) pack(s, dtype, st);
+    *outs[i] = {s.out, s.pitch, s.rows * s.pitch};
+  }
+}
+
+// ---- backward: dz and the bias gradient -------------------------------------------------------
+
+// dz = dy act'(z) rounded to the operands' type (float: its three bf16 parts), rows at `pitch`
+// (dz NULL: only the sums), and per block of rows the float column sums of the unrounded dz.
+// A block is 32 lanes x V columns by 8 rows; its rows' sums are added in a fixed order.
+template <typename T, int ACT, int V>
+__global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t dy_stride, const typename PreactOf<T>::type* z,
+                                                 void* dz, int64_t pitch, float* part, int64_t m, int n,
+                                                 int64_t rows_per_part) {
+  using Z = typename PreactOf<T>::type;
+  constexpr bool SPLIT = sizeof(T) == 4;
+  __shared__ float s_sum[8][32 * V + 1];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int j = (blockIdx.x * 32 + lane) * V;
+  const int64_t lo = blockIdx.y * rows_per_part, hi = min(m, lo + rows_per_part);
+  float s[V];
+#pragma unroll
+  for (int u = 0; u < V; ++u) s[u] = 0.0f;
+  if (j < n) {
+#pragma unroll 4
+    for (int64_t i = lo + g; i < hi; i += 8) {
+      float v[V];
+      load_f32<T, V>(dy + i * dy_stride + j, v);
+      if constexpr (ACT != GSB_ACT_NONE) {
+        float q[V];
+        load_f32<Z, V>(z + i * n + j, q);
+#pragma unroll
+        for (int u = 0; u < V; ++u) v[u] = __fmul_rn(v[u], act_slope<ACT>(q[u]));
+      }
+#pragma unroll
+      for (int u = 0; u < V; ++u) s[u] = __fadd_rn(s[u], v[u]);  // not fused: the same sum with and without dz
+      if (dz) {
+        if constexpr (SPLIT) {
+          Vec<bf16, V> o[3];
+#pragma unroll
+          for (int u = 0; u < V; ++u) {
+            const Parts q = split3(v[u]);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) o[k].v[u] = q.p[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            *reinterpret_cast<Vec<bf16, V>*>(static_cast<bf16*>(dz) + (k * m + i) * pitch + j) = o[k];
+        } else {
+          store_f32<T, V>(static_cast<T*>(dz) + i * pitch + j, v);
+        }
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int u = 0; u < V; ++u) s_sum[g][u * 32 + lane] = s[u];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * V; c += 256) {
+    const int jj = (blockIdx.x * 32 + (c & 31)) * V + (c >> 5);
+    if (jj < n) {
+      float t = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += s_sum[k][c];
+      part[int64_t(blockIdx.y) * n + jj] = t;
+    }
+  }
+}
+
+struct DzJob {
+  const void* dy;
+  int64_t dy_stride;
+  const void* z;
   void* dz;
+  int64_t pitch;
+  float* part;
+  int64_t m;
+  int n;
+  int64_t per;
+  int parts;
+};
+
+template <typename T, int ACT, int V>
+void launch_dz_v(const DzJob& d, cudaStream_t st) {
+  using Z = typename PreactOf<T>::type;
+  dz_kernel<T, ACT, V><<<dim3((d.n + 32 * V - 1) / (32 * V), d.parts), 256, 0, st>>>(
+      static_cast<const T*>(d.dy), d.dy_stride, static_cast<const Z*>(d.z), d.dz, d.pitch, d.part, d.m, d.n, d.per);
+  note_launch();
+}
+
+template <typename T, int ACT>
+void launch_dz(const DzJob& d, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  // z and dz are this library's own, aligned whenever n is a multiple of V
+  if (d.n % V == 0 && vec_ok(d.dy, d.dy_stride, sizeof(T), 16) && vec_ok(d.z, 0, 1, 16)) launch_dz_v<T, ACT, V>(d, st);
+  else launch_dz_v<T, ACT, 1>(d, st);
+}
+
+template <typename T>
+void launch_dz_act(int act, const DzJob& d, cudaStream_t st) {
+  switch (act) {
+    case GSB_ACT_RELU: return launch_dz<T, GSB_ACT_RELU>(d, st);
+    case GSB_ACT_GELU: return launch_dz<T, GSB_ACT_GELU>(d, st);
+    case GSB_ACT_GELU_TANH: return launch_dz<T, GSB_ACT_GELU_TANH>(d, st);
+    case GSB_ACT_SILU: return launch_dz<T, GSB_ACT_SILU>(d, st);
+    default: return launch_dz<T, GSB_ACT_NONE>(d, st);
+  }
+}
+
+// Blocks of rows whose column sums are kept apart: enough blocks to fill the GPU eight times over,
+// at least 32 rows each.
+int dz_parts(int64_t m, int n, int dtype) {
+  const int v = dtype == GSB_F32 ? 4 : 8;
+  const int64_t across = (n + 32 * v - 1) / (32 * v);
+  const int64_t want = std::max<int64_t>(1, int64_t(sm_count()) * 8 / across);
+  return int(std::max<int64_t>(1, std::min<int64_t>(want, (m + 31) / 32)));
+}
+
+// ---- workspaces -------------------------------------------------------------------------------
+
+struct FwdSpace {
+  void *x, *w;
+  size_t bytes;
+};
+
+FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
+  Carver c(ws, cap);
+  FwdSpace s{};
+  if (p.m > kFewRows) {
+    if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
+    if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
+  }
+  s.bytes = std::max(c.used, kAlign);
+  return s;
+}
+
+struct BwdSpace {
+  void *dz, *x, *w;
   float* part;
   size_t bytes;
 };
 
-BwdSpace bwd_space(const gsb_linear& p, void* ws, size_t cap) {
+bool keeps_dy(const gsb_linear& p, const void* dy, int64_t dy_stride) {
+  return p.activation == GSB_ACT_NONE && fits_tma(dy, dy_stride, p.dtype);
+}
+
+BwdSpace bwd_space(const gsb_linear& p, const void* dy, int64_t dy_stride, void* ws, size_t cap) {
   Carver c(ws, cap);
   BwdSpace s{};
-  s.part = c.take<float>(size_t(kDzParts) * p.n);
-  if (p.activation != GSB_ACT_NONE) s.dz = c.take<char>(size_t(p.m) * p.n * elem_bytes(p.dtype));
+  s.part = c.take<float>(size_t(dz_parts(p.m, p.n, p.dtype)) * p.n);
+  if (!keeps_dy(p, dy, dy_stride)) s.dz = c.take<char>(copy_bytes(p.m, p.n, p.dtype));
+  if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
+  if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
   s.bytes = c.used;
   return s;
 }
 
-template <typename T>
-gsb_status bwd_of_type(const gsb_linear& p, const void* z, const void* dy, int64_t dy_stride, void* dx, void* dw,
-                       void* db, const BwdSpace& s, cudaStream_t st) {
-  const int64_t per = (p.m + kDzParts - 1) / kDzParts;
-  const int parts = int((p.m + per - 1) / per);
-  const void* dz = dy;
-  int64_t dz_stride = dy_stride;
-  if (p.activation != GSB_ACT_NONE) {
-    dz = s.dz;
-    dz_stride = p.n;
-  }
-  if (db || p.activation != GSB_ACT_NONE) {
-    void* out = p.activation != GSB_ACT_NONE ? s.dz : nullptr;
-    float* part = db ? s.part : nullptr;
-    switch (p.activation) {
-      case GSB_ACT_RELU: launch_dz<T, GSB_ACT_RELU>(dy, dy_stride, z, out, part, p.m, p.n, per, parts, st); break;
-      case GSB_ACT_GELU: launch_dz<T, GSB_ACT_GELU>(dy, dy_stride, z, out, part, p.m, p.n, per, parts, st); break;
-      case GSB_ACT_GELU_TANH:
-        launch_dz<T, GSB_ACT_GELU_TANH>(dy, dy_stride, z, out, part, p.m, p.n, per, parts, st);
-        break;
-      case GSB_ACT_SILU: launch_dz<T, GSB_ACT_SILU>(dy, dy_stride, z, out, part, p.m, p.n, per, parts, st); break;
-      default: launch_dz<T, GSB_ACT_NONE>(dy, dy_stride, z, out, part, p.m, p.n, per, parts, st); break;
-    }
-    if (db) {
-      column_sum_kernel<T><<<(p.n + 31) / 32, 256, 0, st>>>(s.part, parts, p.n, static_cast<T*>(db));
-      note_launch();
+Epilogue plain_output(void* out, int64_t cols, int dtype) {
+  Epilogue e{};
+  e.out = out;
+  e.out_stride = cols;
+  const int b = elem_bytes(dtype);
+  e.vec = cols % (16 / b) == 0 && vec_ok(out, cols, b, 16);
+  return e;
+}
+
+gsb_status bwd(const gsb_linear& p, const void* z, const void* dy, int64_t dy_stride, void* dx, void* dw, void* db,
+               const BwdSpace& s, cudaStream_t st) {
+  const bool keep = keeps_dy(p, dy, dy_stride);
+  const bool products = dx || dw;
+  const int64_t pitch = keep ? dy_stride : pitch_of(p.n, p.dtype);
+  DzJob d{dy, dy_stride, z, keep || !products ? nullptr : s.dz, pitch, db ? s.part : nullptr, p.m, p.n, 0, 0};
+  d.parts = dz_parts(p.m, p.n, p.dtype);
+  d.per = (p.m + d.parts - 1) / d.parts;
+  d.parts = int((p.m + d.per - 1) / d.per);
+  if (d.dz || db) {
+    switch (p.dtype) {
+      case GSB_F32: launch_dz_act<float>(p.activation, d, st); break;
+      case GSB_BF16: launch_dz_act<bf16>(p.activation, d, st); break;
+      default: launch_dz_act<f16>(p.activation, d, st); break;
     }
   }
-  if (dx) {
-    Epilogue e{};
-    e.out = dx;
-    e.out_stride = p.k;
-    product<T, T, GSB_ACT_NONE>({dz, dz_stride, 1, p.weight, 1, p.weight_stride, p.m, p.k, p.n}, e, st);
+  if (db) {
+    const int blocks = (p.n + 31) / 32;
+    switch (p.dtype) {
+      case GSB_F32: column_sum_kernel<float><<<blocks, 256, 0, st>>>(s.part, d.parts, p.n, static_cast<float*>(db)); break;
+      case GSB_BF16: column_sum_kernel<bf16><<<blocks, 256, 0, st>>>(s.part, d.parts, p.n, static_cast<bf16*>(db)); break;
+      default: column_sum_kernel<f16><<<blocks, 256, 0, st>>>(s.part, d.parts, p.n, static_cast<f16*>(db)); break;
+    }
+    note_launch();
   }
-  if (dw) {
-    Epilogue e{};
-    e.out = dw;
-    e.out_stride = p.k;
-    product<T, T, GSB_ACT_NONE>({dz, 1, dz_stride, p.x, 1, p.x_stride, p.n, p.k, p.m}, e, st);
-  }
-  return launch_status();
+  if (!products) return launch_status();
+  const Ready g = keep ? Ready{dy, dy_stride, 0} : Ready{s.dz, pitch, p.m * pitch};
+  CopyJob jx = job_of(p.x, p.x_stride, dw ? p.m : 0, p.k, p.dtype, s.x);
+  CopyJob jw = job_of(p.weight, p.weight_stride, dx ? p.n : 0, p.k, p.dtype, s.w);
+  Ready x, w;
+  if (jx.rows) ready_pair(jx, jw, p.dtype, x, w, st);
+  else ready_pair(jw, jx, p.dtype, w, x, st);
+  gsb_status status = launch_status();
+  if (dx && status == GSB_OK)
+    status = mma_product({g.p, g.ld, false, w.p, w.ld, true, p.m, p.k, p.n, p.dtype, p.dtype, g.plane, w.plane},
+                         plain_output(dx, p.k, p.dtype), st);
+  if (dw && status == GSB_OK)
+    status = mma_product({g.p, g.ld, true, x.p, x.ld, true, p.n, p.k, p.m, p.dtype, p.dtype, g.plane, x.plane},
+                         plain_output(dw, p.k, p.dtype), st);
+  return status;
 }
 
 gsb_status check_linear(const gsb_linear* p) {
@@ -226,7 +420,7 @@ gsb_status check_operands(const gsb_linear* p) {
 
 size_t linear_fwd_workspace(const gsb_linear* p) {
   if (check_linear(p) != GSB_OK) return 0;
-  return kAlign;
+  return fwd_space(*p, nullptr, 0).bytes;
 }
 
 gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -235,8 +429,7 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   if (p->dtype == GSB_E4M3 && preact) return GSB_ERR_ARG;
   if (p->m == 0) return GSB_OK;
   if (!y) return GSB_ERR_ARG;
-  Operands o{p->x, p->x_stride, 1, p->weight, p->weight_stride, 1, p->m, p->n, p->k};
-  Epilogue e{};
+  Epilogue e = plain_output(y, p->n, p->out_dtype);
   if (p->dtype == GSB_E4M3) {
     e.row_scale = p->x_scale;
     e.col_scale = p->weight_scale;
@@ -245,23 +438,35 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   e.res = p->residual;
   e.res_stride = p->residual_stride;
   e.preact = preact;
-  e.out = y;
-  e.out_stride = p->n;
-  switch (p->dtype) {
-    case GSB_F32: product_act<float, float>(p->activation, o, e, st); break;
-    case GSB_BF16: product_act<bf16, bf16>(p->activation, o, e, st); break;
-    case GSB_F16: product_act<f16, f16>(p->activation, o, e, st); break;
-    default:
-      if (p->out_dtype == GSB_F32) product_act<e4m3, float>(p->activation, o, e, st);
-      else if (p->out_dtype == GSB_BF16) product_act<e4m3, bf16>(p->activation, o, e, st);
-      else product_act<e4m3, f16>(p->activation, o, e, st);
+  e.act = p->activation;
+  const int b = elem_bytes(p->out_dtype);
+  e.vec = e.vec && vec_ok(p->bias, 0, b, 16) && vec_ok(preact, 0, b, 16) &&
+          (!p->residual || vec_ok(p->residual, p->residual_stride, b, 16));
+  if (p->m <= kFewRows) {
+    switch (p->dtype) {
+      case GSB_F32: few_rows<float, float>(*p, e, st); break;
+      case GSB_BF16: few_rows<bf16, bf16>(*p, e, st); break;
+      case GSB_F16: few_rows<f16, f16>(*p, e, st); break;
+      default:
+        if (p->out_dtype == GSB_F32) few_rows<e4m3, float>(*p, e, st);
+        else if (p->out_dtype == GSB_BF16) few_rows<e4m3, bf16>(*p, e, st);
+        else few_rows<e4m3, f16>(*p, e, st);
+    }
+    return launch_status();
   }
-  return launch_status();
+  if (!ws || ws_bytes < linear_fwd_workspace(p)) return GSB_ERR_WORKSPACE;
+  const FwdSpace s = fwd_space(*p, ws, ws_bytes);
+  Ready x, w;
+  ready_pair(job_of(p->x, p->x_stride, p->m, p->k, p->dtype, s.x),
+             job_of(p->weight, p->weight_stride, p->n, p->k, p->dtype, s.w), p->dtype, x, w, st);
+  if (gsb_status q = launch_status(); q != GSB_OK) return q;
+  return mma_product({x.p, x.ld, false, w.p, w.ld, false, p->m, p->n, p->k, p->dtype, p->out_dtype, x.plane, w.plane},
+                     e, st);
 }
 
-size_t linear_bwd_workspace(const gsb_linear* p) {
+size_t linear_bwd_workspace(const gsb_linear* p, const void* dy, int64_t dy_stride) {
   if (check_linear(p) != GSB_OK) return 0;
-  return bwd_space(*p, nullptr, 0).bytes;
+  return bwd_space(*p, dy, dy_stride, nullptr, 0).bytes;
 }
 
 gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, int64_t dy_stride, void* dx,
@@ -276,13 +481,14 @@ gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, i
   }
   if (!dy || (p->activation != GSB_ACT_NONE && !preact)) return GSB_ERR_ARG;
   if ((dx && !p->weight) || (dweight && !p->x)) return GSB_ERR_ARG;
-  if (!ws || ws_bytes < linear_bwd_workspace(p)) return GSB_ERR_WORKSPACE;
-  const BwdSpace s = bwd_space(*p, ws, ws_bytes);
-  switch (p->dtype) {
-    case GSB_F32: return bwd_of_type<float>(*p, preact, dy, dy_stride, dx, dweight, dbias, s, st);
-    case GSB_BF16: return bwd_of_type<bf16>(*p, preact, dy, dy_stride, dx, dweight, dbias, s, st);
-    default: return bwd_of_type<f16>(*p, preact, dy, dy_stride, dx, dweight, dbias, s, st);
-  }
+  if (!ws || ws_bytes < linear_bwd_workspace(p, dy, dy_stride)) return GSB_ERR_WORKSPACE;
+  return bwd(*p, preact, dy, dy_stride, dx, dweight, dbias, bwd_space(*p, dy, dy_stride, ws, ws_bytes), st);
+}
+
+gsb_status linear_status() {
+  int gave_up = 0;
+  if (gsb_status s = mma_status(&gave_up); s != GSB_OK) return s;
+  return gave_up ? GSB_ERR_TIMEOUT : GSB_OK;
 }
 
 }  // namespace gsb

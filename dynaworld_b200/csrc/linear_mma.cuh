@@ -1,0 +1,719 @@
+// Matrix product on the fifth-generation tensor cores (sm_100a): D = A B^T in float.
+//
+// Persistent kernel, one CTA per SM; CG = 2 pairs the CTAs of a cluster on one 256 x BN tile, so
+// that each loads half of B.  Warp roles of a CTA (384 threads):
+//   warp 0      loads: TMA copies of 128-byte wide boxes (swizzled) into a ring of slots
+//   warp 1      issues tcgen05.mma, accumulators in TMEM (two buffers: the next tile's products
+//               run while this tile's epilogue reads)
+//   warp 2      allocates and frees TMEM
+//   warps 4-11  epilogue: TMEM -> registers -> a padded shared-memory transpose, so that the
+//               stores (and the residual's loads) are rows of 16-byte accesses
+// Operands are K-major (rows of k) or MN-major (rows of m or n, as the backward's products have
+// them): the TMA box and the shared-memory descriptor differ, nothing is transposed in memory.
+//
+// Float operands (PLANES = 3) are sums of three bf16 parts; the products (3,1) (1,3) (2,2) (1,2)
+// (2,1) go to one accumulator and (1,1) to another, and every kChunk blocks of K both are added to
+// float registers: the tensor core's additions truncate, and a long chain of them loses about
+// steps x 2^-25 of the sum.
+//
+// Every wait is bounded (4 s).  A wait that gives up sets a sticky flag, its CTA's remaining tiles
+// become NaN, and every role leaves its loop.
+#pragma once
+
+#include <cuda.h>
+
+#include <atomic>
+
+#include "linear_parts.cuh"
+
+namespace gsb {
+namespace mma {
+
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
+constexpr int kPitch = 36;                  // floats per row of an epilogue warp's 32 x 32 block
+constexpr int kStageBytes = kEpiWarps * 32 * kPitch * 4;
+constexpr int kRowBytes = 128;              // one swizzled row of a box
+constexpr int kABytes = 128 * kRowBytes;
+constexpr int kChunk = 4;                   // PLANES = 3: blocks of 64 k per accumulation chain
+constexpr uint64_t kWaitNs = 4000000000ull;
+
+
+struct Args {
+  int64_t m, n;
+  int k_blocks;
+  int m_tiles, n_tiles;
+  int64_t tiles;
+  int group;        // m tiles walked together, for reuse in L2
+  uint32_t idesc;
+  int* gave_up;
+  Epilogue e;
+};
+
+// ---- PTX ----
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// bar: an address in the cluster's shared window
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Bounded wait; false when it gave up.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* gave_up) {
+  for (int i = 0; i < 256; ++i)
+    if (bar_try(bar, parity)) return true;
+  const uint64_t t0 = now_ns();
+  while (now_ns() - t0 < kWaitNs) {
+    for (int i = 0; i < 64; ++i)
+      if (bar_try(bar, parity)) return true;
+  }
+  atomicExch(gave_up, 1);
+  return false;
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int plane, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(plane), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(plane), "r"(bar)
+        : "memory");
+}
+
+template <int KIND, int CG>
+__device__ __forceinline__ void mma_issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define GSB_MMA(cg, kind)                                                                                     \
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"                                                     \
+               "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), \
+               "r"(idesc), "r"(accumulate)                                                                     \
+               : "memory")
+  if constexpr (KIND == 1) {
+    if constexpr (CG == 1) GSB_MMA("1", "f8f6f4");
+    else GSB_MMA("2", "f8f6f4");
+  } else {
+    if constexpr (CG == 1) GSB_MMA("1", "f16");
+    else GSB_MMA("2", "f16");
+  }
+#undef GSB_MMA
+}
+
+// Arrives on bar (both CTAs' barriers at this offset with CG = 2) when the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(uint16_t(3))
+        : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle (layout type 2 in bits 61-63, version 1 in bits
+// 46-47).  K-major: 8-row groups 1024 bytes apart (the stride offset).  MN-major: blocks of 64
+// columns 8192 bytes apart (the leading offset), groups of 8 k 1024 bytes apart.
+template <bool MN>
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+  constexpr uint64_t lead = MN ? 8192 / 16 : 1, stride = 1024 / 16;
+  return uint64_t((addr >> 4) & 0x3fff) | (lead << 16) | (stride << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Descriptor advance per MMA (16 k of 16-bit, 32 of 8-bit values): 32 bytes along a K-major row,
+// two 8-k groups MN-major; in units of 16 bytes.
+template <bool MN>
+constexpr uint32_t kDescStep = MN ? 2048 / 16 : 32 / 16;
+
+__device__ __forceinline__ void tile_of(const Args& p, int64_t t, int64_t& mt, int64_t& nt) {
+  const int64_t per = int64_t(p.group) * p.n_tiles;
+  const int64_t band = t / per, r = t - band * per;
+  const int64_t first = band * p.group;
+  const int64_t rows = min(int64_t(p.group), int64_t(p.m_tiles) - first);
+  mt = first + r % rows;
+  nt = r / rows;
+}
+
+// A warp's part of the epilogue.  A 32 x 32 block of sums (lane = row) goes through shared memory so
+// that global accesses are 16 bytes per lane: V values, 32 / V lanes per row, kSteps rows per lane.
+// The residual and bias of the next block are loaded while this one is finished: a block takes
+// about 600 cycles, the residual's way from HBM more.
+template <typename O, int ACT>
+struct Rows {
+  static constexpr int V = 16 / int(sizeof(O));
+  static constexpr int kPerRow = 32 / V;
+  static constexpr int kAtOnce = 32 / kPerRow;  // rows in one access of the warp
+  static constexpr int kSteps = 32 / kAtOnce;
+  using Z = typename PreactOf<O>::type;
+  struct Ahead {
+    uint4 res[kSteps];
+    uint4 bias;
+  };
+  int row0, col;  // this lane's first row and column within the block
+  int steps;      // its rows inside the matrix
+  int64_t i;      // its first row
+  float rs[kSteps];
+
+  __device__ __forceinline__ void start(const Args& p, int64_t i0) {
+    const int lane = threadIdx.x & 31;
+    row0 = lane / kPerRow;
+    col = (lane % kPerRow) * V;
+    i = i0 + row0;
+    steps = int(max(int64_t(0), min(int64_t(kSteps), (p.m - i + kAtOnce - 1) / kAtOnce)));
+    if (p.e.row_scale) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) rs[s] = s < steps ? p.e.row_scale[i + s * kAtOnce] : 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void prefetch(const Args& p, int64_t j0, Ahead& a) const {
+    const int64_t j = j0 + col;
+    const bool in = p.e.vec && j < p.n;
+    if (p.e.bias && in) a.bias = __ldg(reinterpret_cast<const uint4*>(static_cast<const O*>(p.e.bias) + j));
+    if (p.e.res) {
+      const O* r = static_cast<const O*>(p.e.res) + i * p.e.res_stride + j;
+      const int64_t step = kAtOnce * p.e.res_stride;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (in && s < steps) a.res[s] = __ldg(reinterpret_cast<const uint4*>(r + s * step));
+    }
+  }
+
+  __device__ __forceinline__ void emit(const Args& p, float* stage, int64_t i0, int64_t j0, const float (&v)[32],
+                                       const Ahead& a) const {
+    const int lane = threadIdx.x & 31;
+    float4* mine = reinterpret_cast<float4*>(stage + lane * kPitch);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) mine[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    __syncwarp();
+    if (p.e.vec) {
+      const int64_t j = j0 + col;
+      if (j < p.n) {
+        float bias[V], cs[V];
+        if (p.e.bias) {
+          const Vec<O, V> b = *reinterpret_cast<const Vec<O, V>*>(&a.bias);
+#pragma unroll
+          for (int u = 0; u < V; ++u) bias[u] = to_f32(b.v[u]);
+        }
+        if (p.e.row_scale) {
+#pragma unroll
+          for (int u = 0; u < V; ++u) cs[u] = p.e.col_scale[j + u];
+        }
+        O* out = static_cast<O*>(p.e.out) + i * p.e.out_stride + j;
+        Z* keep = static_cast<Z*>(p.e.preact) + i * p.n + j;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          if (s >= steps) break;
+          float z[V];
+          const float* from = stage + (row0 + s * kAtOnce) * kPitch + col;
+#pragma unroll
+          for (int u = 0; u < V; u += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(from + u);
+            z[u] = q.x, z[u + 1] = q.y, z[u + 2] = q.z, z[u + 3] = q.w;
+          }
+          if (p.e.row_scale) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) z[u] *= rs[s] * cs[u];
+          }
+          if (p.e.bias) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) z[u] += bias[u];
+          }
+          if (p.e.preact) {
+            Vec<Z, V> kept;
+#pragma unroll
+            for (int u = 0; u < V; ++u) kept.v[u] = as_preact(static_cast<Z*>(nullptr), z[u]);
+            *reinterpret_cast<Vec<Z, V>*>(keep + s * kAtOnce * p.n) = kept;
+          }
+          #pragma unroll
+          for (int u = 0; u < V; ++u) z[u] = act_value<ACT>(z[u]);
+          if (p.e.res) {
+            const Vec<O, V> r = *reinterpret_cast<const Vec<O, V>*>(&a.res[s]);
+#pragma unroll
+            for (int u = 0; u < V; ++u) z[u] += to_f32(r.v[u]);
+          }
+          store_f32<O, V>(out + s * kAtOnce * p.e.out_stride, z);
+        }
+      }
+    } else {
+      // rows that start anywhere: a lane per column, eight rows' loads in flight
+      const int64_t j = j0 + lane;
+      if (j < p.n) {
+        const float b = p.e.bias ? to_f32(static_cast<const O*>(p.e.bias)[j]) : 0.0f;
+        const float cs = p.e.row_scale ? p.e.col_scale[j] : 1.0f;
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          const int rows = int(min(int64_t(8), p.m - i0 - r0));
+          float z[8], add[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            z[r] = stage[(r0 + r) * kPitch + lane];
+            add[r] = 0.0f;
+            if (r < rows) {
+              if (p.e.row_scale) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
+              if (p.e.res) add[r] = to_f32(static_cast<const O*>(p.e.res)[(i0 + r0 + r) * p.e.res_stride + j]);
+            }
+            z[r] += b;
+          }
+          if (p.e.preact) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (r < rows)
+                static_cast<Z*>(p.e.preact)[(i0 + r0 + r) * p.n + j] = as_preact(static_cast<Z*>(nullptr), z[r]);
+          }
+          #pragma unroll
+          for (int r = 0; r < 8; ++r) z[r] = act_value<ACT>(z[r]);
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < rows) static_cast<O*>(p.e.out)[(i0 + r0 + r) * p.e.out_stride + j] = from_f32<O>(z[r] + add[r]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+};
+
+template <int CG, int BN, int PLANES>
+struct Shape {
+  static constexpr int kBRows = BN / CG;              // rows of B that one CTA loads
+  static constexpr int kBBytes = kBRows * kRowBytes;
+  static constexpr int kSlot = kABytes + kBBytes;
+  static constexpr int kBudget = 232448 - 1024 - kStageBytes - 256;
+  static constexpr int kSlots = kBudget / kSlot < 8 ? kBudget / kSlot : 8;
+  static constexpr int kBufs = 2;
+  static constexpr int kAccCols = PLANES == 1 ? BN : 2 * BN;  // TMEM columns of one accumulator buffer
+  static constexpr int kCols = kBufs * kAccCols;
+  static constexpr int kBytes = 1024 + kSlots * kSlot + kStageBytes + 256;
+  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0 && kCols >= 32, "TMEM columns");
+  static_assert(PLANES == 1 || kSlots >= 4, "a block's three slots and one ahead");
+};
+
+// KIND 0: 16-bit operands, 1: e4m3.
+template <int KIND, int CG, int BN, bool A_MN, bool B_MN, int PLANES, typename O, int ACT>
+__global__ void __launch_bounds__(kThreads, 1)
+    mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ Args p) {
+  using S = Shape<CG, BN, PLANES>;
+  constexpr int kElems = KIND == 1 ? 128 : 64;  // k per block
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  uint8_t* smem = raw + (base - smem_addr(raw));
+  float* stage_all = reinterpret_cast<float*>(smem + S::kSlots * S::kSlot);
+  const uint32_t bars = base + S::kSlots * S::kSlot + kStageBytes;
+  const auto full = [&](int s) { return bars + 8 * s; };
+  const auto empty = [&](int s) { return bars + 8 * (S::kSlots + s); };
+  const auto acc_full = [&](int b) { return bars + 8 * (2 * S::kSlots + b); };
+  const auto acc_empty = [&](int b) { return bars + 8 * (2 * S::kSlots + 2 + b); };
+  const uint32_t tmem_slot = bars + 8 * (2 * S::kSlots + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kSlots; ++s) {
+      bar_init(full(s), 1);
+      bar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      bar_init(acc_full(b), 1);
+      bar_init(acc_empty(b), kEpiWarps * CG);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc<CG>(tmem_slot, S::kCols);
+  fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
+
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int s = 0;
+      uint32_t phase = 0;
+      for (int64_t t = first; ok && t < p.tiles; t += step) {
+        int64_t mt, nt;
+        tile_of(p, t, mt, nt);
+        const int i0 = int((mt * CG + rank) * 128);
+        const int j0 = int(nt * BN + rank * S::kBRows);
+        for (int kb = 0; ok && kb < p.k_blocks; ++kb) {
+          const int k0 = kb * kElems;
+#pragma unroll
+          for (int q = 0; q < PLANES; ++q) {
+            const int plane = PLANES == 1 ? 0 : (q == 0 ? 2 : q - 1);  // parts 3, 1, 2
+            if (!(ok = bar_wait(empty(s), phase ^ 1, p.gave_up))) break;
+            const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
+            if (rank == 0) bar_expect(full(s), CG * S::kSlot);
+            const uint32_t a = base + s * S::kSlot, b = a + kABytes;
+            if constexpr (A_MN) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) tma_load<CG>(a + u * 8192, &map_a, i0 + 64 * u, k0, plane, bar);
+            } else {
+              tma_load<CG>(a, &map_a, k0, i0, plane, bar);
+            }
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int u = 0; u < S::kBRows / 64; ++u) tma_load<CG>(b + u * 8192, &map_b, j0 + 64 * u, k0, plane, bar);
+            } else {
+              tma_load<CG>(b, &map_b, k0, j0, plane, bar);
+            }
+            if (++s == S::kSlots) s = 0, phase ^= 1;
+          }
+        }
+      }
+      // every slot released: no arrival of a commit comes after the CTA's end
+      for (int q = 0; ok && q < S::kSlots; ++q) {
+        ok = bar_wait(empty(s), phase ^ 1, p.gave_up);
+        if (++s == S::kSlots) s = 0, phase ^= 1;
+      }
+      if (!ok)
+        for (int i = 0; i < 1000; ++i) __nanosleep(10000);  // copies in flight land before the CTA ends
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      bool ok = true;
+      int s = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      const auto next = [&](int x) { return x + 1 == S::kSlots ? 0 : x + 1; };
+      for (int64_t t = first; ok && t < p.tiles; t += step) {
+        for (int kb = 0; ok && kb < p.k_blocks;) {
+          if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
+          fence_after();
+          const uint32_t acc = tmem + buf * S::kAccCols;
+          const int stop = PLANES == 1 ? p.k_blocks : min(p.k_blocks, kb + kChunk);
+          uint32_t more = 0, more_low = 0;
+          for (; kb < stop; ++kb) {
+            if constexpr (PLANES == 1) {
+              if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
+              fence_after();
+              const uint64_t a = smem_desc<A_MN>(base + s * S::kSlot);
+              const uint64_t b = smem_desc<B_MN>(base + s * S::kSlot + kABytes);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                mma_issue<KIND, CG>(acc, a + u * kDescStep<A_MN>, b + u * kDescStep<B_MN>, p.idesc, more);
+                more = 1;
+              }
+              mma_commit<CG>(empty(s));
+              if (++s == S::kSlots) s = 0, phase ^= 1;
+            } else {
+              const int s3 = s, s1 = next(s3), s2 = next(s1);
+              const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
+              const auto da = [&](int q) { return smem_desc<A_MN>(base + q * S::kSlot); };
+              const auto db = [&](int q) { return smem_desc<B_MN>(base + q * S::kSlot + kABytes); };
+              const auto run = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t& on) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  mma_issue<KIND, CG>(d, a + u * kDescStep<A_MN>, b + u * kDescStep<B_MN>, p.idesc, on);
+                  on = 1;
+                }
+              };
+              if (!(ok = bar_wait(full(s3), phase, p.gave_up) && bar_wait(full(s1), ph1, p.gave_up))) break;
+              fence_after();
+              run(acc + BN, da(s3), db(s1), more_low);
+              run(acc + BN, da(s1), db(s3), more_low);
+              mma_commit<CG>(empty(s3));
+              if (!(ok = bar_wait(full(s2), ph2, p.gave_up))) break;
+              fence_after();
+              run(acc + BN, da(s2), db(s2), more_low);
+              run(acc + BN, da(s1), db(s2), more_low);
+              run(acc + BN, da(s2), db(s1), more_low);
+              mma_commit<CG>(empty(s2));
+              run(acc, da(s1), db(s1), more);
+              mma_commit<CG>(empty(s1));
+              s = next(s2);
+              phase = ph2 ^ (s < s2);
+            }
+          }
+          mma_commit<CG>(acc_full(buf));
+          buf ^= 1;
+          if (buf == 0) acc_phase ^= 1;
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    const int w = warp - 4, quad = warp & 3, half = w >> 2;  // quad: the 32 TMEM lanes this warp may read
+    float* stage = stage_all + w * 32 * kPitch;
+    const uint32_t lanes = uint32_t(quad * 32) << 16;
+    constexpr int kHalfCols = BN / 2;
+    bool ok = true;
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    Rows<O, ACT> rows;
+    typename Rows<O, ACT>::Ahead ahead;
+    for (int64_t t = first; t < p.tiles; t += step) {
+      int64_t mt, nt;
+      tile_of(p, t, mt, nt);
+      const int64_t i0 = (mt * CG + rank) * 128 + quad * 32;
+      const int64_t j0 = nt * BN + half * kHalfCols;
+      const auto release = [&](int b) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(map_to_rank(acc_empty(b), 0));
+      };
+      if constexpr (PLANES == 1) {
+        rows.start(p, i0);
+        rows.prefetch(p, j0, ahead);
+        ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
+        fence_after();
+        const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
+#pragma unroll 1
+        for (int c = 0; c < kHalfCols; c += 32) {
+          const typename Rows<O, ACT>::Ahead now = ahead;
+          if (c + 32 < kHalfCols) rows.prefetch(p, j0 + c + 32, ahead);
+          float v[32];
+          tmem_load32(acc + c, v);
+          if (c + 32 == kHalfCols) release(buf);
+          if (!ok) {
+#pragma unroll
+            for (int u = 0; u < 32; ++u) v[u] = __int_as_float(0x7fc00000);
+          }
+          if (i0 < p.m && j0 + c < p.n) rows.emit(p, stage, i0, j0 + c, v, now);
+        }
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
+      } else {
+        float sum[kHalfCols];
+#pragma unroll
+        for (int u = 0; u < kHalfCols; ++u) sum[u] = 0.0f;
+        for (int kb = 0; kb < p.k_blocks; kb += kChunk) {
+          ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
+          fence_after();
+          const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
+#pragma unroll
+          for (int c = 0; c < kHalfCols; c += 16) {
+            float low[16], high[16];
+            tmem_load16(acc + BN + c, low);
+            tmem_load16(acc + c, high);
+#pragma unroll
+            for (int u = 0; u < 16; ++u) sum[c + u] += high[u] + low[u];
+          }
+          release(buf);
+          buf ^= 1;
+          if (buf == 0) acc_phase ^= 1;
+        }
+        rows.start(p, i0);
+#pragma unroll
+        for (int c = 0; c < kHalfCols; c += 32) {
+          rows.prefetch(p, j0 + c, ahead);
+          float v[32];
+#pragma unroll
+          for (int u = 0; u < 32; ++u) v[u] = ok ? sum[c + u] : __int_as_float(0x7fc00000);
+          if (i0 < p.m && j0 + c < p.n) rows.emit(p, stage, i0, j0 + c, v, ahead);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();
+  fence_after();
+  if (warp == 2) tmem_free<CG>(tmem, S::kCols);
+}
+
+// ---- host ----
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn();  // NULL when the driver does not offer it
+
+// An operand [rows, k] as boxes of 128 bytes: K-major 128-byte rows of k, MN-major 64 rows of k by 64
+// columns.  Values outside the matrix read as 0.
+inline bool make_map(CUtensorMap* map, const void* ptr, int dtype, bool mn, int64_t rows, int64_t k, int64_t ld,
+                     int box_rows, int planes, int64_t plane_stride) {
+  EncodeFn encode = encode_fn();
+  if (!encode) return false;
+  const int e = dtype == GSB_E4M3 ? 1 : 2;
+  const CUtensorMapDataType type = dtype == GSB_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == GSB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint64_t dims[3] = {cuuint64_t(mn ? rows : k), cuuint64_t(mn ? k : rows), cuuint64_t(planes)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * e, cuuint64_t(planes > 1 ? plane_stride : ld) * e};
+  const cuuint32_t box[3] = {cuuint32_t(128 / e), cuuint32_t(mn ? 64 : box_rows), 1};
+  const cuuint32_t unit[3] = {1, 1, 1};
+  return encode(map, type, 3, const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// kind::f16: D float (bit 4), A and B formats (0 fp16, 1 bf16; e4m3 is 0 of kind::f8f6f4), MN-major
+// flags in bits 15 and 16, N / 8 from bit 17, M / 16 from bit 24.
+inline uint32_t instr_desc(int dtype, bool a_mn, bool b_mn, int m, int n) {
+  const uint32_t f = (dtype == GSB_BF16 || dtype == GSB_F32) ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+template <int KIND, int CG, int BN, bool A_MN, bool B_MN, int PLANES, typename O, int ACT>
+gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
+  using S = Shape<CG, BN, PLANES>;
+  auto* kernel = mma_kernel<KIND, CG, BN, A_MN, B_MN, PLANES, O, ACT>;
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
+  static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel has its shared memory
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return GSB_ERR_CUDA;
+    }
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  constexpr int kElems = KIND == 1 ? 128 : 64;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, p.a, p.dtype, A_MN, p.m, p.k, p.a_ld, 128, PLANES, p.a_plane) ||
+      !make_map(&mb, p.b, p.dtype, B_MN, p.n, p.k, p.b_ld, S::kBRows, PLANES, p.b_plane))
+    return GSB_ERR_CUDA;
+  Args a{};
+  a.m = p.m;
+  a.n = p.n;
+  a.k_blocks = int((p.k + kElems - 1) / kElems);
+  a.m_tiles = int((p.m + 128 * CG - 1) / (128 * CG));
+  a.n_tiles = int((p.n + BN - 1) / BN);
+  a.tiles = int64_t(a.m_tiles) * a.n_tiles;
+  a.group = 8;
+  a.idesc = instr_desc(p.dtype, A_MN, B_MN, 128 * CG, BN);
+  a.gave_up = mma_flag();
+  if (!a.gave_up) return GSB_ERR_CUDA;
+  a.e = e;
+  const int clusters = int(std::min<int64_t>(a.tiles, sm_count() / CG));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(clusters * CG));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
+  note_launch();
+  if (err != cudaSuccess) {
+    (void)cudaGetLastError();
+    return GSB_ERR_CUDA;
+  }
+  return launch_status();
+}
+
+template <int KIND, int CG, int BN, int PLANES, typename O>
+gsb_status launch_act(const Product& p, const Epilogue& e, cudaStream_t st) {
+  switch (e.act) {
+    case GSB_ACT_RELU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_RELU>(p, e, st);
+    case GSB_ACT_GELU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_GELU>(p, e, st);
+    case GSB_ACT_GELU_TANH: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_GELU_TANH>(p, e, st);
+    case GSB_ACT_SILU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_SILU>(p, e, st);
+    default: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_NONE>(p, e, st);
+  }
+}
+
+// The forward's product, or one of the backward's two (which have no epilogue).
+template <int CG, int BN, int PLANES, typename O>
+gsb_status launch_any(const Product& p, const Epilogue& e, cudaStream_t st) {
+  if (!p.b_mn) return launch_act<0, CG, BN, PLANES, O>(p, e, st);
+  if (!p.a_mn) return launch<0, CG, BN, false, true, PLANES, O, GSB_ACT_NONE>(p, e, st);
+  return launch<0, CG, BN, true, true, PLANES, O, GSB_ACT_NONE>(p, e, st);
+}
+
+}  // namespace mma
+}  // namespace gsb

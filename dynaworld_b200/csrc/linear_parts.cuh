@@ -1,0 +1,122 @@
+// What the matrix product's kernels share: operands, epilogue and the element-wise tail.
+#pragma once
+
+#include "activation.cuh"
+#include "gsb_common.cuh"
+#include "gsb_internal.h"
+#include "token_types.cuh"
+
+namespace gsb {
+
+// What happens to a sum z: scales (e4m3 operands), bias, copy of z for the backward, activation,
+// residual, rounding.  bias, res and out are of the output type.
+struct Epilogue {
+  const float* row_scale;
+  const float* col_scale;
+  const void* bias;
+  const void* res;
+  int64_t res_stride;
+  void* preact;
+  void* out;
+  int64_t out_stride;
+  int act;
+  int vec;  // out, preact, bias and res rows allow 16-byte accesses
+};
+
+// D = A B^T, A [m, k] and B [n, k]; *_mn: stored [k, m] ([k, n]) with the rows of k.
+struct Product {
+  const void* a;
+  int64_t a_ld;  // elements between stored rows
+  bool a_mn;
+  const void* b;
+  int64_t b_ld;
+  bool b_mn;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int dtype;      // of a and b: GSB_BF16, GSB_F16, GSB_E4M3; GSB_F32: three bf16 parts each
+  int out_dtype;
+  int64_t a_plane, b_plane;  // GSB_F32: elements between the parts
+};
+
+// The pre-activation kept for the backward: float beside float operands, else fp16 saturated at
+// its largest value.  fp16 and not bf16: its 11 bits keep the slope's error (at most 2^-11 |z|
+// act'') an eighth of the rounding that dz gets, and beyond +-65504 every slope is constant.
+__device__ __forceinline__ float as_preact(float*, float z) { return z; }
+__device__ __forceinline__ f16 as_preact(f16*, float z) {
+  uint16_t h;
+  asm("cvt.rn.satfinite.f16.f32 %0, %1;" : "=h"(h) : "f"(z));
+  return __ushort_as_half(h);
+}
+
+template <typename T>
+struct PreactOf { using type = f16; };
+template <>
+struct PreactOf<float> { using type = float; };
+
+template <int V>
+__device__ __forceinline__ void apply_act(int act, float (&z)[V]) {
+  switch (act) {
+    case GSB_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_RELU>(z[i]);
+      break;
+    case GSB_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_GELU>(z[i]);
+      break;
+    case GSB_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_GELU_TANH>(z[i]);
+      break;
+    case GSB_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_SILU>(z[i]);
+      break;
+    default: break;
+  }
+}
+
+// V adjacent sums of row i from column j on.
+template <typename O, int V>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t n, int64_t i, int64_t j, float (&z)[V]) {
+  using Z = typename PreactOf<O>::type;
+  if (e.row_scale) {
+    const float rs = e.row_scale[i];
+#pragma unroll
+    for (int u = 0; u < V; ++u) z[u] *= rs * e.col_scale[j + u];
+  }
+  if (e.bias) {
+    float b[V];
+    load_f32<O, V>(static_cast<const O*>(e.bias) + j, b);
+#pragma unroll
+    for (int u = 0; u < V; ++u) z[u] += b[u];
+  }
+  if (e.preact) {
+    Vec<Z, V> keep;
+#pragma unroll
+    for (int u = 0; u < V; ++u) keep.v[u] = as_preact(static_cast<Z*>(nullptr), z[u]);
+    *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) = keep;
+  }
+  apply_act<V>(e.act, z);
+  if (e.res) {
+    float r[V];
+    load_f32<O, V>(static_cast<const O*>(e.res) + i * e.res_stride + j, r);
+#pragma unroll
+    for (int u = 0; u < V; ++u) z[u] += r[u];
+  }
+  store_f32<O, V>(static_cast<O*>(e.out) + i * e.out_stride + j, z);
+}
+
+// Tensor-core product (linear_mma.cu).  The operands' rows (and parts) start on 16-byte boundaries.
+gsb_status mma_product(const Product& p, const Epilogue& e, cudaStream_t st);
+gsb_status mma_product_bf16(const Product& p, const Epilogue& e, cudaStream_t st);
+gsb_status mma_product_f16(const Product& p, const Epilogue& e, cudaStream_t st);
+gsb_status mma_product_f32(const Product& p, const Epilogue& e, cudaStream_t st);
+gsb_status mma_product_e4m3(const Product& p, const Epilogue& e, cudaStream_t st);
+// Device word (of the current device) that a kernel sets when a bounded wait gave up; NULL on error.
+int* mma_flag();
+// Its value.
+gsb_status mma_status(int* gave_up);
+
+}  // namespace gsb

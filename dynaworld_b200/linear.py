@@ -75,7 +75,7 @@ class _Linear(torch.autograd.Function):
         db = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
         p = ctypes.byref(_spec(x, weight, None, None, ctx.act, ctx.code, ctx.code))
         with on_device(dev), _stage("linear_bwd"):
-            ws = torch.empty(L.gsb_linear_bwd_workspace(p), dtype=torch.uint8, device=dev)
+            ws = torch.empty(L.gsb_linear_bwd_workspace(p, g.data_ptr(), g.stride(0)), dtype=torch.uint8, device=dev)
             _lib.check("gsb_linear_bwd", L.gsb_linear_bwd(
                 p, _lib.ptr(preact), g.data_ptr(), g.stride(0), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
                 ws.data_ptr(), ws.numel(), _stream(dev)))

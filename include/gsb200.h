@@ -462,7 +462,8 @@ GSB_API size_t gsb_linear_fwd_workspace(const gsb_linear* linear);
    saturated at its largest value for 16-bit ones (every activation is flat or linear there). */
 GSB_API gsb_status gsb_linear_fwd(const gsb_linear* linear, void* y, void* preact, void* workspace,
                                   size_t workspace_bytes, void* stream);
-GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear);
+GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear, const void* dy,
+                                        int64_t dy_stride);
 /* dz = dy act'(z), dx = dz weight, dweight = dz^T x, dbias = the column sums of dz; outputs that
    are NULL are not computed, all are contiguous and of dtype (not E4M3).  preact is read unless
    the activation is NONE.  dz is rounded to dtype before the two products (dbias sums it in
@@ -470,6 +471,11 @@ GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear);
 GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, const void* dy,
                                   int64_t dy_stride, void* dx, void* dweight, void* dbias,
                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* GSB_ERR_TIMEOUT once a bounded device-side wait of a matrix product gave up on the current device
+   since the library was loaded (the outputs of that call hold NaN where it happened), else GSB_OK.
+   Waits for the device's queued work. */
+GSB_API gsb_status gsb_linear_status(void);
 
 /* ---- utility: the library's radix sort on its own (tests, benchmarks) --------------------- */
 GSB_API size_t gsb_radix_sort_workspace(uint32_t n, int key_bytes, int with_values);

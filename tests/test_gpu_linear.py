@@ -364,3 +364,9 @@ def test_two_captured_graphs_replayed_together(m, t):
     for got, ref in zip(outs, refs):
         for a, b in zip(got, ref):
             assert torch.equal(a, b)
+
+
+def test_no_wait_gave_up():
+    x, w, b, r, dy = make(300, 264, 144, torch.bfloat16)
+    linear(x, w, b)
+    assert _lib.lib().gsb_linear_status() == _lib.GSB_OK
