@@ -24,9 +24,15 @@ def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     (any positive row stride), else a copy."""
     if t.ndim != 2:
         t = t.reshape(-1, width)
-    if (t.stride(1) != 1 and width > 1) or (t.shape[0] > 1 and t.stride(0) < 1):
+    down, along = t.stride()
+    if (along != 1 and width > 1) or (down < 1 and t.shape[0] > 1):
         t = t.contiguous()
     return t
+
+
+def workspace(like: torch.Tensor, nbytes: int) -> torch.Tensor | None:
+    """Scratch on the device of ``like``, or None when none is needed."""
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def check_input(what: str, x: torch.Tensor) -> int:
@@ -45,7 +51,7 @@ def check_device(what: str, x: torch.Tensor) -> None:
 
 
 def check_like(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")

@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libgsb200.so"
 SOURCES = ["abi.cu", "preprocess.cu", "sort.cu", "bin.cu", "raster.cu", "loss.cu", "splat2d.cu",
-           "norm.cu", "linear.cu", "linear_mma.cu", "linear_mma_bf16.cu", "linear_mma_f16.cu",
+           "norm.cu", "norm_ring.cu", "linear.cu", "linear_mma.cu", "linear_mma_bf16.cu", "linear_mma_f16.cu",
            "linear_mma_f32.cu", "linear_mma_e4m3.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -625,6 +625,6 @@ GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, 
   return linear_bwd(linear, preact, dy, dy_stride, dx, dweight, dbias, workspace, workspace_bytes, as_stream(stream));
 }
 
-GSB_API gsb_status gsb_linear_status(void) { return linear_status(); }
+GSB_API gsb_status gsb_token_status(void) { return token_status(); }
 
 }  // extern "C"

@@ -323,7 +323,7 @@ FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
     if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
     if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
   }
-  s.bytes = std::max(c.used, kAlign);
+  s.bytes = c.used;
   return s;
 }
 
@@ -454,8 +454,8 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
     }
     return launch_status();
   }
-  if (!ws || ws_bytes < linear_fwd_workspace(p)) return GSB_ERR_WORKSPACE;
   const FwdSpace s = fwd_space(*p, ws, ws_bytes);
+  if (s.bytes && (!ws || ws_bytes < s.bytes)) return GSB_ERR_WORKSPACE;
   Ready x, w;
   ready_pair(job_of(p->x, p->x_stride, p->m, p->k, p->dtype, s.x),
              job_of(p->weight, p->weight_stride, p->n, p->k, p->dtype, s.w), p->dtype, x, w, st);
@@ -485,9 +485,9 @@ gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, i
   return bwd(*p, preact, dy, dy_stride, dx, dweight, dbias, bwd_space(*p, dy, dy_stride, ws, ws_bytes), st);
 }
 
-gsb_status linear_status() {
+gsb_status token_status() {
   int gave_up = 0;
-  if (gsb_status s = mma_status(&gave_up); s != GSB_OK) return s;
+  if (gsb_status s = gave_up_status(&gave_up); s != GSB_OK) return s;
   return gave_up ? GSB_ERR_TIMEOUT : GSB_OK;
 }
 

@@ -22,7 +22,7 @@ EncodeFn encode_fn() {
 
 static __device__ int g_gave_up;
 
-int* mma_flag() {
+int* gave_up_flag() {
   static std::atomic<int*> at[64];  // by device
   int dev = 0;
   (void)cudaGetDevice(&dev);
@@ -37,7 +37,7 @@ int* mma_flag() {
   return static_cast<int*>(q);
 }
 
-gsb_status mma_status(int* gave_up) {
+gsb_status gave_up_status(int* gave_up) {
   if (cudaMemcpyFromSymbol(gave_up, g_gave_up, sizeof(int)) != cudaSuccess) {
     (void)cudaGetLastError();
     return GSB_ERR_CUDA;

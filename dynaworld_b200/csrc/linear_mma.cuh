@@ -24,6 +24,7 @@
 
 #include <atomic>
 
+#include "async_copy.cuh"
 #include "linear_parts.cuh"
 
 namespace gsb {
@@ -36,7 +37,6 @@ constexpr int kStageBytes = kEpiWarps * 32 * kPitch * 4;
 constexpr int kRowBytes = 128;              // one swizzled row of a box
 constexpr int kABytes = 128 * kRowBytes;
 constexpr int kChunk = 4;                   // PLANES = 3: blocks of 64 k per accumulation chain
-constexpr uint64_t kWaitNs = 4000000000ull;
 
 
 struct Args {
@@ -51,8 +51,6 @@ struct Args {
 };
 
 // ---- PTX ----
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -70,48 +68,9 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
 // bar: an address in the cluster's shared window
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait; false when it gave up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* gave_up) {
-  for (int i = 0; i < 256; ++i)
-    if (bar_try(bar, parity)) return true;
-  const uint64_t t0 = now_ns();
-  while (now_ns() - t0 < kWaitNs) {
-    for (int i = 0; i < 64; ++i)
-      if (bar_try(bar, parity)) return true;
-  }
-  atomicExch(gave_up, 1);
-  return false;
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -463,8 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = bar_wait(empty(s), phase ^ 1, p.gave_up);
         if (++s == S::kSlots) s = 0, phase ^= 1;
       }
-      if (!ok)
-        for (int i = 0; i < 1000; ++i) __nanosleep(10000);  // copies in flight land before the CTA ends
+      if (!ok) let_copies_land();
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
@@ -671,7 +629,7 @@ gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
   a.tiles = int64_t(a.m_tiles) * a.n_tiles;
   a.group = 8;
   a.idesc = instr_desc(p.dtype, A_MN, B_MN, 128 * CG, BN);
-  a.gave_up = mma_flag();
+  a.gave_up = gave_up_flag();
   if (!a.gave_up) return GSB_ERR_CUDA;
   a.e = e;
   const int clusters = int(std::min<int64_t>(a.tiles, sm_count() / CG));

@@ -114,9 +114,7 @@ gsb_status mma_product_bf16(const Product& p, const Epilogue& e, cudaStream_t st
 gsb_status mma_product_f16(const Product& p, const Epilogue& e, cudaStream_t st);
 gsb_status mma_product_f32(const Product& p, const Epilogue& e, cudaStream_t st);
 gsb_status mma_product_e4m3(const Product& p, const Epilogue& e, cudaStream_t st);
-// Device word (of the current device) that a kernel sets when a bounded wait gave up; NULL on error.
-int* mma_flag();
-// Its value.
-gsb_status mma_status(int* gave_up);
+// 1 once a bounded wait of a token-side kernel gave up on the current device.
+gsb_status gave_up_status(int* gave_up);
 
 }  // namespace gsb

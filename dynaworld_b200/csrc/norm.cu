@@ -12,89 +12,13 @@
 // above that, and above what 256 threads hold in registers it is walked twice (the second walk
 // finds it in L2).  Blocks walk rows with a grid stride so that the weight, and in the backward the
 // weight gradient's partial sums, stay in registers over all rows of a block.
-#include "gsb_common.cuh"
-#include "gsb_internal.h"
-#include "token_types.cuh"
+#include "norm_parts.cuh"
+
+#include <type_traits>
 
 namespace gsb {
 
 namespace {
-
-constexpr int kThreads = 256;
-constexpr float kTiny = 1e-30f;   // a row of zeros gets the scale 1e-30 / 448 and codes 0
-constexpr float kE4M3Max = 448.0f;
-
-struct NormArgs {
-  int64_t rows;
-  int dim;
-  float eps, inv_dim;
-  const void* x;
-  int64_t x_stride;
-  const void* res;
-  int64_t res_stride;
-  const void* w;
-  void* y;        // [rows, dim]: values or e4m3 codes
-  void* sum;      // [rows, dim] or NULL
-  float* rstd;    // [rows] or NULL (forward); read in the backward
-  float* scale;   // [rows], e4m3 outputs
-  const void* dy;
-  int64_t dy_stride;
-  const void* dsum;  // or NULL
-  int64_t dsum_stride;
-  void* dx;       // [rows, dim]
-  float* dw_part; // [blocks, dim]
-};
-
-// Sum / unsigned maximum over the GROUP threads (a warp or the block) that share a row.
-template <int GROUP>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-  v = warp_sum(v);
-  if constexpr (GROUP > 32) {
-    constexpr int W = GROUP / 32;
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();  // the previous use of red has been read
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) v += red[i];
-  }
-  return v;
-}
-
-template <int GROUP>
-__device__ __forceinline__ uint32_t group_max(uint32_t v, float* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if constexpr (GROUP > 32) {
-    constexpr int W = GROUP / 32;
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[warp] = __uint_as_float(v);
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) v = max(v, __float_as_uint(red[i]));
-  }
-  return v;
-}
-
-// |v| as bits: their unsigned order is the order of the magnitudes with NaN above infinity, so a
-// maximum over them keeps a NaN.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-template <int V>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[V], float inv) {
-  if constexpr (V == 1) {
-    *p = e4m3x1(y[0] * inv);
-  } else {
-    Vec<uint16_t, V / 2> c;
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) c.v[i] = e4m3x2(y[2 * i] * inv, y[2 * i + 1] * inv);
-    *reinterpret_cast<Vec<uint16_t, V / 2>*>(p) = c;
-  }
-}
-
-enum { kNorm = 0, kNormFp8 = 1, kQuantize = 2 };
 
 // One row per GROUP threads, held in registers: access j of lane t covers elements
 // (j GROUP + t) V .. + V.
@@ -221,7 +145,8 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(NormArgs a) {
   }
 }
 
-// Backward of one row per GROUP threads.  x is the stream h as the forward wrote it.  Every thread
+// Backward of one row per GROUP threads.  h is formed again from x and the residual (the rounded
+// stream would put half a step of error into every term of dw and dx).  Every thread
 // adds its columns' dy h rstd over its rows in registers; a block's threads of one column are
 // added in shared memory in a fixed order and leave one row of dw_part, so the weight gradient is
 // the same on every run.
@@ -244,13 +169,27 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(NormArgs a) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     const float rstd = a.rstd[row];
-    Vec<T, V> h[PV], g[PV], ds[PV];
+    Vec<T, V> g[PV], ds[PV];
+    float h[PV][V];
 #pragma unroll
     for (int j = 0; j < PV; ++j) {
       const int i = j * GROUP + t;
       if (i < nv) {
-        h[j] = *reinterpret_cast<const Vec<T, V>*>(x + int64_t(i) * V);
+        load_f32<T, V>(x + int64_t(i) * V, h[j]);
         g[j] = *reinterpret_cast<const Vec<T, V>*>(dy + int64_t(i) * V);
+      }
+    }
+    if (a.res) {
+      const T* r = static_cast<const T*>(a.res) + row * a.res_stride;
+#pragma unroll
+      for (int j = 0; j < PV; ++j) {
+        const int i = j * GROUP + t;
+        if (i < nv) {
+          float rv[V];
+          load_f32<T, V>(r + int64_t(i) * V, rv);
+#pragma unroll
+          for (int e = 0; e < V; ++e) h[j][e] += rv[e];
+        }
       }
     }
     if (a.dsum) {
@@ -267,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(NormArgs a) {
       if (j * GROUP + t < nv) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float gh = to_f32(g[j].v[e]) * to_f32(h[j].v[e]);
+          const float gh = to_f32(g[j].v[e]) * h[j][e];
           dot = fmaf(gh, to_f32(w[j].v[e]), dot);
           acc[j][e] = fmaf(gh, rstd, acc[j][e]);
         }
@@ -281,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(NormArgs a) {
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          o[e] = rstd * (to_f32(g[j].v[e]) * to_f32(w[j].v[e]) - to_f32(h[j].v[e]) * c);
+          o[e] = rstd * (to_f32(g[j].v[e]) * to_f32(w[j].v[e]) - h[j][e] * c);
           if (a.dsum) o[e] += to_f32(ds[j].v[e]);
         }
         store_f32<T, V>(static_cast<T*>(a.dx) + row * a.dim + int64_t(i) * V, o);
@@ -322,13 +261,15 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_wide_kernel(NormArgs a) {
   const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
   const T* d = a.dsum ? static_cast<const T*>(a.dsum) + row * a.dsum_stride : nullptr;
   const T* w = static_cast<const T*>(a.w);
+  const T* r = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
+  const auto h = [&](int i) { return r ? to_f32(x[i]) + to_f32(r[i]) : to_f32(x[i]); };
   const float rstd = a.rstd[row];
   float dot = 0.0f;
-  for (int i = threadIdx.x; i < a.dim; i += kThreads) dot = fmaf(to_f32(dy[i]) * to_f32(x[i]), to_f32(w[i]), dot);
+  for (int i = threadIdx.x; i < a.dim; i += kThreads) dot = fmaf(to_f32(dy[i]) * h(i), to_f32(w[i]), dot);
   dot = group_sum<kThreads>(dot, red);
   const float c = rstd * rstd * (dot * a.inv_dim);
   for (int i = threadIdx.x; i < a.dim; i += kThreads) {
-    float o = rstd * (to_f32(dy[i]) * to_f32(w[i]) - to_f32(x[i]) * c);
+    float o = rstd * (to_f32(dy[i]) * to_f32(w[i]) - h(i) * c);
     if (d) o += to_f32(d[i]);
     static_cast<T*>(a.dx)[row * a.dim + i] = from_f32<T>(o);
   }
@@ -341,9 +282,11 @@ __global__ void __launch_bounds__(kThreads) norm_dw_wide_kernel(NormArgs a, int6
   if (i >= a.dim) return;
   const int64_t lo = blockIdx.y * rows_per_part, hi = min(a.rows, lo + rows_per_part);
   float s = 0.0f;
-  for (int64_t row = lo; row < hi; ++row)
-    s = fmaf(to_f32(static_cast<const T*>(a.dy)[row * a.dy_stride + i]) *
-                 to_f32(static_cast<const T*>(a.x)[row * a.x_stride + i]), a.rstd[row], s);
+  for (int64_t row = lo; row < hi; ++row) {
+    float h = to_f32(static_cast<const T*>(a.x)[row * a.x_stride + i]);
+    if (a.res) h += to_f32(static_cast<const T*>(a.res)[row * a.res_stride + i]);
+    s = fmaf(to_f32(static_cast<const T*>(a.dy)[row * a.dy_stride + i]) * h, a.rstd[row], s);
+  }
   a.dw_part[int64_t(blockIdx.y) * a.dim + i] = s;
 }
 
@@ -402,6 +345,8 @@ gsb_status fwd_of_type(const NormArgs& a, cudaStream_t st) {
   constexpr int E = sizeof(T);
   bool ok = a.dim % (16 / E) == 0 && vec_ok(a.x, a.x_stride, E, 16) && (!a.res || vec_ok(a.res, a.res_stride, E, 16)) &&
             vec_ok(a.w, 0, E, 16) && vec_ok(a.sum, 0, E, 16) && vec_ok(a.y, 0, E, 16);
+  const int code = sizeof(T) == 4 ? GSB_F32 : std::is_same<T, bf16>::value ? GSB_BF16 : GSB_F16;
+  if (ok && ring_fwd(a, code, MODE, st)) return launch_status();
   const Split s = split_of(a.dim, E, ok);
   if (s.group == 0)
     norm_fwd_wide_kernel<T, MODE><<<unsigned(a.rows), kThreads, 0, st>>>(a);
@@ -446,9 +391,17 @@ template <typename T>
 gsb_status bwd_of_type(const NormArgs& a, void* dw, cudaStream_t st) {
   constexpr int E = sizeof(T);
   const bool ok = a.dim % (16 / E) == 0 && vec_ok(a.x, a.x_stride, E, 16) && vec_ok(a.dy, a.dy_stride, E, 16) &&
-                  (!a.dsum || vec_ok(a.dsum, a.dsum_stride, E, 16)) && vec_ok(a.w, 0, E, 16) && vec_ok(a.dx, 0, E, 16);
+                  (!a.res || vec_ok(a.res, a.res_stride, E, 16)) && (!a.dsum || vec_ok(a.dsum, a.dsum_stride, E, 16)) && vec_ok(a.w, 0, E, 16) && vec_ok(a.dx, 0, E, 16);
+  const int code = sizeof(T) == 4 ? GSB_F32 : std::is_same<T, bf16>::value ? GSB_BF16 : GSB_F16;
   const Split s = split_of(a.dim, E, ok);
   int parts;
+  if (ok && ring_bwd(a, code, &parts, st)) {
+    if (dw) {
+      column_sum_kernel<T><<<(a.dim + 31) / 32, 256, 0, st>>>(a.dw_part, parts, a.dim, static_cast<T*>(dw));
+      note_launch();
+    }
+    return launch_status();
+  }
   if (s.group == 0) {
     norm_bwd_wide_kernel<T><<<unsigned(a.rows), kThreads, 0, st>>>(a);
     note_launch();
@@ -527,7 +480,7 @@ gsb_status quantize_rows_fp8(const gsb_norm* n, void* codes, float* scales, cuda
 
 size_t rms_norm_bwd_workspace(const gsb_norm* n) {
   if (check_norm(n) != GSB_OK) return 0;
-  const size_t parts = std::max<size_t>(kWideParts, bwd_blocks(n->rows, 1));
+  const size_t parts = std::max<size_t>(kWideParts, bwd_blocks(n->rows, 1));  // at least one per SM: the ring's too
   return align_up(parts * size_t(n->dim) * 4);
 }
 
@@ -542,7 +495,6 @@ gsb_status rms_norm_bwd(const gsb_norm* n, const float* rstd, const void* dy, in
   if (!rstd || !dy || !dx || !ws) return GSB_ERR_ARG;
   if (ws_bytes < rms_norm_bwd_workspace(n)) return GSB_ERR_WORKSPACE;
   NormArgs a = args_of(*n);
-  a.res = nullptr;
   a.rstd = const_cast<float*>(rstd);
   a.dy = dy;
   a.dy_stride = dy_stride;

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import E4M3, TYPE_CODES, check_device, check_input, check_like, on_device, rows_of
+from ._rows import E4M3, TYPE_CODES, check_device, check_input, check_like, on_device, rows_of, workspace
 from .norm import _refuse_grad
 from .render import _stage, _stream
 
@@ -34,27 +34,25 @@ def _spec(x, weight, bias, residual, act, code, out_code, x_scale=None, weight_s
                        0 if residual is None else residual.stride(0), _lib.ptr(x_scale), _lib.ptr(weight_scale))
 
 
-def _run_forward(spec, rows: int, n: int, dtype, dev, preact) -> torch.Tensor:
+def _run_forward(spec, y: torch.Tensor, preact: torch.Tensor | None) -> None:
     L = _lib.lib()
-    y = torch.empty((rows, n), dtype=dtype, device=dev)
+    dev = y.device
     p = ctypes.byref(spec)
     with on_device(dev), _stage("linear"):
-        ws = torch.empty(L.gsb_linear_fwd_workspace(p), dtype=torch.uint8, device=dev)
-        _lib.check("gsb_linear_fwd", L.gsb_linear_fwd(p, y.data_ptr(), _lib.ptr(preact), ws.data_ptr(), ws.numel(),
+        nbytes = L.gsb_linear_fwd_workspace(p)
+        ws = workspace(y, nbytes)
+        _lib.check("gsb_linear_fwd", L.gsb_linear_fwd(p, y.data_ptr(), _lib.ptr(preact), _lib.ptr(ws), nbytes,
                                                       _stream(dev)))
-    return y
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, code):
-        dev = x.device
+        y = x.new_empty((x.shape[0], weight.shape[0]))
         preact = None
         if act and any(ctx.needs_input_grad[:3]):
-            preact = torch.empty((x.shape[0], weight.shape[0]), device=dev,
-                                 dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
-        y = _run_forward(_spec(x, weight, bias, residual, act, code, code), x.shape[0], weight.shape[0], x.dtype, dev,
-                         preact)
+            preact = y.new_empty(y.shape, dtype=torch.float32 if code == _lib.F32 else torch.float16)
+        _run_forward(_spec(x, weight, bias, residual, act, code, code), y, preact)
         ctx.act, ctx.code = act, code
         ctx.save_for_backward(x, weight, preact)
         return y
@@ -70,15 +68,16 @@ class _Linear(torch.autograd.Function):
         dev = x.device
         n, k = weight.shape
         g = rows_of(dy, n)
-        dx = torch.empty((x.shape[0], k), dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
+        dx = x.new_empty((x.shape[0], k)) if need_x else None
+        dw = x.new_empty((n, k)) if need_w else None
+        db = x.new_empty(n) if need_b else None
         p = ctypes.byref(_spec(x, weight, None, None, ctx.act, ctx.code, ctx.code))
+        gp, gs = g.data_ptr(), g.stride(0)
         with on_device(dev), _stage("linear_bwd"):
-            ws = torch.empty(L.gsb_linear_bwd_workspace(p, g.data_ptr(), g.stride(0)), dtype=torch.uint8, device=dev)
-            _lib.check("gsb_linear_bwd", L.gsb_linear_bwd(
-                p, _lib.ptr(preact), g.data_ptr(), g.stride(0), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
-                ws.data_ptr(), ws.numel(), _stream(dev)))
+            nbytes = L.gsb_linear_bwd_workspace(p, gp, gs)
+            ws = workspace(x, nbytes)
+            _lib.check("gsb_linear_bwd", L.gsb_linear_bwd(p, _lib.ptr(preact), gp, gs, _lib.ptr(dx), _lib.ptr(dw),
+                                                          _lib.ptr(db), _lib.ptr(ws), nbytes, _stream(dev)))
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -117,9 +116,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (b is not None and b.requires_grad)
                                     or (r2 is not None and r2.requires_grad)):
         y = _Linear.apply(x2, w2, b, r2, act, code)
-    else:
-        y = _run_forward(_spec(x2, w2, b, r2, act, code, code), x2.shape[0], n, x.dtype, x.device, None)
-    return y.view(*x.shape[:-1], n)
+        return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
+    y = x.new_empty((*x.shape[:-1], n))
+    _run_forward(_spec(x2, w2, b, r2, act, code, code), y, None)
+    return y
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -144,6 +144,6 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     x2, w2 = rows_of(x, x.shape[-1]), rows_of(weight, weight.shape[1])
     r2 = None if residual is None else rows_of(residual, n)
     b = None if bias is None else bias.contiguous()
-    y = _run_forward(_spec(x2, w2, b, r2, act, _lib.E4M3, out_code, x_scale.contiguous(), weight_scale.contiguous()),
-                     x2.shape[0], n, dtype, x.device, None)
-    return y.view(*x.shape[:-1], n)
+    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    _run_forward(_spec(x2, w2, b, r2, act, _lib.E4M3, out_code, x_scale.contiguous(), weight_scale.contiguous()), y, None)
+    return y

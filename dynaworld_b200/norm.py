@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import E4M3, check_device, check_input, check_like, on_device, rows_of
+from ._rows import E4M3, check_device, check_input, check_like, on_device, rows_of, workspace
 from .render import _stage, _stream
 
 
@@ -27,9 +27,9 @@ def _forward(x, weight, residual, eps, code, need_rstd):
     """x [rows, dim] -> y, summed (None without a residual), rstd (None unless needed)."""
     L = _lib.lib()
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    summed = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(x.shape[0], dtype=torch.float32, device=dev) if need_rstd else None
+    y = x.new_empty(x.shape)
+    summed = None if residual is None else x.new_empty(x.shape)
+    rstd = x.new_empty(x.shape[0], dtype=torch.float32) if need_rstd else None
     with on_device(dev), _stage("rms_norm"):
         _lib.check("gsb_rms_norm_fwd", L.gsb_rms_norm_fwd(
             ctypes.byref(_norm(x, code, eps, residual, weight)), y.data_ptr(), _lib.ptr(summed), _lib.ptr(rstd),
@@ -43,30 +43,32 @@ class _RmsNorm(torch.autograd.Function):
         y, summed, rstd = _forward(x, weight, residual, eps, code, True)
         ctx.eps, ctx.code = eps, code
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if summed is None else summed, weight, rstd)
+        ctx.save_for_backward(x, residual, weight, rstd)
         return y, summed
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dsummed):
-        h, weight, rstd = ctx.saved_tensors
+        x, residual, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:  # only the stream was used
             return (dsummed if need_x else None, None if not need_w else torch.zeros_like(weight),
                     dsummed if need_r else None, None, None)
         L = _lib.lib()
-        dev = h.device
-        dim = h.shape[1]
+        dev = x.device
+        dim = x.shape[1]
         dy = rows_of(dy, dim)
         dsummed = None if dsummed is None else rows_of(dsummed, dim)
-        dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
-        dw = torch.empty(dim, dtype=weight.dtype, device=dev) if need_w else None
-        norm = _norm(h, ctx.code, ctx.eps, None, weight)
+        dx = x.new_empty(x.shape)
+        dw = weight.new_empty(dim) if need_w else None
+        norm = _norm(x, ctx.code, ctx.eps, residual, weight)
+        p = ctypes.byref(norm)
         with on_device(dev), _stage("rms_norm_bwd"):
-            ws = torch.empty(L.gsb_rms_norm_bwd_workspace(ctypes.byref(norm)), dtype=torch.uint8, device=dev)
+            nbytes = L.gsb_rms_norm_bwd_workspace(p)
+            ws = workspace(x, nbytes)
             _lib.check("gsb_rms_norm_bwd", L.gsb_rms_norm_bwd(
-                ctypes.byref(norm), rstd.data_ptr(), dy.data_ptr(), dy.stride(0), _lib.ptr(dsummed),
-                0 if dsummed is None else dsummed.stride(0), dx.data_ptr(), _lib.ptr(dw), ws.data_ptr(), ws.numel(),
+                p, rstd.data_ptr(), dy.data_ptr(), dy.stride(0), _lib.ptr(dsummed),
+                0 if dsummed is None else dsummed.stride(0), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(ws), nbytes,
                 _stream(dev)))
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
@@ -89,7 +91,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
     x and residual [..., D], weight [D], all float32, bfloat16 or float16 of one type.  Returns y,
     or with a residual the pair (y, h): h is the new residual stream.  The sum, the statistics and
     the product are formed in float; y and h are rounded once.  Differentiable in x, weight and
-    residual (once; the backward uses h as returned); the weight gradient is the same on every run."""
+    residual (once; the backward forms h again from x and residual); the weight gradient is the same on every run."""
     code = _check("rms_norm", x, weight, residual, eps)
     dim = x.shape[-1]
     x2 = rows_of(x, dim)
@@ -100,8 +102,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
         y, h = _RmsNorm.apply(x2, w, r2, float(eps), code)
     else:
         y, h, _ = _forward(x2, w, r2, float(eps), code, False)
-    y = y.view(x.shape)
-    return y if residual is None else (y, h.view(x.shape))
+    if x.ndim != 2:
+        y, h = y.view(x.shape), None if h is None else h.view(x.shape)
+    return y if residual is None else (y, h)
 
 
 def _refuse_grad(what, *tensors):
@@ -121,9 +124,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tenso
     x2 = rows_of(x, dim)
     r2 = None if residual is None else rows_of(residual, dim)
     w = weight.contiguous()
-    q = torch.empty(x.shape, dtype=E4M3, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    q = x.new_empty(x.shape, dtype=E4M3)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    h = None if residual is None else x.new_empty(x.shape)
     with on_device(dev), _stage("rms_norm_fp8"):
         _lib.check("gsb_rms_norm_fp8", L.gsb_rms_norm_fp8(
             ctypes.byref(_norm(x2, code, float(eps), r2, w)), q.data_ptr(), scale.data_ptr(), _lib.ptr(h),
@@ -140,8 +143,8 @@ def quantize_rows_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     L = _lib.lib()
     dev, dim = x.device, x.shape[-1]
     x2 = rows_of(x, dim)
-    q = torch.empty(x.shape, dtype=E4M3, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    q = x.new_empty(x.shape, dtype=E4M3)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     with on_device(dev), _stage("quantize_rows_fp8"):
         _lib.check("gsb_quantize_rows_fp8", L.gsb_quantize_rows_fp8(
             ctypes.byref(_norm(x2, code, 0.0, None, None)), q.data_ptr(), scale.data_ptr(), _stream(dev)))

@@ -412,8 +412,8 @@ typedef struct gsb_norm {
 GSB_API gsb_status gsb_rms_norm_fwd(const gsb_norm* norm, void* y, void* summed, float* rstd,
                                     void* stream);
 GSB_API size_t gsb_rms_norm_bwd_workspace(const gsb_norm* norm);
-/* norm->x is h (x, or `summed` where there was a residual); dy and dsummed (or NULL) the gradients
-   of y and summed.  dx is the gradient of x and of the residual.  dweight may be NULL.  The same
+/* The same norm as the forward's (h is formed again from x and residual, unrounded); dy and dsummed
+   (or NULL) the gradients of y and summed.  dx is the gradient of x and of the residual.  dweight may be NULL.  The same
    inputs give the same bits. */
 GSB_API gsb_status gsb_rms_norm_bwd(const gsb_norm* norm, const float* rstd, const void* dy,
                                     int64_t dy_stride, const void* dsummed, int64_t dsummed_stride,
@@ -472,10 +472,10 @@ GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, 
                                   int64_t dy_stride, void* dx, void* dweight, void* dbias,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
-/* GSB_ERR_TIMEOUT once a bounded device-side wait of a matrix product gave up on the current device
+/* GSB_ERR_TIMEOUT once a bounded device-side wait of a token-side operator gave up on the current device
    since the library was loaded (the outputs of that call hold NaN where it happened), else GSB_OK.
    Waits for the device's queued work. */
-GSB_API gsb_status gsb_linear_status(void);
+GSB_API gsb_status gsb_token_status(void);
 
 /* ---- utility: the library's radix sort on its own (tests, benchmarks) --------------------- */
 GSB_API size_t gsb_radix_sort_workspace(uint32_t n, int key_bytes, int with_values);

@@ -369,4 +369,4 @@ def test_two_captured_graphs_replayed_together(m, t):
 def test_no_wait_gave_up():
     x, w, b, r, dy = make(300, 264, 144, torch.bfloat16)
     linear(x, w, b)
-    assert _lib.lib().gsb_linear_status() == _lib.GSB_OK
+    assert _lib.lib().gsb_token_status() == _lib.GSB_OK

@@ -3,8 +3,7 @@
 Bounds.  u = 2^-24 is half a float step; half(t) half a relative step of the type t.  A sum over D
 values with at most 64 of them added one after the other per thread and the rest in trees is within
 80 u of the sum of magnitudes; with the handful of roundings after it every factor below is within
-128 u.  The stream h that the backward reads is rounded to the type first (half(t) per value) when
-there is a residual; that enters the backward's two h terms once each."""
+128 u.  The backward forms h from x and the residual, unrounded."""
 import pytest
 import torch
 
@@ -64,18 +63,16 @@ def check_all(x, r, w, dy, dh, t):
     mag = (G * W * H).abs().sum(-1, keepdim=True) / D
     dx = rstd * (G * W - H * rstd.square() * dot)
     terms = rstd * ((G * W).abs() + H.abs() * rstd.square() * mag)
-    stored = 0.0 if r is None else half(t)
-    extra = 2 * stored * rstd * H.abs() * rstd.square() * mag
     if r is not None:
         dx = dx + dh.double()
         terms = terms + dh.double().abs()
-    within(grads[0], dx, dx.abs() * half(t) + 128 * U * terms + extra * 1.01 + tiny(t))
+    within(grads[0], dx, dx.abs() * half(t) + 128 * U * terms + tiny(t))
     if r is not None:
         assert torch.equal(grads[2], grads[0])
     dw = (G * H * rstd).reshape(-1, D).sum(0)
     mag = (G * H * rstd).abs().reshape(-1, D).sum(0)
     rows = x.numel() // D
-    within(grads[1], dw, dw.abs() * half(t) + mag * (stored * 1.01 + (rows + 128) * U) + tiny(t))
+    within(grads[1], dw, dw.abs() * half(t) + mag * ((rows + 128) * U) + tiny(t))
 
 
 # one value, one access, a warp's row, odd widths (scalar accesses), a block's row, rows wider than
@@ -89,6 +86,25 @@ SHAPES = [(1, 1), (3, 8), (5, 31), (1, 1024), (33, 257), (1000, 512), (7, 515), 
 @pytest.mark.parametrize("residual", [True, False])
 def test_norm_and_gradients(rows, dim, t, residual):
     check_all(*make(rows, dim, t, seed=dim, residual=residual), t)
+
+
+# many aligned rows: a warp per row (two, four and, forward, eight accesses), a block per row; row
+# counts that leave the last round ragged; rows apart in a wider tensor
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,dim", [(4739, 256), (9500, 520), (4800, 1024), (5001, 2048), (1000, 2080), (700, 4096),
+                                      (611, 8192), (601, 16384)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_many_rows(rows, dim, t, residual):
+    x, r, w, dy, dh = make(rows, dim, t, seed=rows, residual=residual)
+    wide = torch.full((rows, dim + 64), float("nan"), dtype=t, device=DEV)
+    wide[:, 32:32 + dim] = x
+    part = wide[:, 32:32 + dim]
+    check_all(x, r, w, dy, dh, t)
+    got, ref = rms_norm(part, w, eps=EPS), rms_norm(x, w, eps=EPS)
+    assert torch.equal(got, ref)
+    q, s = quantize_rows_fp8(part)
+    rq, rs = ref_codes(x.float())
+    assert torch.equal(s, rs) and torch.equal(q.view(torch.uint8), rq.view(torch.uint8))
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -194,7 +210,7 @@ def test_quantised_special_rows(t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("rows,dim", SHAPES)
+@pytest.mark.parametrize("rows,dim", SHAPES + [(4800, 1024), (5001, 2048), (700, 4096), (601, 16384)])
 @pytest.mark.parametrize("residual", [True, False])
 def test_norm_in_8_bits(rows, dim, t, residual):
     x, r, w, _, _ = make(rows, dim, t, seed=dim + 1, residual=residual)
