@@ -112,13 +112,20 @@ struct CopyJob {
   void* out;
 };
 
-// Rows copied to a pitch that TMA takes (16-bit and 8-bit values), one value per thread and step.
+// Rows of up to two matrices copied to a pitch that TMA takes (16-bit and 8-bit values): a warp per
+// row, the unaligned reads a value per lane.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(CopyJob a) {
-  const int64_t total = a.rows * a.cols;
-  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
-    const int64_t i = t / a.cols, j = t - i * a.cols;
-    static_cast<T*>(a.out)[i * a.pitch + j] = static_cast<const T*>(a.in)[i * a.stride + j];
+__global__ void __launch_bounds__(256) pack_kernel(CopyJob a, CopyJob b, int a_blocks) {
+  const bool second = blockIdx.x >= a_blocks;
+  const CopyJob& s = second ? b : a;
+  const int64_t block = second ? blockIdx.x - a_blocks : blockIdx.x;
+  const int64_t blocks = second ? gridDim.x - a_blocks : a_blocks;
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = block * 8 + (threadIdx.x >> 5); i < s.rows; i += blocks * 8) {
+    const T* in = static_cast<const T*>(s.in) + i * s.stride;
+    T* out = static_cast<T*>(s.out) + i * s.pitch;
+#pragma unroll 8
+    for (int64_t j = lane; j < s.cols; j += 32) out[j] = in[j];
   }
 }
 
@@ -162,15 +169,16 @@ CopyJob job_of(const void* in, int64_t stride, int64_t rows, int64_t cols, int d
 }
 
 void split(const CopyJob& a, const CopyJob& b, cudaStream_t st) {
-  const int na = copy_blocks(a.rows * (a.pitch / 4)), nb = b.rows ? copy_blocks(b.rows * (b.pitch / 4)) : 0;
+  const int na = a.rows ? copy_blocks(a.rows * (a.pitch / 4)) : 0, nb = b.rows ? copy_blocks(b.rows * (b.pitch / 4)) : 0;
   split_kernel<<<na + nb, 256, 0, st>>>(a, b, na);
   note_launch();
 }
 
-void pack(const CopyJob& a, int dtype, cudaStream_t st) {
-  const int blocks = copy_blocks(a.rows * a.cols);
-  if (dtype == GSB_E4M3) pack_kernel<uint8_t><<<blocks, 256, 0, st>>>(a);
-  else pack_kernel<uint16_t><<<blocks, 256, 0, st>>>(a);
+void pack(const CopyJob& a, const CopyJob& b, int dtype, cudaStream_t st) {
+  const int na = a.rows ? copy_blocks(a.rows * 32) : 0, nb = b.rows ? copy_blocks(b.rows * 32) : 0;
+  if (na + nb == 0) return;
+  if (dtype == GSB_E4M3) pack_kernel<uint8_t><<<na + nb, 256, 0, st>>>(a, b, na);
+  else pack_kernel<uint16_t><<<na + nb, 256, 0, st>>>(a, b, na);
   note_launch();
 }
 
@@ -181,19 +189,16 @@ struct Ready {
 };
 
 // Two operands at once: in place where their rows are aligned, else copied (split) to the space given.
-void ready_pair(const CopyJob& a, const CopyJob& b, int dtype, Ready& ra, Ready& rb, cudaStream_t st) {
-  const CopyJob* jobs[2] = {&a, &b};
-  Ready* outs[2] = {&ra, &rb};
+void ready_pair(CopyJob a, CopyJob b, int dtype, Ready& ra, Ready& rb, cudaStream_t st) {
+  const auto in_place = [&](CopyJob& s, Ready& r) {
+    const bool fits = fits_tma(s.in, s.stride, dtype);
+    r = fits ? Ready{s.in, s.stride, 0} : Ready{s.out, s.pitch, s.rows * s.pitch};
+    if (fits) s.rows = 0;
+  };
+  in_place(a, ra);
+  in_place(b, rb);
   if (dtype == GSB_F32) split(a, b, st);
-  for (int i = 0; i < 2; ++i) {
-    const CopyJob& s = *jobs[i];
-    if (fits_tma(s.in, s.stride, dtype)) {
-      *outs[i] = {s.in, s.stride, 0};
-      continue;
-    }
-    if (dtype != GSB_F32 && s.rows) pack(s, dtype, st);
-    *outs[i] = {s.out, s.pitch, s.rows * s.pitch};
-  }
+  else pack(a, b, dtype, st);
 }
 
 // ---- backward: dz and the bias gradient -------------------------------------------------------
@@ -312,9 +317,29 @@ int dz_parts(int64_t m, int n, int dtype) {
 // ---- workspaces -------------------------------------------------------------------------------
 
 struct FwdSpace {
-  void *x, *w;
+  void *x, *w, *part;
+  Plan plan;
   size_t bytes;
 };
+
+// The forward's product without its operands' addresses, and the backward's two.
+Product fwd_shape(const gsb_linear& p) {
+  Product q{};
+  q.m = p.m, q.n = p.n, q.k = p.k, q.dtype = p.dtype, q.out_dtype = p.out_dtype;
+  return q;
+}
+Product dx_shape(const gsb_linear& p) {
+  Product q{};
+  q.b_mn = true;
+  q.m = p.m, q.n = p.k, q.k = p.n, q.dtype = p.dtype, q.out_dtype = p.dtype;
+  return q;
+}
+Product dw_shape(const gsb_linear& p) {
+  Product q{};
+  q.a_mn = q.b_mn = true;
+  q.m = p.n, q.n = p.k, q.k = p.m, q.dtype = p.dtype, q.out_dtype = p.dtype;
+  return q;
+}
 
 FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
   Carver c(ws, cap);
@@ -322,14 +347,19 @@ FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
   if (p.m > kFewRows) {
     if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
     if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
+    const Product q = fwd_shape(p);
+    s.plan = plan_product(q);
+    if (s.plan.splits > 1) s.part = c.take<char>(partial_bytes(q, s.plan));
   }
   s.bytes = c.used;
   return s;
 }
 
 struct BwdSpace {
-  void *dz, *x, *w;
+  void *dz, *x, *w, *sums;  // sums: the pieces of one of the two products after the other
   float* part;
+  Plan dx, dw, pair;
+  bool together;  // both products in one launch
   size_t bytes;
 };
 
@@ -344,6 +374,14 @@ BwdSpace bwd_space(const gsb_linear& p, const void* dy, int64_t dy_stride, void*
   if (!keeps_dy(p, dy, dy_stride)) s.dz = c.take<char>(copy_bytes(p.m, p.n, p.dtype));
   if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
   if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
+  const Product x = dx_shape(p), w = dw_shape(p);
+  s.dx = plan_product(x);
+  s.dw = plan_product(w);
+  s.pair = plan_pair(x, w);
+  s.together = s.pair.cost < s.dx.cost + s.dw.cost;
+  // also when one gradient alone is wanted: the plan that asked for less could not be known here
+  const size_t sums = std::max(partial_bytes(x, s.dx), partial_bytes(w, s.dw));
+  if (sums) s.sums = c.take<char>(sums);
   s.bytes = c.used;
   return s;
 }
@@ -387,15 +425,18 @@ gsb_status bwd(const gsb_linear& p, const void* z, const void* dy, int64_t dy_st
   CopyJob jx = job_of(p.x, p.x_stride, dw ? p.m : 0, p.k, p.dtype, s.x);
   CopyJob jw = job_of(p.weight, p.weight_stride, dx ? p.n : 0, p.k, p.dtype, s.w);
   Ready x, w;
-  if (jx.rows) ready_pair(jx, jw, p.dtype, x, w, st);
-  else ready_pair(jw, jx, p.dtype, w, x, st);
+  ready_pair(jx, jw, p.dtype, x, w, st);
   gsb_status status = launch_status();
-  if (dx && status == GSB_OK)
-    status = mma_product({g.p, g.ld, false, w.p, w.ld, true, p.m, p.k, p.n, p.dtype, p.dtype, g.plane, w.plane},
-                         plain_output(dx, p.k, p.dtype), st);
-  if (dw && status == GSB_OK)
-    status = mma_product({g.p, g.ld, true, x.p, x.ld, true, p.n, p.k, p.m, p.dtype, p.dtype, g.plane, x.plane},
-                         plain_output(dw, p.k, p.dtype), st);
+  Product p2[2] = {dx_shape(p), dw_shape(p)};
+  p2[0].a = p2[1].a = g.p;
+  p2[0].a_ld = p2[1].a_ld = g.ld;
+  p2[0].a_plane = p2[1].a_plane = g.plane;
+  p2[0].b = w.p, p2[0].b_ld = w.ld, p2[0].b_plane = w.plane;
+  p2[1].b = x.p, p2[1].b_ld = x.ld, p2[1].b_plane = x.plane;
+  const Epilogue e2[2] = {plain_output(dx, p.k, p.dtype), plain_output(dw, p.k, p.dtype)};
+  if (dx && dw && s.together) return status == GSB_OK ? mma_pair(p2, e2, s.pair, st) : status;
+  if (dx && status == GSB_OK) status = mma_product(p2[0], e2[0], s.dx, s.sums, st);
+  if (dw && status == GSB_OK) status = mma_product(p2[1], e2[1], s.dw, s.sums, st);
   return status;
 }
 
@@ -460,8 +501,10 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   ready_pair(job_of(p->x, p->x_stride, p->m, p->k, p->dtype, s.x),
              job_of(p->weight, p->weight_stride, p->n, p->k, p->dtype, s.w), p->dtype, x, w, st);
   if (gsb_status q = launch_status(); q != GSB_OK) return q;
-  return mma_product({x.p, x.ld, false, w.p, w.ld, false, p->m, p->n, p->k, p->dtype, p->out_dtype, x.plane, w.plane},
-                     e, st);
+  Product q = fwd_shape(*p);
+  q.a = x.p, q.a_ld = x.ld, q.a_plane = x.plane;
+  q.b = w.p, q.b_ld = w.ld, q.b_plane = w.plane;
+  return mma_product(q, e, s.plan, s.part, st);
 }
 
 size_t linear_bwd_workspace(const gsb_linear* p, const void* dy, int64_t dy_stride) {

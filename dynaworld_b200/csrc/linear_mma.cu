@@ -45,13 +45,136 @@ gsb_status gave_up_status(int* gave_up) {
   return GSB_OK;
 }
 
-gsb_status mma_product(const Product& p, const Epilogue& e, cudaStream_t st) {
-  switch (p.dtype) {
-    case GSB_F32: return mma_product_f32(p, e, st);
-    case GSB_BF16: return mma_product_bf16(p, e, st);
-    case GSB_F16: return mma_product_f16(p, e, st);
-    default: return mma_product_e4m3(p, e, st);
+// ---- plans ------------------------------------------------------------------------------------
+//
+// Costs in units of one 64-element block of K of a 256 x 256 tile (about 0.27 us).  A 256 x 128
+// tile's block costs 0.6 of that (B is half, A is not), a float block (six products, 256 x 128) 3.
+// A launch ends with one exposed epilogue (about 2 us, half of it for 128 columns); pieces along K
+// cost a second kernel (about 4 us) and their sums' way through L2.
+constexpr float kBlock128 = 0.6f, kBlockF32 = 3.0f, kTail256 = 8.0f, kTail128 = 4.0f, kReduce = 14.0f;
+constexpr float kPartialPerMB = 1.0f;  // written and read once
+
+struct Walk {
+  int bn;
+  float block, tail;
+};
+
+static int walks_of(int dtype, Walk (&w)[2]) {
+  if (dtype == GSB_F32) {
+    w[0] = {128, kBlockF32, kTail128};
+    return 1;
   }
+  w[0] = {256, 1.0f, kTail256};
+  w[1] = {128, kBlock128, kTail128};
+  return 2;
+}
+
+static int64_t tiles_of(const Product& p, int bn) { return ((p.m + 255) / 256) * ((p.n + bn - 1) / bn); }
+
+Plan plan_product(const Product& p) {
+  const int64_t clusters = sm_count() / 2;
+  const int blocks = k_blocks_of(p);
+  Plan best{0, 1, 0.0f};
+  Walk walks[2];
+  const int n = walks_of(p.dtype, walks);
+  for (int i = 0; i < n; ++i) {
+    const int64_t tiles = tiles_of(p, walks[i].bn);
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (blocks < 4 * splits || tiles * splits > 2 * clusters)) break;
+      const int64_t rounds = (tiles * splits + clusters - 1) / clusters;
+      float cost = float(rounds) * float((blocks + splits - 1) / splits) * walks[i].block + walks[i].tail;
+      if (splits > 1) cost += kReduce + kPartialPerMB * float(splits) * float(p.m) * float(p.n) * 4e-6f;
+      if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, splits, cost};
+    }
+  }
+  return best;
+}
+
+Plan plan_pair(const Product& p, const Product& q) {
+  const int64_t clusters = sm_count() / 2;
+  Plan best{0, 1, 0.0f};
+  Walk walks[2];
+  const int n = walks_of(p.dtype, walks);
+  for (int i = 0; i < n; ++i) {
+    const float a = float(k_blocks_of(p)) * walks[i].block, b = float(k_blocks_of(q)) * walks[i].block;
+    const float all = (float(tiles_of(p, walks[i].bn)) * a + float(tiles_of(q, walks[i].bn)) * b) / float(clusters);
+    // an even share, at least the longer tile, and half of the shorter one lost at the end
+    const float cost = std::max(all + 0.5f * std::min(a, b), std::max(a, b)) + walks[i].tail;
+    if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, 1, cost};
+  }
+  return best;
+}
+
+size_t partial_bytes(const Product& p, const Plan& plan) {
+  return plan.splits > 1 ? size_t(plan.splits) * size_t(p.m) * size_t(p.n) * 4 : 0;
+}
+
+// ---- the sums of a product's pieces, finished --------------------------------------------------
+
+template <typename O, int V>
+static __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, int splits, int64_t m, int64_t n,
+                                                              Epilogue e) {
+  const int64_t per_row = n / V, total = m * per_row, plane = m * n;
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
+    const int64_t i = t / per_row, j = (t - i * per_row) * V;
+    const float* p = part + i * n + j;
+    float z[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) z[u] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      if constexpr (V > 1) {
+#pragma unroll
+        for (int u = 0; u < V; u += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(p + s * plane + u);
+          z[u] += q.x, z[u + 1] += q.y, z[u + 2] += q.z, z[u + 3] += q.w;
+        }
+      } else {
+        z[0] += p[s * plane];
+      }
+    }
+    finish<O, V>(e, n, i, j, z);
+  }
+}
+
+template <typename O>
+static void add_parts(const float* part, int splits, const Product& p, const Epilogue& e, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(O);
+  const int64_t steps = e.vec ? p.m * p.n / V : p.m * p.n;
+  const int blocks = int(std::min<int64_t>((steps + 255) / 256, int64_t(sm_count()) * 8));
+  if (e.vec) add_parts_kernel<O, V><<<blocks, 256, 0, st>>>(part, splits, p.m, p.n, e);
+  else add_parts_kernel<O, 1><<<blocks, 256, 0, st>>>(part, splits, p.m, p.n, e);
+  note_launch();
+}
+
+static gsb_status launch_of(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st) {
+  switch (p->dtype) {
+    case GSB_F32: return mma_launch_f32(p, e, count, bn, splits, st);
+    case GSB_BF16: return mma_launch_bf16(p, e, count, bn, splits, st);
+    case GSB_F16: return mma_launch_f16(p, e, count, bn, splits, st);
+    default: return mma_launch_e4m3(p, e, count, bn, splits, st);
+  }
+}
+
+gsb_status mma_product(const Product& p, const Epilogue& e, const Plan& plan, void* part, cudaStream_t st) {
+  if (plan.splits == 1) return launch_of(&p, &e, 1, plan.bn, 1, st);
+  Product sums = p;
+  sums.out_dtype = GSB_F32;
+  Epilogue plain{};
+  plain.out = part;
+  plain.out_stride = p.n;
+  plain.vec = p.n % 4 == 0;
+  if (gsb_status s = launch_of(&sums, &plain, 1, plan.bn, plan.splits, st); s != GSB_OK) return s;
+  const int blocks = k_blocks_of(p), per = (blocks + plan.splits - 1) / plan.splits;
+  const int pieces = (blocks + per - 1) / per;
+  const float* f = static_cast<const float*>(part);
+  if (p.out_dtype == GSB_F32) add_parts<float>(f, pieces, p, e, st);
+  else if (p.out_dtype == GSB_BF16) add_parts<bf16>(f, pieces, p, e, st);
+  else add_parts<f16>(f, pieces, p, e, st);
+  return launch_status();
+}
+
+gsb_status mma_pair(const Product (&p)[2], const Epilogue (&e)[2], const Plan& plan, cudaStream_t st) {
+  return launch_of(p, e, 2, plan.bn, 1, st);
 }
 
 }  // namespace gsb

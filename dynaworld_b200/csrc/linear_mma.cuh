@@ -39,15 +39,57 @@ constexpr int kABytes = 128 * kRowBytes;
 constexpr int kChunk = 4;                   // PLANES = 3: blocks of 64 k per accumulation chain
 
 
-struct Args {
+// One product of a launch: m_tiles x n_tiles tiles, each walked in `splits` pieces of `per_split` blocks of
+// K (more than one: every piece writes its float sums to a plane of its own, part_stride apart).
+struct Job {
   int64_t m, n;
-  int k_blocks;
+  int64_t part_stride;
+  int64_t units;    // tiles x splits
+  int k_blocks, per_split, splits;
   int m_tiles, n_tiles;
-  int64_t tiles;
   int group;        // m tiles walked together, for reuse in L2
+  int a_mn;         // A is MN-major (backward launches)
   uint32_t idesc;
-  int* gave_up;
   Epilogue e;
+};
+
+// A launch's products over C clusters.  The units of job 0 (the longer ones) go round; clusters that
+// got one less take `extra` rounds of job 1 before all share the rest of it.
+template <int JOBS>
+struct Args {
+  Job job[JOBS];
+  CUtensorMap a[JOBS], b[JOBS];
+  int extra;
+  int* gave_up;
+
+  // The cluster's i-th unit; false past its last one.
+  __device__ __forceinline__ bool unit(int c, int clusters, int64_t i, int& which, int64_t& u) const {
+    which = 0;
+    if constexpr (JOBS == 1) {
+      u = c + i * clusters;
+      return u < job[0].units;
+    } else {
+      const int64_t all = job[0].units / clusters;
+      const int hi = int(job[0].units - all * clusters);
+      const int64_t mine = all + (c < hi);
+      if (i < mine) {
+        u = c + i * clusters;
+        return true;
+      }
+      which = 1;
+      i -= mine;
+      const int early = clusters - hi;
+      if (c >= hi) {
+        if (i < extra) {
+          u = i * early + (c - hi);
+          return u < job[1].units;
+        }
+        i -= extra;
+      }
+      u = int64_t(extra) * early + i * clusters + (c >= hi ? c - hi : c + early);
+      return u < job[1].units;
+    }
+  }
 };
 
 // ---- PTX ----
@@ -169,18 +211,16 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 // Shared-memory matrix descriptor, 128-byte swizzle (layout type 2 in bits 61-63, version 1 in bits
 // 46-47).  K-major: 8-row groups 1024 bytes apart (the stride offset).  MN-major: blocks of 64
 // columns 8192 bytes apart (the leading offset), groups of 8 k 1024 bytes apart.
-template <bool MN>
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  constexpr uint64_t lead = MN ? 8192 / 16 : 1, stride = 1024 / 16;
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn) {
+  const uint64_t lead = mn ? 8192 / 16 : 1, stride = 1024 / 16;
   return uint64_t((addr >> 4) & 0x3fff) | (lead << 16) | (stride << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // Descriptor advance per MMA (16 k of 16-bit, 32 of 8-bit values): 32 bytes along a K-major row,
 // two 8-k groups MN-major; in units of 16 bytes.
-template <bool MN>
-constexpr uint32_t kDescStep = MN ? 2048 / 16 : 32 / 16;
+__device__ __forceinline__ uint32_t desc_step(bool mn) { return mn ? 2048 / 16 : 32 / 16; }
 
-__device__ __forceinline__ void tile_of(const Args& p, int64_t t, int64_t& mt, int64_t& nt) {
+__device__ __forceinline__ void tile_of(const Job& p, int64_t t, int64_t& mt, int64_t& nt) {
   const int64_t per = int64_t(p.group) * p.n_tiles;
   const int64_t band = t / per, r = t - band * per;
   const int64_t first = band * p.group;
@@ -207,9 +247,11 @@ struct Rows {
   int row0, col;  // this lane's first row and column within the block
   int steps;      // its rows inside the matrix
   int64_t i;      // its first row
+  int64_t plane;  // offset of this piece's output
   float rs[kSteps];
 
-  __device__ __forceinline__ void start(const Args& p, int64_t i0) {
+  __device__ __forceinline__ void start(const Job& p, int64_t i0, int64_t plane_) {
+    plane = plane_;
     const int lane = threadIdx.x & 31;
     row0 = lane / kPerRow;
     col = (lane % kPerRow) * V;
@@ -221,7 +263,7 @@ struct Rows {
     }
   }
 
-  __device__ __forceinline__ void prefetch(const Args& p, int64_t j0, Ahead& a) const {
+  __device__ __forceinline__ void prefetch(const Job& p, int64_t j0, Ahead& a) const {
     const int64_t j = j0 + col;
     const bool in = p.e.vec && j < p.n;
     if (p.e.bias && in) a.bias = __ldg(reinterpret_cast<const uint4*>(static_cast<const O*>(p.e.bias) + j));
@@ -234,7 +276,7 @@ struct Rows {
     }
   }
 
-  __device__ __forceinline__ void emit(const Args& p, float* stage, int64_t i0, int64_t j0, const float (&v)[32],
+  __device__ __forceinline__ void emit(const Job& p, float* stage, int64_t i0, int64_t j0, const float (&v)[32],
                                        const Ahead& a) const {
     const int lane = threadIdx.x & 31;
     float4* mine = reinterpret_cast<float4*>(stage + lane * kPitch);
@@ -254,7 +296,7 @@ struct Rows {
 #pragma unroll
           for (int u = 0; u < V; ++u) cs[u] = p.e.col_scale[j + u];
         }
-        O* out = static_cast<O*>(p.e.out) + i * p.e.out_stride + j;
+        O* out = static_cast<O*>(p.e.out) + plane + i * p.e.out_stride + j;
         Z* keep = static_cast<Z*>(p.e.preact) + i * p.n + j;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -319,7 +361,7 @@ struct Rows {
           for (int r = 0; r < 8; ++r) z[r] = act_value<ACT>(z[r]);
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (r < rows) static_cast<O*>(p.e.out)[(i0 + r0 + r) * p.e.out_stride + j] = from_f32<O>(z[r] + add[r]);
+            if (r < rows) static_cast<O*>(p.e.out)[plane + (i0 + r0 + r) * p.e.out_stride + j] = from_f32<O>(z[r] + add[r]);
         }
       }
     }
@@ -342,11 +384,9 @@ struct Shape {
   static_assert(PLANES == 1 || kSlots >= 4, "a block's three slots and one ahead");
 };
 
-// KIND 0: 16-bit operands, 1: e4m3.
-template <int KIND, int CG, int BN, bool A_MN, bool B_MN, int PLANES, typename O, int ACT>
-__global__ void __launch_bounds__(kThreads, 1)
-    mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ Args p) {
+// KIND 0: 16-bit operands, 1: e4m3.  BWD: up to two products, B MN-major; else one, both K-major.
+template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT>
+__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<1 + BWD> p) {
   using S = Shape<CG, BN, PLANES>;
   constexpr int kElems = KIND == 1 ? 128 : 64;  // k per block
   extern __shared__ uint8_t raw[];
@@ -380,19 +420,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
 
-  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+  int which;
+  int64_t u;
 
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
       int s = 0;
       uint32_t phase = 0;
-      for (int64_t t = first; ok && t < p.tiles; t += step) {
+      for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
+        const Job& job = p.job[which];
+        const CUtensorMap* map_a = &p.a[which];
+        const CUtensorMap* map_b = &p.b[which];
+        const bool a_mn = BWD && job.a_mn;
         int64_t mt, nt;
-        tile_of(p, t, mt, nt);
+        tile_of(job, u / job.splits, mt, nt);
         const int i0 = int((mt * CG + rank) * 128);
         const int j0 = int(nt * BN + rank * S::kBRows);
-        for (int kb = 0; ok && kb < p.k_blocks; ++kb) {
+        const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
+        for (int kb = kb0; ok && kb < kb1; ++kb) {
           const int k0 = kb * kElems;
 #pragma unroll
           for (int q = 0; q < PLANES; ++q) {
@@ -401,17 +448,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
             if (rank == 0) bar_expect(full(s), CG * S::kSlot);
             const uint32_t a = base + s * S::kSlot, b = a + kABytes;
-            if constexpr (A_MN) {
+            if (a_mn) {
 #pragma unroll
-              for (int u = 0; u < 2; ++u) tma_load<CG>(a + u * 8192, &map_a, i0 + 64 * u, k0, plane, bar);
+              for (int v = 0; v < 2; ++v) tma_load<CG>(a + v * 8192, map_a, i0 + 64 * v, k0, plane, bar);
             } else {
-              tma_load<CG>(a, &map_a, k0, i0, plane, bar);
+              tma_load<CG>(a, map_a, k0, i0, plane, bar);
             }
-            if constexpr (B_MN) {
+            if constexpr (BWD) {
 #pragma unroll
-              for (int u = 0; u < S::kBRows / 64; ++u) tma_load<CG>(b + u * 8192, &map_b, j0 + 64 * u, k0, plane, bar);
+              for (int v = 0; v < S::kBRows / 64; ++v) tma_load<CG>(b + v * 8192, map_b, j0 + 64 * v, k0, plane, bar);
             } else {
-              tma_load<CG>(b, &map_b, k0, j0, plane, bar);
+              tma_load<CG>(b, map_b, k0, j0, plane, bar);
             }
             if (++s == S::kSlots) s = 0, phase ^= 1;
           }
@@ -430,22 +477,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0, buf = 0;
       uint32_t phase = 0, acc_phase = 0;
       const auto next = [&](int x) { return x + 1 == S::kSlots ? 0 : x + 1; };
-      for (int64_t t = first; ok && t < p.tiles; t += step) {
-        for (int kb = 0; ok && kb < p.k_blocks;) {
+      for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
+        const Job& job = p.job[which];
+        const bool a_mn = BWD && job.a_mn;
+        const uint32_t idesc = job.idesc, a_step = desc_step(a_mn), b_step = desc_step(BWD);
+        const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
+        for (int kb = kb0; ok && kb < kb1;) {
           if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
           fence_after();
           const uint32_t acc = tmem + buf * S::kAccCols;
-          const int stop = PLANES == 1 ? p.k_blocks : min(p.k_blocks, kb + kChunk);
+          const int stop = PLANES == 1 ? kb1 : min(kb1, kb + kChunk);
           uint32_t more = 0, more_low = 0;
           for (; kb < stop; ++kb) {
             if constexpr (PLANES == 1) {
               if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
               fence_after();
-              const uint64_t a = smem_desc<A_MN>(base + s * S::kSlot);
-              const uint64_t b = smem_desc<B_MN>(base + s * S::kSlot + kABytes);
+              const uint64_t a = smem_desc(base + s * S::kSlot, a_mn);
+              const uint64_t b = smem_desc(base + s * S::kSlot + kABytes, BWD);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                mma_issue<KIND, CG>(acc, a + u * kDescStep<A_MN>, b + u * kDescStep<B_MN>, p.idesc, more);
+              for (int v = 0; v < 4; ++v) {
+                mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
                 more = 1;
               }
               mma_commit<CG>(empty(s));
@@ -453,12 +504,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               const int s3 = s, s1 = next(s3), s2 = next(s1);
               const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
-              const auto da = [&](int q) { return smem_desc<A_MN>(base + q * S::kSlot); };
-              const auto db = [&](int q) { return smem_desc<B_MN>(base + q * S::kSlot + kABytes); };
+              const auto da = [&](int q) { return smem_desc(base + q * S::kSlot, a_mn); };
+              const auto db = [&](int q) { return smem_desc(base + q * S::kSlot + kABytes, BWD); };
               const auto run = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t& on) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  mma_issue<KIND, CG>(d, a + u * kDescStep<A_MN>, b + u * kDescStep<B_MN>, p.idesc, on);
+                for (int v = 0; v < 4; ++v) {
+                  mma_issue<KIND, CG>(d, a + v * a_step, b + v * b_step, idesc, on);
                   on = 1;
                 }
               };
@@ -495,9 +546,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_phase = 0;
     Rows<O, ACT> rows;
     typename Rows<O, ACT>::Ahead ahead;
-    for (int64_t t = first; t < p.tiles; t += step) {
+    for (int64_t i = 0; p.unit(cluster, clusters, i, which, u); ++i) {
+      const Job& job = p.job[which];
       int64_t mt, nt;
-      tile_of(p, t, mt, nt);
+      tile_of(job, u / job.splits, mt, nt);
+      const int64_t plane = (u % job.splits) * job.part_stride;
       const int64_t i0 = (mt * CG + rank) * 128 + quad * 32;
       const int64_t j0 = nt * BN + half * kHalfCols;
       const auto release = [&](int b) {
@@ -506,15 +559,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) bar_arrive_cluster(map_to_rank(acc_empty(b), 0));
       };
       if constexpr (PLANES == 1) {
-        rows.start(p, i0);
-        rows.prefetch(p, j0, ahead);
+        rows.start(job, i0, plane);
+        rows.prefetch(job, j0, ahead);
         ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
         fence_after();
         const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
 #pragma unroll 1
         for (int c = 0; c < kHalfCols; c += 32) {
           const typename Rows<O, ACT>::Ahead now = ahead;
-          if (c + 32 < kHalfCols) rows.prefetch(p, j0 + c + 32, ahead);
+          if (c + 32 < kHalfCols) rows.prefetch(job, j0 + c + 32, ahead);
           float v[32];
           tmem_load32(acc + c, v);
           if (c + 32 == kHalfCols) release(buf);
@@ -522,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int u = 0; u < 32; ++u) v[u] = __int_as_float(0x7fc00000);
           }
-          if (i0 < p.m && j0 + c < p.n) rows.emit(p, stage, i0, j0 + c, v, now);
+          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, v, now);
         }
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
@@ -530,7 +583,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sum[kHalfCols];
 #pragma unroll
         for (int u = 0; u < kHalfCols; ++u) sum[u] = 0.0f;
-        for (int kb = 0; kb < p.k_blocks; kb += kChunk) {
+        const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
+        for (int kb = kb0; kb < kb1; kb += kChunk) {
           ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
           fence_after();
           const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
@@ -546,14 +600,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           buf ^= 1;
           if (buf == 0) acc_phase ^= 1;
         }
-        rows.start(p, i0);
+        rows.start(job, i0, plane);
 #pragma unroll
         for (int c = 0; c < kHalfCols; c += 32) {
-          rows.prefetch(p, j0 + c, ahead);
+          rows.prefetch(job, j0 + c, ahead);
           float v[32];
 #pragma unroll
           for (int u = 0; u < 32; ++u) v[u] = ok ? sum[c + u] : __int_as_float(0x7fc00000);
-          if (i0 < p.m && j0 + c < p.n) rows.emit(p, stage, i0, j0 + c, v, ahead);
+          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, v, ahead);
         }
       }
     }
@@ -600,10 +654,33 @@ inline uint32_t instr_desc(int dtype, bool a_mn, bool b_mn, int m, int n) {
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
-template <int KIND, int CG, int BN, bool A_MN, bool B_MN, int PLANES, typename O, int ACT>
-gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
+template <int KIND, int CG, int BN, int PLANES>
+bool make_job(Job& j, CUtensorMap* a, CUtensorMap* b, const Product& p, const Epilogue& e, int splits) {
   using S = Shape<CG, BN, PLANES>;
-  auto* kernel = mma_kernel<KIND, CG, BN, A_MN, B_MN, PLANES, O, ACT>;
+  if (!make_map(a, p.a, p.dtype, p.a_mn, p.m, p.k, p.a_ld, 128, PLANES, p.a_plane) ||
+      !make_map(b, p.b, p.dtype, p.b_mn, p.n, p.k, p.b_ld, S::kBRows, PLANES, p.b_plane))
+    return false;
+  j.m = p.m;
+  j.n = p.n;
+  j.k_blocks = k_blocks_of(p);
+  j.per_split = (j.k_blocks + splits - 1) / splits;
+  j.splits = (j.k_blocks + j.per_split - 1) / j.per_split;
+  j.part_stride = j.splits > 1 ? p.m * p.n : 0;
+  j.m_tiles = int((p.m + 128 * CG - 1) / (128 * CG));
+  j.n_tiles = int((p.n + BN - 1) / BN);
+  j.units = int64_t(j.m_tiles) * j.n_tiles * j.splits;
+  j.group = 8;
+  j.a_mn = p.a_mn;
+  j.idesc = instr_desc(p.dtype, p.a_mn, p.b_mn, 128 * CG, BN);
+  j.e = e;
+  return true;
+}
+
+// products[0 .. count): one forward product, or one or two of the backward's.
+template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT>
+gsb_status launch(const Product* products, const Epilogue* e, int count, int splits, cudaStream_t st) {
+  using S = Shape<CG, BN, PLANES>;
+  auto* kernel = mma_kernel<KIND, CG, BN, BWD, PLANES, O, ACT>;
   int dev = 0;
   (void)cudaGetDevice(&dev);
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel has its shared memory
@@ -615,24 +692,26 @@ gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
     }
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  constexpr int kElems = KIND == 1 ? 128 : 64;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, p.a, p.dtype, A_MN, p.m, p.k, p.a_ld, 128, PLANES, p.a_plane) ||
-      !make_map(&mb, p.b, p.dtype, B_MN, p.n, p.k, p.b_ld, S::kBRows, PLANES, p.b_plane))
-    return GSB_ERR_CUDA;
-  Args a{};
-  a.m = p.m;
-  a.n = p.n;
-  a.k_blocks = int((p.k + kElems - 1) / kElems);
-  a.m_tiles = int((p.m + 128 * CG - 1) / (128 * CG));
-  a.n_tiles = int((p.n + BN - 1) / BN);
-  a.tiles = int64_t(a.m_tiles) * a.n_tiles;
-  a.group = 8;
-  a.idesc = instr_desc(p.dtype, A_MN, B_MN, 128 * CG, BN);
+  Args<1 + BWD> a{};
+  int64_t units = 0;
+  const bool swap = count == 2 && k_blocks_of(products[1]) > k_blocks_of(products[0]);  // the longer first
+  for (int i = 0; i < count; ++i) {
+    const int from = swap ? 1 - i : i;
+    if (!make_job<KIND, CG, BN, PLANES>(a.job[i], &a.a[i], &a.b[i], products[from], e[from], splits))
+      return GSB_ERR_CUDA;
+    units += a.job[i].units;
+  }
   a.gave_up = gave_up_flag();
   if (!a.gave_up) return GSB_ERR_CUDA;
-  a.e = e;
-  const int clusters = int(std::min<int64_t>(a.tiles, sm_count() / CG));
+  const int clusters = int(std::min<int64_t>(units, sm_count() / CG));
+  if constexpr (BWD) {
+    const int early = clusters - int(a.job[0].units % clusters);
+    if (count == 2 && early < clusters) {
+      const int64_t d0 = a.job[0].per_split, d1 = a.job[1].per_split;
+      a.extra = int(std::min<int64_t>((d0 + d1 / 2) / d1, (a.job[1].units + early - 1) / early));
+    }
+    if (count == 1) a.job[1].splits = 1;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(clusters * CG));
   cfg.blockDim = dim3(kThreads);
@@ -645,7 +724,7 @@ gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
   note_launch();
   if (err != cudaSuccess) {
     (void)cudaGetLastError();
@@ -655,22 +734,14 @@ gsb_status launch(const Product& p, const Epilogue& e, cudaStream_t st) {
 }
 
 template <int KIND, int CG, int BN, int PLANES, typename O>
-gsb_status launch_act(const Product& p, const Epilogue& e, cudaStream_t st) {
+gsb_status launch_fwd(const Product& p, const Epilogue& e, int splits, cudaStream_t st) {
   switch (e.act) {
-    case GSB_ACT_RELU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_RELU>(p, e, st);
-    case GSB_ACT_GELU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_GELU>(p, e, st);
-    case GSB_ACT_GELU_TANH: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_GELU_TANH>(p, e, st);
-    case GSB_ACT_SILU: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_SILU>(p, e, st);
-    default: return launch<KIND, CG, BN, false, false, PLANES, O, GSB_ACT_NONE>(p, e, st);
+    case GSB_ACT_RELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_RELU>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_GELU>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU_TANH: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_GELU_TANH>(&p, &e, 1, splits, st);
+    case GSB_ACT_SILU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_SILU>(&p, &e, 1, splits, st);
+    default: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_NONE>(&p, &e, 1, splits, st);
   }
-}
-
-// The forward's product, or one of the backward's two (which have no epilogue).
-template <int CG, int BN, int PLANES, typename O>
-gsb_status launch_any(const Product& p, const Epilogue& e, cudaStream_t st) {
-  if (!p.b_mn) return launch_act<0, CG, BN, PLANES, O>(p, e, st);
-  if (!p.a_mn) return launch<0, CG, BN, false, true, PLANES, O, GSB_ACT_NONE>(p, e, st);
-  return launch<0, CG, BN, true, true, PLANES, O, GSB_ACT_NONE>(p, e, st);
 }
 
 }  // namespace mma

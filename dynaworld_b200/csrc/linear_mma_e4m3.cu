@@ -3,12 +3,17 @@
 
 namespace gsb {
 
-gsb_status mma_product_e4m3(const Product& p, const Epilogue& e, cudaStream_t st) {
+template <int BN>
+static gsb_status of_width(const Product& p, const Epilogue& e, int splits, cudaStream_t st) {
   switch (p.out_dtype) {
-    case GSB_F32: return mma::launch_act<1, 2, 256, 1, float>(p, e, st);
-    case GSB_BF16: return mma::launch_act<1, 2, 256, 1, bf16>(p, e, st);
-    default: return mma::launch_act<1, 2, 256, 1, f16>(p, e, st);
+    case GSB_F32: return mma::launch_fwd<1, 2, BN, 1, float>(p, e, splits, st);
+    case GSB_BF16: return mma::launch_fwd<1, 2, BN, 1, bf16>(p, e, splits, st);
+    default: return mma::launch_fwd<1, 2, BN, 1, f16>(p, e, splits, st);
   }
+}
+
+gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int, int bn, int splits, cudaStream_t st) {
+  return bn == 256 ? of_width<256>(*p, *e, splits, st) : of_width<128>(*p, *e, splits, st);
 }
 
 }  // namespace gsb

@@ -108,12 +108,33 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t n, int64_t i, 
   store_f32<O, V>(static_cast<O*>(e.out) + i * e.out_stride + j, z);
 }
 
-// Tensor-core product (linear_mma.cu).  The operands' rows (and parts) start on 16-byte boundaries.
-gsb_status mma_product(const Product& p, const Epilogue& e, cudaStream_t st);
-gsb_status mma_product_bf16(const Product& p, const Epilogue& e, cudaStream_t st);
-gsb_status mma_product_f16(const Product& p, const Epilogue& e, cudaStream_t st);
-gsb_status mma_product_f32(const Product& p, const Epilogue& e, cudaStream_t st);
-gsb_status mma_product_e4m3(const Product& p, const Epilogue& e, cudaStream_t st);
+inline int k_blocks_of(const Product& p) {
+  const int64_t per = p.dtype == GSB_E4M3 ? 128 : 64;
+  return int((p.k + per - 1) / per);
+}
+
+// How the tensor-core kernel walks a product: tiles of 256 x bn, each in `splits` pieces along K whose
+// float sums a second kernel adds (in order) and finishes.
+struct Plan {
+  int bn;
+  int splits;
+  float cost;  // estimated, in blocks of K of a 256 x 256 tile
+};
+Plan plan_product(const Product& p);
+// The backward's two products in one launch (no splits).
+Plan plan_pair(const Product& p, const Product& q);
+size_t partial_bytes(const Product& p, const Plan& plan);
+
+// The products (linear_mma.cu).  The operands' rows (and parts) start on 16-byte boundaries; `part` is
+// partial_bytes long.
+gsb_status mma_product(const Product& p, const Epilogue& e, const Plan& plan, void* part, cudaStream_t st);
+gsb_status mma_pair(const Product (&p)[2], const Epilogue (&e)[2], const Plan& plan, cudaStream_t st);
+// By operand type: products[0 .. count) of one launch, count 2 only with b_mn.  out_dtype F32 beside
+// 16-bit operands writes sums (no epilogue).
+gsb_status mma_launch_bf16(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
+gsb_status mma_launch_f16(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
+gsb_status mma_launch_f32(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
+gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
 // 1 once a bounded wait of a token-side kernel gave up on the current device.
 gsb_status gave_up_status(int* gave_up);
 

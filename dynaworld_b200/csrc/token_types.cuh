@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace gsb {
 
 using bf16 = __nv_bfloat16;
@@ -67,10 +69,22 @@ inline bool vec_ok(const void* p, int64_t stride, int elem, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (stride * elem) % bytes == 0;
 }
 
+// SMs of the current device (a B200's without one).
 inline int sm_count() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  int n = known[dev & 63].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return 148;
+    }
+    known[dev & 63].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
