@@ -27,60 +27,122 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// Phi(-|z|) and exp(-z^2 / 2): 7.1.26 with its coefficients halved and its argument |z| / sqrt(2).
-__device__ __forceinline__ float normal_tail(float z, float& gauss) {
-  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
-  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-  p = fmaf(p, t, 0.5f * 1.421413741f);
-  p = fmaf(p, t, 0.5f * -0.284496736f);
-  p = fmaf(p, t, 0.5f * 0.254829592f);
-  gauss = fast_exp2(z * z * (-0.5f * kLog2E));
-  return p * t * gauss;
+// Two floats in one register pair: the FMA pipe takes both in one instruction (sm_100).
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() = default;
+  __device__ __forceinline__ explicit F2(float both) : F2(both, both) {}
+  __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+template <typename F>
+__device__ __forceinline__ F2 each(F2 a, F f) {
+  float lo, hi;
+  a.get(lo, hi);
+  return F2(f(lo), f(hi));
+}
+__device__ __forceinline__ F2 exp2_2(F2 a) { return each(a, [](float x) { return fast_exp2(x); }); }
+__device__ __forceinline__ F2 rcp_2(F2 a) { return each(a, [](float x) { return fast_rcp(x); }); }
+
+// -|z|, Phi(-|z|) and exp(-z^2 / 2): 7.1.26 with its coefficients halved, its argument |z| / sqrt(2).
+__device__ __forceinline__ F2 normal_tail(F2 z, F2& minus, F2& gauss) {
+  minus = each(z, [](float x) { return __int_as_float(__float_as_int(x) | 0x80000000); });
+  const F2 t = rcp_2(fma2(F2(-0.3275911f * 0.70710678118654752f), minus, F2(1.0f)));
+  F2 p = fma2(F2(0.5f * 1.061405429f), t, F2(0.5f * -1.453152027f));
+  p = fma2(p, t, F2(0.5f * 1.421413741f));
+  p = fma2(p, t, F2(0.5f * -0.284496736f));
+  p = fma2(p, t, F2(0.5f * 0.254829592f));
+  gauss = exp2_2(mul2(mul2(z, z), F2(-0.5f * kLog2E)));
+  return mul2(mul2(p, t), gauss);
 }
 
-__device__ __forceinline__ float sigmoid_of(float z) { return fast_rcp(1.0f + fast_exp2(-kLog2E * z)); }
+__device__ __forceinline__ F2 sigmoid_of(F2 z) { return rcp_2(add2(exp2_2(mul2(z, F2(-kLog2E))), F2(1.0f))); }
 
-// 2 sqrt(2 / pi) (z + 0.044715 z^3)
-__device__ __forceinline__ float gelu_tanh_arg(float z) {
-  return z * fmaf(2.0f * kSqrt2OverPi * kGeluCubic * z, z, 2.0f * kSqrt2OverPi);
+// 2 sqrt(2 / pi) (z + 0.044715 z^3), from z and z^2
+__device__ __forceinline__ F2 gelu_tanh_arg(F2 z, F2 zz) {
+  return mul2(z, fma2(F2(2.0f * kSqrt2OverPi * kGeluCubic), zz, F2(2.0f * kSqrt2OverPi)));
 }
 
 // ReLU passes a NaN on, as torch does.
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
+__device__ __forceinline__ F2 act_value(F2 z) {
   if constexpr (ACT == GSB_ACT_RELU) {
-    return z < 0.0f ? 0.0f : z;
+    return each(z, [](float x) { return x < 0.0f ? 0.0f : x; });
   } else if constexpr (ACT == GSB_ACT_GELU) {
-    float gauss;
-    const float tail = normal_tail(z, gauss);
-    return fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    F2 minus, gauss;
+    const F2 tail = normal_tail(z, minus, gauss);
+    return fma2(minus, tail, each(z, [](float x) { return fmaxf(x, 0.0f); }));  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
-    return z * sigmoid_of(gelu_tanh_arg(z));
+    return mul2(z, sigmoid_of(gelu_tanh_arg(z, mul2(z, z))));
   } else if constexpr (ACT == GSB_ACT_SILU) {
-    return z * sigmoid_of(z);
+    return mul2(z, sigmoid_of(z));
   } else {
     return z;
   }
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
+__device__ __forceinline__ F2 act_slope(F2 z) {
   if constexpr (ACT == GSB_ACT_RELU) {
-    return z <= 0.0f ? 0.0f : 1.0f;
+    return each(z, [](float x) { return x <= 0.0f ? 0.0f : 1.0f; });
   } else if constexpr (ACT == GSB_ACT_GELU) {
-    float gauss;
-    const float tail = normal_tail(z, gauss);
-    return fmaf(z * kInvSqrt2Pi, gauss, z < 0.0f ? tail : 1.0f - tail);
+    F2 minus, gauss;
+    const F2 tail = normal_tail(z, minus, gauss);
+    float z0, z1, t0, t1;
+    z.get(z0, z1);
+    tail.get(t0, t1);
+    const F2 cdf(z0 < 0.0f ? t0 : 1.0f - t0, z1 < 0.0f ? t1 : 1.0f - t1);
+    return fma2(mul2(z, F2(kInvSqrt2Pi)), gauss, cdf);
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
-    const float s = sigmoid_of(gelu_tanh_arg(z));
+    const F2 zz = mul2(z, z);
+    const F2 s = sigmoid_of(gelu_tanh_arg(z, zz));
     // s (1 - s) is 0 from |z| = 10 on, where z^2 must not overflow
-    const float du = fmaf(6.0f * kSqrt2OverPi * kGeluCubic, fminf(z * z, 1e4f), 2.0f * kSqrt2OverPi);
-    return fmaf(z * s * (1.0f - s), du, s);
+    const F2 du = fma2(F2(6.0f * kSqrt2OverPi * kGeluCubic), each(zz, [](float x) { return fminf(x, 1e4f); }),
+                       F2(2.0f * kSqrt2OverPi));
+    return fma2(mul2(z, mul2(s, fma2(s, F2(-1.0f), F2(1.0f)))), du, s);
   } else if constexpr (ACT == GSB_ACT_SILU) {
-    const float s = sigmoid_of(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    const F2 s = sigmoid_of(z);
+    return mul2(s, fma2(z, fma2(s, F2(-1.0f), F2(1.0f)), F2(1.0f)));
   } else {
-    return 1.0f;
+    return F2(1.0f);
+  }
+}
+
+// V values at once.
+template <int ACT, int V>
+__device__ __forceinline__ void apply_value(float (&z)[V]) {
+  if constexpr (ACT == GSB_ACT_NONE) return;
+#pragma unroll
+  for (int u = 0; u < V; u += 2) {
+    float unused;
+    if (u + 1 < V) act_value<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
+    else act_value<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
+  }
+}
+template <int ACT, int V>
+__device__ __forceinline__ void apply_slope(float (&z)[V]) {
+#pragma unroll
+  for (int u = 0; u < V; u += 2) {
+    float unused;
+    if (u + 1 < V) act_slope<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
+    else act_slope<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
   }
 }
 

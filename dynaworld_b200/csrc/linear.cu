@@ -1,6 +1,8 @@
 // y = act(x w^T + b) + r and its backward.
 #include "linear_parts.cuh"
 
+#include <type_traits>
+
 namespace gsb {
 
 namespace {
@@ -206,29 +208,40 @@ void ready_pair(CopyJob a, CopyJob b, int dtype, Ready& ra, Ready& rb, cudaStrea
 // dz = dy act'(z) rounded to the operands' type (float: its three bf16 parts), rows at `pitch`
 // (dz NULL: only the sums), and per block of rows the float column sums of the unrounded dz.
 // A block is 32 lanes x V columns by 8 rows; its rows' sums are added in a fixed order.
+// Each thread's next two rows are on their way while it works on one (left to the compiler, the loads
+// waited for the arithmetic: SiLU took 95 us at 16384 x 4096 bf16 where the bytes take 62, float
+// GELU 195 us where they take 144).
 template <typename T, int ACT, int V>
-__global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t dy_stride, const typename PreactOf<T>::type* z,
-                                                 void* dz, int64_t pitch, float* part, int64_t m, int n,
-                                                 int64_t rows_per_part) {
+__global__ void __launch_bounds__(256, 4)
+    dz_kernel(const T* dy, int64_t dy_stride, const typename PreactOf<T>::type* z, void* dz, int64_t pitch, float* part,
+              int64_t m, int n, int64_t rows_per_part) {
   using Z = typename PreactOf<T>::type;
   constexpr bool SPLIT = sizeof(T) == 4;
+  using D = typename std::conditional<SPLIT, bf16, T>::type;
   __shared__ float s_sum[8][32 * V + 1];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int j = (blockIdx.x * 32 + lane) * V;
-  const int64_t lo = blockIdx.y * rows_per_part, hi = min(m, lo + rows_per_part);
+  const int64_t lo = blockIdx.y * rows_per_part;
+  const int rows = int(min(m, lo + rows_per_part) - lo);
   float s[V];
 #pragma unroll
   for (int u = 0; u < V; ++u) s[u] = 0.0f;
   if (j < n) {
-#pragma unroll 4
-    for (int64_t i = lo + g; i < hi; i += 8) {
+    const T* from = dy + (lo + g) * dy_stride + j;
+    const Z* zs = z + (lo + g) * n + j;
+    D* to = static_cast<D*>(dz) + (lo + g) * pitch + j;
+    const int64_t dy_step = 8 * dy_stride, z_step = 8 * int64_t(n), dz_step = 8 * pitch, plane = m * pitch;
+    const auto work = [&](const Vec<T, V>& d, const Vec<Z, V>& at) {
       float v[V];
-      load_f32<T, V>(dy + i * dy_stride + j, v);
-      if constexpr (ACT != GSB_ACT_NONE) {
-        float q[V];
-        load_f32<Z, V>(z + i * n + j, q);
 #pragma unroll
-        for (int u = 0; u < V; ++u) v[u] = __fmul_rn(v[u], act_slope<ACT>(q[u]));
+      for (int u = 0; u < V; ++u) v[u] = to_f32(d.v[u]);
+      if constexpr (ACT != GSB_ACT_NONE) {
+        float slope[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u) slope[u] = to_f32(at.v[u]);
+        apply_slope<ACT, V>(slope);
+#pragma unroll
+        for (int u = 0; u < V; ++u) v[u] = __fmul_rn(v[u], slope[u]);
       }
 #pragma unroll
       for (int u = 0; u < V; ++u) s[u] = __fadd_rn(s[u], v[u]);  // not fused: the same sum with and without dz
@@ -237,17 +250,38 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t dy_stride,
           Vec<bf16, V> o[3];
 #pragma unroll
           for (int u = 0; u < V; ++u) {
-            const Parts q = split3(v[u]);
+            const Parts p = split3(v[u]);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) o[k].v[u] = q.p[k];
+            for (int k = 0; k < 3; ++k) o[k].v[u] = p.p[k];
           }
 #pragma unroll
-          for (int k = 0; k < 3; ++k)
-            *reinterpret_cast<Vec<bf16, V>*>(static_cast<bf16*>(dz) + (k * m + i) * pitch + j) = o[k];
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, V>*>(to + k * plane) = o[k];
         } else {
-          store_f32<T, V>(static_cast<T*>(dz) + i * pitch + j, v);
+          store_f32<T, V>(to, v);
         }
       }
+      to += dz_step;
+    };
+    Vec<T, V> d0, d1;
+    Vec<Z, V> z0, z1;
+    const auto fetch = [&](Vec<T, V>& d, Vec<Z, V>& at) {
+      d = read_once<T, V>(from);
+      if constexpr (ACT != GSB_ACT_NONE) at = read_once<Z, V>(zs);
+      from += dy_step;
+      zs += z_step;
+    };
+    if (g < rows) fetch(d0, z0);
+    if (g + 8 < rows) fetch(d1, z1);
+    for (int i = g; i < rows; i += 16) {
+      Vec<T, V> d = d0;
+      Vec<Z, V> at = z0;
+      if (i + 16 < rows) fetch(d0, z0);
+      work(d, at);
+      if (i + 8 >= rows) break;
+      d = d1;
+      at = z1;
+      if (i + 24 < rows) fetch(d1, z1);
+      work(d, at);
     }
   }
   if (!part) return;
@@ -290,7 +324,7 @@ template <typename T, int ACT>
 void launch_dz(const DzJob& d, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   // z and dz are this library's own, aligned whenever n is a multiple of V
-  if (d.n % V == 0 && vec_ok(d.dy, d.dy_stride, sizeof(T), 16) && vec_ok(d.z, 0, 1, 16)) launch_dz_v<T, ACT, V>(d, st);
+  if (d.n % V == 0 && vec_ok(d.dy, d.dy_stride, sizeof(T), V * sizeof(T)) && vec_ok(d.z, 0, 1, 16)) launch_dz_v<T, ACT, V>(d, st);
   else launch_dz_v<T, ACT, 1>(d, st);
 }
 

@@ -32,8 +32,7 @@ namespace mma {
 
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
-constexpr int kPitch = 36;                  // floats per row of an epilogue warp's 32 x 32 block
-constexpr int kStageBytes = kEpiWarps * 32 * kPitch * 4;
+constexpr int kStageBytes = kEpiWarps * 32 * 32 * 4;  // a 32 x 32 block of floats per epilogue warp
 constexpr int kRowBytes = 128;              // one swizzled row of a box
 constexpr int kABytes = 128 * kRowBytes;
 constexpr int kChunk = 4;                   // PLANES = 3: blocks of 64 k per accumulation chain
@@ -110,9 +109,11 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// bar: an address in the cluster's shared window
+// bar: an address in the cluster's shared window.  Relaxed: what the arrival hands over is TMEM that has
+// been read (tcgen05.wait::ld, tcgen05.fence); a release would also wait for the warp's stores of
+// outputs, about a microsecond per tile.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -137,8 +138,9 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of the warp's lanes, asynchronously: the registers hold them after tmem_wait32 on the same
+// array, whose operands keep the compiler from reading them earlier.
+__device__ __forceinline__ void tmem_start32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
@@ -148,9 +150,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
@@ -229,6 +236,10 @@ __device__ __forceinline__ void tile_of(const Job& p, int64_t t, int64_t& mt, in
   nt = r / rows;
 }
 
+// Where the q-th 16 bytes of row r of a warp's block are: a permutation by row, so that eight lanes
+// meet eight banks groups whether they hold eight rows (writing) or adjacent parts of one (reading).
+__device__ __forceinline__ int stage_at(int r, int q) { return r * 32 + ((q ^ (r & 7)) << 2); }
+
 // A warp's part of the epilogue.  A 32 x 32 block of sums (lane = row) goes through shared memory so
 // that global accesses are 16 bytes per lane: V values, 32 / V lanes per row, kSteps rows per lane.
 // The residual and bias of the next block are loaded while this one is finished: a block takes
@@ -276,13 +287,18 @@ struct Rows {
     }
   }
 
-  __device__ __forceinline__ void emit(const Job& p, float* stage, int64_t i0, int64_t j0, const float (&v)[32],
-                                       const Ahead& a) const {
+  // The block's sums into shared memory ...
+  __device__ __forceinline__ static void put(float* stage, const uint32_t (&v)[32]) {
     const int lane = threadIdx.x & 31;
-    float4* mine = reinterpret_cast<float4*>(stage + lane * kPitch);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) mine[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(stage + stage_at(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     __syncwarp();
+  }
+
+  // ... and from there to the output.
+  __device__ __forceinline__ void emit(const Job& p, const float* stage, int64_t i0, int64_t j0, const Ahead& a) const {
+    const int lane = threadIdx.x & 31;
     if (p.e.vec) {
       const int64_t j = j0 + col;
       if (j < p.n) {
@@ -298,38 +314,47 @@ struct Rows {
         }
         O* out = static_cast<O*>(p.e.out) + plane + i * p.e.out_stride + j;
         Z* keep = static_cast<Z*>(p.e.preact) + i * p.n + j;
+        // two rows' arithmetic at a time, no branch between them: a warp's latencies overlap
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          if (s >= steps) break;
-          float z[V];
-          const float* from = stage + (row0 + s * kAtOnce) * kPitch + col;
+        for (int s0 = 0; s0 < kSteps; s0 += 2) {
+          float z[2 * V];
 #pragma unroll
-          for (int u = 0; u < V; u += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(from + u);
-            z[u] = q.x, z[u + 1] = q.y, z[u + 2] = q.z, z[u + 3] = q.w;
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int v = 0; v < V; v += 4) {
+              const float4 q =
+                  *reinterpret_cast<const float4*>(stage + stage_at(row0 + (s0 + h) * kAtOnce, (col + v) >> 2));
+              float* to = z + h * V + v;
+              to[0] = q.x, to[1] = q.y, to[2] = q.z, to[3] = q.w;
+            }
           if (p.e.row_scale) {
 #pragma unroll
-            for (int u = 0; u < V; ++u) z[u] *= rs[s] * cs[u];
+            for (int v = 0; v < 2 * V; ++v) z[v] *= rs[s0 + v / V] * cs[v % V];
           }
           if (p.e.bias) {
 #pragma unroll
-            for (int u = 0; u < V; ++u) z[u] += bias[u];
+            for (int v = 0; v < 2 * V; ++v) z[v] += bias[v % V];
           }
           if (p.e.preact) {
-            Vec<Z, V> kept;
 #pragma unroll
-            for (int u = 0; u < V; ++u) kept.v[u] = as_preact(static_cast<Z*>(nullptr), z[u]);
-            *reinterpret_cast<Vec<Z, V>*>(keep + s * kAtOnce * p.n) = kept;
+            for (int h = 0; h < 2; ++h)
+              if (s0 + h < steps)
+                *reinterpret_cast<Vec<Z, V>*>(keep + (s0 + h) * kAtOnce * p.n) =
+                    kept_of<V>(static_cast<Z*>(nullptr), reinterpret_cast<const float(&)[V]>(z[h * V]));
           }
-          #pragma unroll
-          for (int u = 0; u < V; ++u) z[u] = act_value<ACT>(z[u]);
+          apply_value<ACT, 2 * V>(z);
           if (p.e.res) {
-            const Vec<O, V> r = *reinterpret_cast<const Vec<O, V>*>(&a.res[s]);
 #pragma unroll
-            for (int u = 0; u < V; ++u) z[u] += to_f32(r.v[u]);
+            for (int h = 0; h < 2; ++h) {
+              const Vec<O, V> r = *reinterpret_cast<const Vec<O, V>*>(&a.res[s0 + h]);
+#pragma unroll
+              for (int v = 0; v < V; ++v) z[h * V + v] += to_f32(r.v[v]);
+            }
           }
-          store_f32<O, V>(out + s * kAtOnce * p.e.out_stride, z);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (s0 + h < steps)
+              store_f32<O, V>(out + (s0 + h) * kAtOnce * p.e.out_stride, reinterpret_cast<const float(&)[V]>(z[h * V]));
         }
       }
     } else {
@@ -343,7 +368,7 @@ struct Rows {
           float z[8], add[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            z[r] = stage[(r0 + r) * kPitch + lane];
+            z[r] = stage[stage_at(r0 + r, lane >> 2) + (lane & 3)];
             add[r] = 0.0f;
             if (r < rows) {
               if (p.e.row_scale) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
@@ -357,8 +382,7 @@ struct Rows {
               if (r < rows)
                 static_cast<Z*>(p.e.preact)[(i0 + r0 + r) * p.n + j] = as_preact(static_cast<Z*>(nullptr), z[r]);
           }
-          #pragma unroll
-          for (int r = 0; r < 8; ++r) z[r] = act_value<ACT>(z[r]);
+                    apply_value<ACT, 8>(z);
 #pragma unroll
           for (int r = 0; r < 8; ++r)
             if (r < rows) static_cast<O*>(p.e.out)[plane + (i0 + r0 + r) * p.e.out_stride + j] = from_f32<O>(z[r] + add[r]);
@@ -538,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     }
   } else if (warp >= 4) {
     const int w = warp - 4, quad = warp & 3, half = w >> 2;  // quad: the 32 TMEM lanes this warp may read
-    float* stage = stage_all + w * 32 * kPitch;
+    float* stage = stage_all + w * 32 * 32;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
     constexpr int kHalfCols = BN / 2;
     bool ok = true;
@@ -564,18 +588,21 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
         fence_after();
         const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
+        uint32_t v[32];
+        tmem_start32(acc, v);
 #pragma unroll 1
         for (int c = 0; c < kHalfCols; c += 32) {
           const typename Rows<O, ACT>::Ahead now = ahead;
           if (c + 32 < kHalfCols) rows.prefetch(job, j0 + c + 32, ahead);
-          float v[32];
-          tmem_load32(acc + c, v);
-          if (c + 32 == kHalfCols) release(buf);
+          tmem_wait32(v);
           if (!ok) {
 #pragma unroll
-            for (int u = 0; u < 32; ++u) v[u] = __int_as_float(0x7fc00000);
+            for (int q = 0; q < 32; ++q) v[q] = 0x7fc00000;
           }
-          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, v, now);
+          rows.put(stage, v);
+          if (c + 32 < kHalfCols) tmem_start32(acc + c + 32, v);
+          else release(buf);
+          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, now);
         }
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
@@ -604,10 +631,11 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
 #pragma unroll
         for (int c = 0; c < kHalfCols; c += 32) {
           rows.prefetch(job, j0 + c, ahead);
-          float v[32];
+          uint32_t v[32];
 #pragma unroll
-          for (int u = 0; u < 32; ++u) v[u] = ok ? sum[c + u] : __int_as_float(0x7fc00000);
-          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, v, ahead);
+          for (int q = 0; q < 32; ++q) v[q] = ok ? __float_as_uint(sum[c + q]) : 0x7fc00000;
+          rows.put(stage, v);
+          if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, ahead);
         }
       }
     }

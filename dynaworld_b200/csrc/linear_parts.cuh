@@ -57,24 +57,35 @@ struct PreactOf<float> { using type = float; };
 template <int V>
 __device__ __forceinline__ void apply_act(int act, float (&z)[V]) {
   switch (act) {
-    case GSB_ACT_RELU:
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_RELU>(z[i]);
-      break;
-    case GSB_ACT_GELU:
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_GELU>(z[i]);
-      break;
-    case GSB_ACT_GELU_TANH:
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_GELU_TANH>(z[i]);
-      break;
-    case GSB_ACT_SILU:
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = act_value<GSB_ACT_SILU>(z[i]);
-      break;
+    case GSB_ACT_RELU: apply_value<GSB_ACT_RELU, V>(z); break;
+    case GSB_ACT_GELU: apply_value<GSB_ACT_GELU, V>(z); break;
+    case GSB_ACT_GELU_TANH: apply_value<GSB_ACT_GELU_TANH, V>(z); break;
+    case GSB_ACT_SILU: apply_value<GSB_ACT_SILU, V>(z); break;
     default: break;
   }
+}
+
+// z as it is kept.
+template <int V>
+__device__ __forceinline__ Vec<float, V> kept_of(float*, const float (&z)[V]) {
+  Vec<float, V> k;
+#pragma unroll
+  for (int u = 0; u < V; ++u) k.v[u] = z[u];
+  return k;
+}
+template <int V>
+__device__ __forceinline__ Vec<f16, V> kept_of(f16*, const float (&z)[V]) {
+  Vec<f16, V> k;
+  if constexpr (V == 1) {
+    k.v[0] = as_preact(static_cast<f16*>(nullptr), z[0]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < V; u += 2)
+      asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;"
+          : "=r"(*reinterpret_cast<uint32_t*>(&k.v[u]))
+          : "f"(z[u + 1]), "f"(z[u]));
+  }
+  return k;
 }
 
 // V adjacent sums of row i from column j on.
@@ -93,10 +104,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t n, int64_t i, 
     for (int u = 0; u < V; ++u) z[u] += b[u];
   }
   if (e.preact) {
-    Vec<Z, V> keep;
-#pragma unroll
-    for (int u = 0; u < V; ++u) keep.v[u] = as_preact(static_cast<Z*>(nullptr), z[u]);
-    *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) = keep;
+    *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) = kept_of<V>(static_cast<Z*>(nullptr), z);
   }
   apply_act<V>(e.act, z);
   if (e.res) {

@@ -31,6 +31,14 @@ __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat1
 template <>
 __device__ __forceinline__ f16 from_f32<f16>(float v) { return __float2half_rn(v); }
 
+// Two at once.
+__device__ __forceinline__ void pack2(bf16* p, float lo, float hi) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(lo, hi);
+}
+__device__ __forceinline__ void pack2(f16* p, float lo, float hi) {
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(lo, hi);
+}
+
 // V elements moved by one access of V * sizeof(T) bytes.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -44,11 +52,27 @@ __device__ __forceinline__ void load_f32(const T* p, float (&out)[V]) {
   for (int i = 0; i < V; ++i) out[i] = to_f32(t.v[i]);
 }
 
+// Data that is read once: it is the first to leave L2.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> read_once(const T* p) {
+  if constexpr (sizeof(Vec<T, V>) == 16) {
+    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const Vec<T, V>*>(&q);
+  } else {
+    return *reinterpret_cast<const Vec<T, V>*>(p);
+  }
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void store_f32(T* p, const float (&in)[V]) {
   Vec<T, V> t;
+  if constexpr (V % 2 == 0 && sizeof(T) == 2) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) t.v[i] = from_f32<T>(in[i]);
+    for (int i = 0; i < V; i += 2) pack2(&t.v[i], in[i], in[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.v[i] = from_f32<T>(in[i]);
+  }
   *reinterpret_cast<Vec<T, V>*>(p) = t;
 }
 
