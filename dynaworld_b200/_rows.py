@@ -5,7 +5,7 @@ import contextlib
 
 import torch
 
-from . import _lib
+from . import _lib, render
 
 TYPE_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 E4M3 = torch.float8_e4m3fn
@@ -17,6 +17,25 @@ def on_device(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _NOTHING
     return torch.cuda.device(device)
+
+
+def call(stage: str, name: str, device: torch.device, *args) -> None:
+    """C entry point ``name`` with ``args`` and the device's current stream, on that device; its status
+    raises.  Without tracing and on the current device nothing is set up around it: the operators of a
+    single token take as long on the host as on the GPU."""
+    fn = getattr(_lib.lib(), name)
+    index = device.index
+    if render.STAGE_EVENTS is None and not render.NVTX and index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with on_device(device), render._stage(stage):
+            status = fn(*args, render._stream(device))
+    if status:
+        _lib.check(name, status)
+
+
+def address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:

@@ -10,15 +10,12 @@ these are the B200 kernels for them.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import E4M3, TYPE_CODES, check_device, check_input, check_like, on_device, rows_of, workspace
+from ._rows import E4M3, TYPE_CODES, address, call, check_device, check_input, check_like, rows_of, workspace
 from .norm import _refuse_grad
-from .render import _stage, _stream
 
 
 def _activation(name: str) -> int:
@@ -28,21 +25,18 @@ def _activation(name: str) -> int:
     return code
 
 
-def _spec(x, weight, bias, residual, act, code, out_code, x_scale=None, weight_scale=None):
-    return _lib.Linear(x.shape[0], weight.shape[0], weight.shape[1], code, out_code, act, 0, x.data_ptr(), x.stride(0),
-                       weight.data_ptr(), weight.stride(0), _lib.ptr(bias), _lib.ptr(residual),
-                       0 if residual is None else residual.stride(0), _lib.ptr(x_scale), _lib.ptr(weight_scale))
+def _spec(x, weight, bias, residual, act, code, out_code, x_scale=None, weight_scale=None) -> bytes:
+    """gsb_linear"""
+    n, k = weight.shape
+    return _lib.pack_linear(x.shape[0], n, k, code, out_code, act, 0, x.data_ptr(), x.stride(0), weight.data_ptr(),
+                            weight.stride(0), address(bias), address(residual),
+                            0 if residual is None else residual.stride(0), address(x_scale), address(weight_scale))
 
 
-def _run_forward(spec, y: torch.Tensor, preact: torch.Tensor | None) -> None:
-    L = _lib.lib()
-    dev = y.device
-    p = ctypes.byref(spec)
-    with on_device(dev), _stage("linear"):
-        nbytes = L.gsb_linear_fwd_workspace(p)
-        ws = workspace(y, nbytes)
-        _lib.check("gsb_linear_fwd", L.gsb_linear_fwd(p, y.data_ptr(), _lib.ptr(preact), _lib.ptr(ws), nbytes,
-                                                      _stream(dev)))
+def _run_forward(spec: bytes, y: torch.Tensor, preact: torch.Tensor | None) -> None:
+    nbytes = _lib.lib().gsb_linear_fwd_workspace(spec)
+    ws = workspace(y, nbytes)
+    call("linear", "gsb_linear_fwd", y.device, spec, y.data_ptr(), address(preact), address(ws), nbytes)
 
 
 class _Linear(torch.autograd.Function):
@@ -64,20 +58,17 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         if not (need_x or need_w or need_b):
             return None, None, None, dy if need_r else None, None, None
-        L = _lib.lib()
-        dev = x.device
         n, k = weight.shape
         g = rows_of(dy, n)
         dx = x.new_empty((x.shape[0], k)) if need_x else None
         dw = x.new_empty((n, k)) if need_w else None
         db = x.new_empty(n) if need_b else None
-        p = ctypes.byref(_spec(x, weight, None, None, ctx.act, ctx.code, ctx.code))
+        spec = _spec(x, weight, None, None, ctx.act, ctx.code, ctx.code)
         gp, gs = g.data_ptr(), g.stride(0)
-        with on_device(dev), _stage("linear_bwd"):
-            nbytes = L.gsb_linear_bwd_workspace(p, gp, gs)
-            ws = workspace(x, nbytes)
-            _lib.check("gsb_linear_bwd", L.gsb_linear_bwd(p, _lib.ptr(preact), gp, gs, _lib.ptr(dx), _lib.ptr(dw),
-                                                          _lib.ptr(db), _lib.ptr(ws), nbytes, _stream(dev)))
+        nbytes = _lib.lib().gsb_linear_bwd_workspace(spec, gp, gs)
+        ws = workspace(x, nbytes)
+        call("linear_bwd", "gsb_linear_bwd", x.device, spec, address(preact), gp, gs, address(dx), address(dw),
+             address(db), address(ws), nbytes)
         return dx, dw, db, dy if need_r else None, None, None
 
 

@@ -8,32 +8,26 @@ are torch modules in the reference; these are the B200 kernels for them, next to
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import E4M3, check_device, check_input, check_like, on_device, rows_of, workspace
-from .render import _stage, _stream
+from ._rows import E4M3, address, call, check_device, check_input, check_like, rows_of, workspace
 
 
-def _norm(x: torch.Tensor, code: int, eps: float, residual: torch.Tensor | None, weight: torch.Tensor | None):
-    return _lib.Norm(x.shape[0], x.shape[1], code, eps, 0, x.data_ptr(), x.stride(0), _lib.ptr(residual),
-                     0 if residual is None else residual.stride(0), _lib.ptr(weight))
+def _norm(x, code: int, eps: float, residual, weight) -> bytes:
+    """gsb_norm"""
+    return _lib.pack_norm(x.shape[0], x.shape[1], code, eps, 0, x.data_ptr(), x.stride(0), address(residual),
+                          0 if residual is None else residual.stride(0), address(weight))
 
 
 def _forward(x, weight, residual, eps, code, need_rstd):
     """x [rows, dim] -> y, summed (None without a residual), rstd (None unless needed)."""
-    L = _lib.lib()
-    dev = x.device
     y = x.new_empty(x.shape)
     summed = None if residual is None else x.new_empty(x.shape)
     rstd = x.new_empty(x.shape[0], dtype=torch.float32) if need_rstd else None
-    with on_device(dev), _stage("rms_norm"):
-        _lib.check("gsb_rms_norm_fwd", L.gsb_rms_norm_fwd(
-            ctypes.byref(_norm(x, code, eps, residual, weight)), y.data_ptr(), _lib.ptr(summed), _lib.ptr(rstd),
-            _stream(dev)))
+    call("rms_norm", "gsb_rms_norm_fwd", x.device, _norm(x, code, eps, residual, weight), y.data_ptr(), address(summed),
+         address(rstd))
     return y, summed, rstd
 
 
@@ -54,22 +48,17 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:  # only the stream was used
             return (dsummed if need_x else None, None if not need_w else torch.zeros_like(weight),
                     dsummed if need_r else None, None, None)
-        L = _lib.lib()
-        dev = x.device
         dim = x.shape[1]
         dy = rows_of(dy, dim)
         dsummed = None if dsummed is None else rows_of(dsummed, dim)
         dx = x.new_empty(x.shape)
-        dw = weight.new_empty(dim) if need_w else None
+        dw = x.new_empty(dim) if need_w else None
         norm = _norm(x, ctx.code, ctx.eps, residual, weight)
-        p = ctypes.byref(norm)
-        with on_device(dev), _stage("rms_norm_bwd"):
-            nbytes = L.gsb_rms_norm_bwd_workspace(p)
-            ws = workspace(x, nbytes)
-            _lib.check("gsb_rms_norm_bwd", L.gsb_rms_norm_bwd(
-                p, rstd.data_ptr(), dy.data_ptr(), dy.stride(0), _lib.ptr(dsummed),
-                0 if dsummed is None else dsummed.stride(0), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(ws), nbytes,
-                _stream(dev)))
+        nbytes = _lib.lib().gsb_rms_norm_bwd_workspace(norm)
+        ws = workspace(x, nbytes)
+        call("rms_norm_bwd", "gsb_rms_norm_bwd", x.device, norm, rstd.data_ptr(), dy.data_ptr(), dy.stride(0),
+             address(dsummed), 0 if dsummed is None else dsummed.stride(0), dx.data_ptr(), address(dw), address(ws),
+             nbytes)
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
 
@@ -119,18 +108,15 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tenso
     infinity stands for NaN.  Not differentiable."""
     code = _check("rms_norm_fp8", x, weight, residual, eps)
     _refuse_grad("rms_norm_fp8", x, weight, residual)
-    L = _lib.lib()
-    dev, dim = x.device, x.shape[-1]
+    dim = x.shape[-1]
     x2 = rows_of(x, dim)
     r2 = None if residual is None else rows_of(residual, dim)
     w = weight.contiguous()
     q = x.new_empty(x.shape, dtype=E4M3)
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     h = None if residual is None else x.new_empty(x.shape)
-    with on_device(dev), _stage("rms_norm_fp8"):
-        _lib.check("gsb_rms_norm_fp8", L.gsb_rms_norm_fp8(
-            ctypes.byref(_norm(x2, code, float(eps), r2, w)), q.data_ptr(), scale.data_ptr(), _lib.ptr(h),
-            _stream(dev)))
+    call("rms_norm_fp8", "gsb_rms_norm_fp8", x.device, _norm(x2, code, float(eps), r2, w), q.data_ptr(), scale.data_ptr(),
+         address(h))
     return (q, scale) if residual is None else (q, scale, h)
 
 
@@ -140,12 +126,10 @@ def quantize_rows_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     8-bit products every step.  Not differentiable."""
     code = _check("quantize_rows_fp8", x, None, None, 0.0)
     _refuse_grad("quantize_rows_fp8", x)
-    L = _lib.lib()
-    dev, dim = x.device, x.shape[-1]
+    dim = x.shape[-1]
     x2 = rows_of(x, dim)
     q = x.new_empty(x.shape, dtype=E4M3)
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    with on_device(dev), _stage("quantize_rows_fp8"):
-        _lib.check("gsb_quantize_rows_fp8", L.gsb_quantize_rows_fp8(
-            ctypes.byref(_norm(x2, code, 0.0, None, None)), q.data_ptr(), scale.data_ptr(), _stream(dev)))
+    call("quantize_rows_fp8", "gsb_quantize_rows_fp8", x.device, _norm(x2, code, 0.0, None, None), q.data_ptr(),
+         scale.data_ptr())
     return q, scale
