@@ -1,0 +1,65 @@
+"""TokenHeads: reading a GaussianParameterHeads-like module and its refusals (no GPU)."""
+import pytest
+import torch
+from torch import nn
+
+from dynaworld_b200.heads import FeedForward, Layer, TokenHeads, head_outputs
+from dynaworld_b200.renderer import HeadActivation
+
+
+class Heads(nn.Module):
+    """The attributes of the reference's module (blocks.py:84-186)."""
+
+    def __init__(self, dim=8, hidden=16, per_token=4, act=nn.GELU, **override):
+        super().__init__()
+        self.xy_extent, self.z_min, self.z_extent, self.scale_init = 1.0, 1.0, 2.0, 0.08
+        for name, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1), ("rgb", 3)):
+            setattr(self, f"{name}_head",
+                    override.get(name) or nn.Sequential(nn.Linear(dim, hidden), act(), nn.Linear(hidden, per_token * c)))
+
+
+@pytest.mark.parametrize("act,name", [(nn.GELU, "gelu"), (lambda: nn.GELU("tanh"), "gelu_tanh"), (nn.SiLU, "silu"),
+                                      (nn.ReLU, "relu")])
+def test_reads_the_module(act, name):
+    m = Heads(act=act)
+    h = TokenHeads.from_heads(m)
+    assert h.activation == name and h.gaussians_per_token == 4 and not h.is_fp8
+    assert h.head == HeadActivation(1.0, 1.0, 3.0, 0.08)
+    assert h.rot[1].weight is m.rot_head[2].weight and h.rot[1].bias is m.rot_head[2].bias
+
+
+@pytest.mark.parametrize("match, make", [
+    ("no activation between", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 8), nn.Linear(8, 12)))),
+    ("starts with an activation", lambda: Heads(rgb=nn.Sequential(nn.GELU(), nn.Linear(8, 12)))),
+    ("two activations", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 8), nn.GELU(), nn.GELU(), nn.Linear(8, 12)))),
+    ("must end in a linear", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 12), nn.GELU()))),
+    ("holds a LayerNorm", lambda: Heads(rgb=nn.Sequential(nn.LayerNorm(8), nn.Linear(8, 12)))),
+    ("active dropout", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 8), nn.GELU(), nn.Dropout(0.1), nn.Linear(8, 12)))),
+    ("different activations", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 8), nn.SiLU(), nn.Linear(8, 12)))),
+    ("not a multiple of 3", lambda: Heads(rgb=nn.Linear(8, 13))),
+    ("different numbers of Gaussians", lambda: Heads(rgb=nn.Linear(8, 15))),
+])
+def test_refused_modules(match, make):
+    with pytest.raises(ValueError, match=match):
+        TokenHeads.from_heads(make())
+
+
+def test_refused_arguments():
+    layers = {n: (Layer(torch.zeros(c, 8)),) for n, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1),
+                                                         ("rgb", 3))}
+    with pytest.raises(ValueError, match="Unknown activation"):
+        TokenHeads(**layers, activation="swish")
+    with pytest.raises(ValueError, match="no layers"):
+        TokenHeads(**{**layers, "rot": ()})
+    mixed = {**layers, "rgb": (Layer(torch.zeros(3, 8), None, torch.zeros(3)),)}
+    with pytest.raises(ValueError, match="every layer is 8-bit or none"):
+        TokenHeads(**mixed)
+    coded = {n: (Layer(v[0].weight, None, torch.zeros(v[0].weight.shape[0])),) for n, v in layers.items()}
+    with pytest.raises(ValueError, match="need the norm"):
+        TokenHeads(**coded)
+    heads = TokenHeads(**layers, blocks=(FeedForward(torch.ones(8), Layer(torch.zeros(8, 8)),
+                                                     Layer(torch.zeros(8, 8))),))
+    with pytest.raises(ValueError, match=r"tokens must be \[S, T, D\]"):
+        head_outputs(torch.zeros(8), heads)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        head_outputs(torch.zeros(2, 8), heads)
