@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libgsb200.so"
@@ -122,11 +121,6 @@ class Linear(C.Structure):
     ]
 
 
-# The same structures as bytes, for the calls a decode loop makes per token: packing them takes a third
-# of the time of building a ctypes.Structure.
-pack_norm = struct.Struct("qiifiPqPqP").pack
-pack_linear = struct.Struct("qiiiiiiPqPqPPqPP").pack
-
 P = C.POINTER
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -161,16 +155,16 @@ SIGNATURES = {
     "gsb_splats2d_preprocess": (C.c_int, [P(Splats2D), C.c_int32, C.c_int32, P(Options), vp, vp, vp, vp, vp,
                                           C.c_size_t, vp]),
     "gsb_splats2d_preprocess_bwd": (C.c_int, [P(Splats2D), vp, vp, P(Splats2DGrads), vp]),
-    "gsb_rms_norm_fwd": (C.c_int, [vp, vp, vp, vp, vp]),
-    "gsb_rms_norm_bwd_workspace": (C.c_size_t, [vp]),
-    "gsb_rms_norm_bwd": (C.c_int, [vp, vp, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, C.c_size_t, vp]),
-    "gsb_rms_norm_fp8": (C.c_int, [vp, vp, vp, vp, vp]),
-    "gsb_quantize_rows_fp8": (C.c_int, [vp, vp, vp, vp]),
-    "gsb_linear_fwd_workspace": (C.c_size_t, [vp]),
-    "gsb_linear_fwd": (C.c_int, [vp, vp, vp, vp, C.c_size_t, vp]),
-    "gsb_linear_bwd_workspace": (C.c_size_t, [vp, vp, C.c_int64]),
+    "gsb_rms_norm_fwd": (C.c_int, [P(Norm), vp, vp, vp, vp]),
+    "gsb_rms_norm_bwd_workspace": (C.c_size_t, [P(Norm)]),
+    "gsb_rms_norm_bwd": (C.c_int, [P(Norm), vp, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, C.c_size_t, vp]),
+    "gsb_rms_norm_fp8": (C.c_int, [P(Norm), vp, vp, vp, vp]),
+    "gsb_quantize_rows_fp8": (C.c_int, [P(Norm), vp, vp, vp]),
+    "gsb_linear_fwd_workspace": (C.c_size_t, [P(Linear)]),
+    "gsb_linear_fwd": (C.c_int, [P(Linear), vp, vp, vp, C.c_size_t, vp]),
+    "gsb_linear_bwd_workspace": (C.c_size_t, [P(Linear), vp, C.c_int64]),
     "gsb_token_status": (C.c_int, []),
-    "gsb_linear_bwd": (C.c_int, [vp, vp, vp, C.c_int64, vp, vp, vp, vp, C.c_size_t, vp]),
+    "gsb_linear_bwd": (C.c_int, [P(Linear), vp, vp, C.c_int64, vp, vp, vp, vp, C.c_size_t, vp]),
     "gsb_radix_sort_workspace": (C.c_size_t, [C.c_uint32, C.c_int, C.c_int]),
     "gsb_radix_sort": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),
     "gsb_debug_sort_lookback_timeout": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, vp, C.c_size_t, vp]),

@@ -164,4 +164,22 @@ def test_no_norm_and_no_blocks():
     for (n, c), a in zip(HEAD_CHANNELS.items(), got):
         l0, l1 = getattr(heads, n)
         ref = F.gelu(h @ l0.weight.double().T + l0.bias.double()) @ l1.weight.double().T + l1.bias.double()
-        assert float((a.double() - ref.reshape(2, -1, c)).norm() / ref.norm()) < 2e-6
+        assert float(((a.double() - ref.reshape(2, -1, c)).norm() / ref.norm()).detach()) < 2e-6
+
+
+def test_stages_are_traced():
+    """Stage events name the operators like the render's stages; without tracing nothing is recorded."""
+    from dynaworld_b200 import render
+
+    heads, (t, r) = make(torch.float32), inputs(torch.float32)
+    assert render.STAGE_EVENTS is None
+    render.STAGE_EVENTS = []
+    try:
+        sum(v.sum() for v in head_outputs(t, heads, residual=r)).backward()
+        torch.cuda.synchronize()
+        names = [e[0] for e in render.STAGE_EVENTS]
+        assert all(e[1].elapsed_time(e[2]) >= 0 for e in render.STAGE_EVENTS)
+    finally:
+        render.STAGE_EVENTS = None
+    assert names.count("rms_norm") == names.count("rms_norm_bwd") == 2
+    assert names.count("linear") == names.count("linear_bwd") == 12

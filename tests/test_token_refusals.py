@@ -60,11 +60,6 @@ def lib():
 
 
 def test_struct_sizes_match_header():
-    fields = lambda c: [getattr(c, f) or 0 for f, _ in c._fields_]  # noqa: E731
-    n = _lib.Norm(3, 8, 1, 0.5, 0, 4096, 16, 8192, 24, 12288)
-    assert _lib.pack_norm(*fields(n)) == bytes(n)
-    p = _lib.Linear(3, 8, 9, 1, 2, 4, 0, 4096, 16, 8192, 24, 12288, 16384, 32, 20480, 24576)
-    assert _lib.pack_linear(*fields(p)) == bytes(p)
     assert ctypes.sizeof(_lib.Norm) == 8 + 4 * 4 + 5 * 8
     assert ctypes.sizeof(_lib.Linear) == 8 + 6 * 4 + 9 * 8
 
