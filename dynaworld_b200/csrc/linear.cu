@@ -383,14 +383,14 @@ FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
     if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
     const Product q = fwd_shape(p);
     s.plan = plan_product(q);
-    if (s.plan.splits > 1) s.part = c.take<char>(partial_bytes(q, s.plan));
+    if (const size_t sums = partial_bytes(&q, 1, s.plan)) s.part = c.take<char>(sums);
   }
   s.bytes = c.used;
   return s;
 }
 
 struct BwdSpace {
-  void *dz, *x, *w, *sums;  // sums: the pieces of one of the two products after the other
+  void *dz, *x, *w, *sums;  // sums: of products in pieces
   float* part;
   Plan dx, dw, pair;
   bool together;  // both products in one launch
@@ -408,13 +408,14 @@ BwdSpace bwd_space(const gsb_linear& p, const void* dy, int64_t dy_stride, void*
   if (!keeps_dy(p, dy, dy_stride)) s.dz = c.take<char>(copy_bytes(p.m, p.n, p.dtype));
   if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
   if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
-  const Product x = dx_shape(p), w = dw_shape(p);
-  s.dx = plan_product(x);
-  s.dw = plan_product(w);
-  s.pair = plan_pair(x, w);
+  const Product two[2] = {dx_shape(p), dw_shape(p)};
+  s.dx = plan_product(two[0]);
+  s.dw = plan_product(two[1]);
+  s.pair = plan_pair(two);
   s.together = s.pair.cost < s.dx.cost + s.dw.cost;
-  // also when one gradient alone is wanted: the plan that asked for less could not be known here
-  const size_t sums = std::max(partial_bytes(x, s.dx), partial_bytes(w, s.dw));
+  // for either gradient alone too: which are wanted is not known here
+  const size_t sums = std::max({partial_bytes(two, 1, s.dx), partial_bytes(two + 1, 1, s.dw),
+                                s.together ? partial_bytes(two, 2, s.pair) : 0});
   if (sums) s.sums = c.take<char>(sums);
   s.bytes = c.used;
   return s;
@@ -468,9 +469,9 @@ gsb_status bwd(const gsb_linear& p, const void* z, const void* dy, int64_t dy_st
   p2[0].b = w.p, p2[0].b_ld = w.ld, p2[0].b_plane = w.plane;
   p2[1].b = x.p, p2[1].b_ld = x.ld, p2[1].b_plane = x.plane;
   const Epilogue e2[2] = {plain_output(dx, p.k, p.dtype), plain_output(dw, p.k, p.dtype)};
-  if (dx && dw && s.together) return status == GSB_OK ? mma_pair(p2, e2, s.pair, st) : status;
-  if (dx && status == GSB_OK) status = mma_product(p2[0], e2[0], s.dx, s.sums, st);
-  if (dw && status == GSB_OK) status = mma_product(p2[1], e2[1], s.dw, s.sums, st);
+  if (dx && dw && s.together) return status == GSB_OK ? mma_products(p2, e2, 2, s.pair, s.sums, st) : status;
+  if (dx && status == GSB_OK) status = mma_products(p2, e2, 1, s.dx, s.sums, st);
+  if (dw && status == GSB_OK) status = mma_products(p2 + 1, e2 + 1, 1, s.dw, s.sums, st);
   return status;
 }
 
@@ -538,7 +539,7 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   Product q = fwd_shape(*p);
   q.a = x.p, q.a_ld = x.ld, q.a_plane = x.plane;
   q.b = w.p, q.b_ld = w.ld, q.b_plane = w.plane;
-  return mma_product(q, e, s.plan, s.part, st);
+  return mma_products(&q, &e, 1, s.plan, s.part, st);
 }
 
 size_t linear_bwd_workspace(const gsb_linear* p, const void* dy, int64_t dy_stride) {

@@ -48,10 +48,11 @@ gsb_status gave_up_status(int* gave_up) {
 // ---- plans ------------------------------------------------------------------------------------
 //
 // Costs in units of one 64-element block of K of a 256 x 256 tile (about 0.27 us).  A 256 x 128
-// tile's block costs 0.6 of that (B is half, A is not), a float block (six products, 256 x 128) 3.
+// tile's block costs 0.9 of that (8192 x 4096 x 4096 bf16: 351 us in 128-wide tiles, 195 in 256-wide
+// ones), a float block (six products) 6.
 // A launch ends with one exposed epilogue (about 2 us, half of it for 128 columns); pieces along K
 // cost a second kernel (about 4 us) and their sums' way through L2.
-constexpr float kBlock128 = 0.6f, kBlockF32 = 3.0f, kTail256 = 8.0f, kTail128 = 4.0f, kReduce = 14.0f;
+constexpr float kBlock128 = 0.9f, kBlockF32 = 6.0f, kTail256 = 8.0f, kTail128 = 4.0f, kReduce = 14.0f;
 constexpr float kPartialPerMB = 1.0f;  // written and read once
 
 struct Walk {
@@ -61,7 +62,7 @@ struct Walk {
 
 static int walks_of(int dtype, Walk (&w)[2]) {
   if (dtype == GSB_F32) {
-    w[0] = {128, kBlockF32, kTail128};
+    w[0] = {256, kBlockF32, kTail256};
     return 1;
   }
   w[0] = {256, 1.0f, kTail256};
@@ -71,42 +72,66 @@ static int walks_of(int dtype, Walk (&w)[2]) {
 
 static int64_t tiles_of(const Product& p, int bn) { return ((p.m + 255) / 256) * ((p.n + bn - 1) / bn); }
 
+// The second kernel and its sums' traffic.
+static float reduce_cost(const Product& p, int splits) {
+  return kReduce + kPartialPerMB * float(splits) * float(p.m) * float(p.n) * 4e-6f;
+}
+
+static bool may_split(const Product& p, int splits, int64_t tiles, int64_t clusters) {
+  return splits == 1 || (k_blocks_of(p) >= 4 * splits && tiles * splits <= 2 * clusters);
+}
+
 Plan plan_product(const Product& p) {
   const int64_t clusters = sm_count() / 2;
-  const int blocks = k_blocks_of(p);
-  Plan best{0, 1, 0.0f};
+  Plan best{0, {1, 1}, 0.0f};
   Walk walks[2];
   const int n = walks_of(p.dtype, walks);
   for (int i = 0; i < n; ++i) {
     const int64_t tiles = tiles_of(p, walks[i].bn);
-    for (int splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (blocks < 4 * splits || tiles * splits > 2 * clusters)) break;
-      const int64_t rounds = (tiles * splits + clusters - 1) / clusters;
-      float cost = float(rounds) * float((blocks + splits - 1) / splits) * walks[i].block + walks[i].tail;
-      if (splits > 1) cost += kReduce + kPartialPerMB * float(splits) * float(p.m) * float(p.n) * 4e-6f;
-      if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, splits, cost};
+    for (int s = 1; s <= 16 && may_split(p, s, tiles, clusters); s *= 2) {
+      const int64_t rounds = (tiles * s + clusters - 1) / clusters;
+      float cost = float(rounds) * float(piece_of(p, s)) * walks[i].block + walks[i].tail;
+      if (s > 1) cost += reduce_cost(p, s);
+      if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, {s, 1}, cost};
     }
   }
   return best;
 }
 
-Plan plan_pair(const Product& p, const Product& q) {
+// Whether a product of the launch leaves float sums: its own pieces, or, where the output is not float,
+// the other's (one kernel writes both).
+static bool leaves_sums(const Product* p, int count, const Plan& plan, int i) {
+  if (plan.splits[i] > 1) return true;
+  return count == 2 && plan.splits[1 - i] > 1 && p[i].out_dtype != GSB_F32;
+}
+
+Plan plan_pair(const Product (&p)[2]) {
   const int64_t clusters = sm_count() / 2;
-  Plan best{0, 1, 0.0f};
+  Plan best{0, {1, 1}, 0.0f};
   Walk walks[2];
-  const int n = walks_of(p.dtype, walks);
+  const int n = walks_of(p[0].dtype, walks);
   for (int i = 0; i < n; ++i) {
-    const float a = float(k_blocks_of(p)) * walks[i].block, b = float(k_blocks_of(q)) * walks[i].block;
-    const float all = (float(tiles_of(p, walks[i].bn)) * a + float(tiles_of(q, walks[i].bn)) * b) / float(clusters);
-    // an even share, at least the longer tile, and half of the shorter one lost at the end
-    const float cost = std::max(all + 0.5f * std::min(a, b), std::max(a, b)) + walks[i].tail;
-    if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, 1, cost};
+    const int64_t t0 = tiles_of(p[0], walks[i].bn), t1 = tiles_of(p[1], walks[i].bn);
+    for (int s0 = 1; s0 <= 16 && may_split(p[0], s0, t0, clusters); s0 *= 2)
+      for (int s1 = 1; s1 <= 16 && may_split(p[1], s1, t1, clusters); s1 *= 2) {
+        const Plan plan{walks[i].bn, {s0, s1}, 0.0f};
+        const float a = float(piece_of(p[0], s0)) * walks[i].block, b = float(piece_of(p[1], s1)) * walks[i].block;
+        const float all = (float(t0 * s0) * a + float(t1 * s1) * b) / float(clusters);
+        // an even share, at least the longer piece, and half of the shorter one lost at the end
+        float cost = std::max(all + 0.5f * std::min(a, b), std::max(a, b)) + walks[i].tail;
+        for (int k = 0; k < 2; ++k)
+          if (leaves_sums(p, 2, plan, k)) cost += reduce_cost(p[k], plan.splits[k]);
+        if (best.bn == 0 || cost < best.cost) best = {plan.bn, {s0, s1}, cost};
+      }
   }
   return best;
 }
 
-size_t partial_bytes(const Product& p, const Plan& plan) {
-  return plan.splits > 1 ? size_t(plan.splits) * size_t(p.m) * size_t(p.n) * 4 : 0;
+size_t partial_bytes(const Product* p, int count, const Plan& plan) {
+  size_t n = 0;
+  for (int i = 0; i < count; ++i)
+    if (leaves_sums(p, count, plan, i)) n += align_up(size_t(plan.splits[i]) * size_t(p[i].m) * size_t(p[i].n) * 4);
+  return n;
 }
 
 // ---- the sums of a product's pieces, finished --------------------------------------------------
@@ -146,7 +171,7 @@ static void add_parts(const float* part, int splits, const Product& p, const Epi
   note_launch();
 }
 
-static gsb_status launch_of(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st) {
+static gsb_status launch_of(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st) {
   switch (p->dtype) {
     case GSB_F32: return mma_launch_f32(p, e, count, bn, splits, st);
     case GSB_BF16: return mma_launch_bf16(p, e, count, bn, splits, st);
@@ -155,26 +180,32 @@ static gsb_status launch_of(const Product* p, const Epilogue* e, int count, int 
   }
 }
 
-gsb_status mma_product(const Product& p, const Epilogue& e, const Plan& plan, void* part, cudaStream_t st) {
-  if (plan.splits == 1) return launch_of(&p, &e, 1, plan.bn, 1, st);
-  Product sums = p;
-  sums.out_dtype = GSB_F32;
-  Epilogue plain{};
-  plain.out = part;
-  plain.out_stride = p.n;
-  plain.vec = p.n % 4 == 0;
-  if (gsb_status s = launch_of(&sums, &plain, 1, plan.bn, plan.splits, st); s != GSB_OK) return s;
-  const int blocks = k_blocks_of(p), per = (blocks + plan.splits - 1) / plan.splits;
-  const int pieces = (blocks + per - 1) / per;
-  const float* f = static_cast<const float*>(part);
-  if (p.out_dtype == GSB_F32) add_parts<float>(f, pieces, p, e, st);
-  else if (p.out_dtype == GSB_BF16) add_parts<bf16>(f, pieces, p, e, st);
-  else add_parts<f16>(f, pieces, p, e, st);
+gsb_status mma_products(const Product* p, const Epilogue* e, int count, const Plan& plan, void* part, cudaStream_t st) {
+  Product q[2];
+  Epilogue f[2];
+  float* sums[2] = {};
+  char* next = static_cast<char*>(part);
+  for (int i = 0; i < count; ++i) {
+    q[i] = p[i];
+    f[i] = e[i];
+    if (!leaves_sums(p, count, plan, i)) continue;
+    sums[i] = reinterpret_cast<float*>(next);
+    next += align_up(size_t(plan.splits[i]) * size_t(p[i].m) * size_t(p[i].n) * 4);
+    q[i].out_dtype = GSB_F32;
+    f[i] = Epilogue{};
+    f[i].out = sums[i];
+    f[i].out_stride = p[i].n;
+    f[i].vec = p[i].n % 4 == 0;
+  }
+  if (gsb_status s = launch_of(q, f, count, plan.bn, plan.splits, st); s != GSB_OK) return s;
+  for (int i = 0; i < count; ++i) {
+    if (!sums[i]) continue;
+    const int pieces = pieces_of(p[i], plan.splits[i]);
+    if (p[i].out_dtype == GSB_F32) add_parts<float>(sums[i], pieces, p[i], e[i], st);
+    else if (p[i].out_dtype == GSB_BF16) add_parts<bf16>(sums[i], pieces, p[i], e[i], st);
+    else add_parts<f16>(sums[i], pieces, p[i], e[i], st);
+  }
   return launch_status();
-}
-
-gsb_status mma_pair(const Product (&p)[2], const Epilogue (&e)[2], const Plan& plan, cudaStream_t st) {
-  return launch_of(p, e, 2, plan.bn, 1, st);
 }
 
 }  // namespace gsb

@@ -11,10 +11,11 @@
 // Operands are K-major (rows of k) or MN-major (rows of m or n, as the backward's products have
 // them): the TMA box and the shared-memory descriptor differ, nothing is transposed in memory.
 //
-// Float operands (PLANES = 3) are sums of three bf16 parts; the products (3,1) (1,3) (2,2) (1,2)
-// (2,1) go to one accumulator and (1,1) to another, and every kChunk blocks of K both are added to
-// float registers: the tensor core's additions truncate, and a long chain of them loses about
-// steps x 2^-25 of the sum.
+// Float operands (PLANES = 3) are sums of three bf16 parts.  The tensor core's additions truncate, and
+// a chain of them loses about steps x 2^-25 of what the accumulator holds.  So every block of 64 k has a
+// chain of its own, the products (3,1) (1,3) (2,2) (1,2) (2,1), which are small, before the four
+// steps of (1,1), and the epilogue warps add each block's sums in float registers while the next
+// block runs: 128 sums per thread, for which they take registers from the other warps.
 //
 // Every wait is bounded (4 s).  A wait that gives up sets a sticky flag, its CTA's remaining tiles
 // become NaN, and every role leaves its loop.
@@ -35,7 +36,8 @@ constexpr int kEpiWarps = 8;
 constexpr int kStageBytes = kEpiWarps * 32 * 32 * 4;  // a 32 x 32 block of floats per epilogue warp
 constexpr int kRowBytes = 128;              // one swizzled row of a box
 constexpr int kABytes = 128 * kRowBytes;
-constexpr int kChunk = 4;                   // PLANES = 3: blocks of 64 k per accumulation chain
+// Registers per thread after the split (PLANES = 3); 128 x 56 + 256 x 224 are the 384 x 168 of the launch.
+constexpr int kFewRegs = 56, kManyRegs = 224;
 
 
 // One product of a launch: m_tiles x n_tiles tiles, each walked in `splits` pieces of `per_split` blocks of
@@ -401,7 +403,7 @@ struct Shape {
   static constexpr int kBudget = 232448 - 1024 - kStageBytes - 256;
   static constexpr int kSlots = kBudget / kSlot < 8 ? kBudget / kSlot : 8;
   static constexpr int kBufs = 2;
-  static constexpr int kAccCols = PLANES == 1 ? BN : 2 * BN;  // TMEM columns of one accumulator buffer
+  static constexpr int kAccCols = BN;  // TMEM columns of one accumulator buffer
   static constexpr int kCols = kBufs * kAccCols;
   static constexpr int kBytes = 1024 + kSlots * kSlot + kStageBytes + 256;
   static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0 && kCols >= 32, "TMEM columns");
@@ -448,119 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
   int which;
   int64_t u;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      int s = 0;
-      uint32_t phase = 0;
-      for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
-        const Job& job = p.job[which];
-        const CUtensorMap* map_a = &p.a[which];
-        const CUtensorMap* map_b = &p.b[which];
-        const bool a_mn = BWD && job.a_mn;
-        int64_t mt, nt;
-        tile_of(job, u / job.splits, mt, nt);
-        const int i0 = int((mt * CG + rank) * 128);
-        const int j0 = int(nt * BN + rank * S::kBRows);
-        const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
-        for (int kb = kb0; ok && kb < kb1; ++kb) {
-          const int k0 = kb * kElems;
-#pragma unroll
-          for (int q = 0; q < PLANES; ++q) {
-            const int plane = PLANES == 1 ? 0 : (q == 0 ? 2 : q - 1);  // parts 3, 1, 2
-            if (!(ok = bar_wait(empty(s), phase ^ 1, p.gave_up))) break;
-            const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
-            if (rank == 0) bar_expect(full(s), CG * S::kSlot);
-            const uint32_t a = base + s * S::kSlot, b = a + kABytes;
-            if (a_mn) {
-#pragma unroll
-              for (int v = 0; v < 2; ++v) tma_load<CG>(a + v * 8192, map_a, i0 + 64 * v, k0, plane, bar);
-            } else {
-              tma_load<CG>(a, map_a, k0, i0, plane, bar);
-            }
-            if constexpr (BWD) {
-#pragma unroll
-              for (int v = 0; v < S::kBRows / 64; ++v) tma_load<CG>(b + v * 8192, map_b, j0 + 64 * v, k0, plane, bar);
-            } else {
-              tma_load<CG>(b, map_b, k0, j0, plane, bar);
-            }
-            if (++s == S::kSlots) s = 0, phase ^= 1;
-          }
-        }
-      }
-      // every slot released: no arrival of a commit comes after the CTA's end
-      for (int q = 0; ok && q < S::kSlots; ++q) {
-        ok = bar_wait(empty(s), phase ^ 1, p.gave_up);
-        if (++s == S::kSlots) s = 0, phase ^= 1;
-      }
-      if (!ok) let_copies_land();
-    }
-  } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
-      bool ok = true;
-      int s = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      const auto next = [&](int x) { return x + 1 == S::kSlots ? 0 : x + 1; };
-      for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
-        const Job& job = p.job[which];
-        const bool a_mn = BWD && job.a_mn;
-        const uint32_t idesc = job.idesc, a_step = desc_step(a_mn), b_step = desc_step(BWD);
-        const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
-        for (int kb = kb0; ok && kb < kb1;) {
-          if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
-          fence_after();
-          const uint32_t acc = tmem + buf * S::kAccCols;
-          const int stop = PLANES == 1 ? kb1 : min(kb1, kb + kChunk);
-          uint32_t more = 0, more_low = 0;
-          for (; kb < stop; ++kb) {
-            if constexpr (PLANES == 1) {
-              if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
-              fence_after();
-              const uint64_t a = smem_desc(base + s * S::kSlot, a_mn);
-              const uint64_t b = smem_desc(base + s * S::kSlot + kABytes, BWD);
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
-                more = 1;
-              }
-              mma_commit<CG>(empty(s));
-              if (++s == S::kSlots) s = 0, phase ^= 1;
-            } else {
-              const int s3 = s, s1 = next(s3), s2 = next(s1);
-              const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
-              const auto da = [&](int q) { return smem_desc(base + q * S::kSlot, a_mn); };
-              const auto db = [&](int q) { return smem_desc(base + q * S::kSlot + kABytes, BWD); };
-              const auto run = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t& on) {
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                  mma_issue<KIND, CG>(d, a + v * a_step, b + v * b_step, idesc, on);
-                  on = 1;
-                }
-              };
-              if (!(ok = bar_wait(full(s3), phase, p.gave_up) && bar_wait(full(s1), ph1, p.gave_up))) break;
-              fence_after();
-              run(acc + BN, da(s3), db(s1), more_low);
-              run(acc + BN, da(s1), db(s3), more_low);
-              mma_commit<CG>(empty(s3));
-              if (!(ok = bar_wait(full(s2), ph2, p.gave_up))) break;
-              fence_after();
-              run(acc + BN, da(s2), db(s2), more_low);
-              run(acc + BN, da(s1), db(s2), more_low);
-              run(acc + BN, da(s2), db(s1), more_low);
-              mma_commit<CG>(empty(s2));
-              run(acc, da(s1), db(s1), more);
-              mma_commit<CG>(empty(s1));
-              s = next(s2);
-              phase = ph2 ^ (s < s2);
-            }
-          }
-          mma_commit<CG>(acc_full(buf));
-          buf ^= 1;
-          if (buf == 0) acc_phase ^= 1;
-        }
-      }
-    }
-  } else if (warp >= 4) {
+  if (warp >= 4) {
+    if constexpr (PLANES > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     const int w = warp - 4, quad = warp & 3, half = w >> 2;  // quad: the 32 TMEM lanes this warp may read
     float* stage = stage_all + w * 32 * 32;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
@@ -611,31 +502,151 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
 #pragma unroll
         for (int u = 0; u < kHalfCols; ++u) sum[u] = 0.0f;
         const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
-        for (int kb = kb0; kb < kb1; kb += kChunk) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           ok = __all_sync(0xffffffffu, ok && bar_wait(acc_full(buf), acc_phase, p.gave_up));
           fence_after();
           const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
 #pragma unroll
-          for (int c = 0; c < kHalfCols; c += 16) {
-            float low[16], high[16];
-            tmem_load16(acc + BN + c, low);
-            tmem_load16(acc + c, high);
+          for (int c = 0; c < kHalfCols; c += 64) {
+            uint32_t v[32], w2[32];
+            tmem_start32(acc + c, v);
+            tmem_start32(acc + c + 32, w2);
+            tmem_wait32(v);
+            tmem_wait32(w2);
 #pragma unroll
-            for (int u = 0; u < 16; ++u) sum[c + u] += high[u] + low[u];
+            for (int q = 0; q < 32; ++q) sum[c + q] += __uint_as_float(v[q]);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) sum[c + 32 + q] += __uint_as_float(w2[q]);
           }
           release(buf);
           buf ^= 1;
           if (buf == 0) acc_phase ^= 1;
         }
+        if (!ok) {
+#pragma unroll
+          for (int q = 0; q < kHalfCols; ++q) sum[q] = __int_as_float(0x7fc00000);
+        }
         rows.start(job, i0, plane);
 #pragma unroll
         for (int c = 0; c < kHalfCols; c += 32) {
+          rows.put(stage, reinterpret_cast<const uint32_t(&)[32]>(sum[c]));
           rows.prefetch(job, j0 + c, ahead);
-          uint32_t v[32];
-#pragma unroll
-          for (int q = 0; q < 32; ++q) v[q] = ok ? __float_as_uint(sum[c + q]) : 0x7fc00000;
-          rows.put(stage, v);
           if (i0 < job.m && j0 + c < job.n) rows.emit(job, stage, i0, j0 + c, ahead);
+        }
+      }
+    }
+  } else {
+    if constexpr (PLANES > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    if (warp == 0) {
+      if (lane == 0) {
+        bool ok = true;
+        int s = 0;
+        uint32_t phase = 0;
+        for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
+          const Job& job = p.job[which];
+          const CUtensorMap* map_a = &p.a[which];
+          const CUtensorMap* map_b = &p.b[which];
+          const bool a_mn = BWD && job.a_mn;
+          int64_t mt, nt;
+          tile_of(job, u / job.splits, mt, nt);
+          const int i0 = int((mt * CG + rank) * 128);
+          const int j0 = int(nt * BN + rank * S::kBRows);
+          const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
+          for (int kb = kb0; ok && kb < kb1; ++kb) {
+            const int k0 = kb * kElems;
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q) {
+              const int plane = PLANES == 1 ? 0 : (q == 0 ? 2 : q - 1);  // parts 3, 1, 2
+              if (!(ok = bar_wait(empty(s), phase ^ 1, p.gave_up))) break;
+              const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
+              if (rank == 0) bar_expect(full(s), CG * S::kSlot);
+              const uint32_t a = base + s * S::kSlot, b = a + kABytes;
+              if (a_mn) {
+#pragma unroll
+                for (int v = 0; v < 2; ++v) tma_load<CG>(a + v * 8192, map_a, i0 + 64 * v, k0, plane, bar);
+              } else {
+                tma_load<CG>(a, map_a, k0, i0, plane, bar);
+              }
+              if constexpr (BWD) {
+#pragma unroll
+                for (int v = 0; v < S::kBRows / 64; ++v) tma_load<CG>(b + v * 8192, map_b, j0 + 64 * v, k0, plane, bar);
+              } else {
+                tma_load<CG>(b, map_b, k0, j0, plane, bar);
+              }
+              if (++s == S::kSlots) s = 0, phase ^= 1;
+            }
+          }
+        }
+        // every slot released: no arrival of a commit comes after the CTA's end
+        for (int q = 0; ok && q < S::kSlots; ++q) {
+          ok = bar_wait(empty(s), phase ^ 1, p.gave_up);
+          if (++s == S::kSlots) s = 0, phase ^= 1;
+        }
+        if (!ok) let_copies_land();
+      }
+    } else if (warp == 1) {
+      if (rank == 0 && lane == 0) {
+        bool ok = true;
+        int s = 0, buf = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        const auto next = [&](int x) { return x + 1 == S::kSlots ? 0 : x + 1; };
+        for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
+          const Job& job = p.job[which];
+          const bool a_mn = BWD && job.a_mn;
+          const uint32_t idesc = job.idesc, a_step = desc_step(a_mn), b_step = desc_step(BWD);
+          const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
+          for (int kb = kb0; ok && kb < kb1;) {
+            if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
+            fence_after();
+            const uint32_t acc = tmem + buf * S::kAccCols;
+            const int stop = PLANES == 1 ? kb1 : kb + 1;
+            uint32_t more = 0;
+            for (; kb < stop; ++kb) {
+              if constexpr (PLANES == 1) {
+                if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
+                fence_after();
+                const uint64_t a = smem_desc(base + s * S::kSlot, a_mn);
+                const uint64_t b = smem_desc(base + s * S::kSlot + kABytes, BWD);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                  mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
+                  more = 1;
+                }
+                mma_commit<CG>(empty(s));
+                if (++s == S::kSlots) s = 0, phase ^= 1;
+              } else {
+                const int s3 = s, s1 = next(s3), s2 = next(s1);
+                const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
+                const auto da = [&](int q) { return smem_desc(base + q * S::kSlot, a_mn); };
+                const auto db = [&](int q) { return smem_desc(base + q * S::kSlot + kABytes, BWD); };
+                const auto run = [&](uint64_t a, uint64_t b) {
+#pragma unroll
+                  for (int v = 0; v < 4; ++v) {
+                    mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
+                    more = 1;
+                  }
+                };
+                if (!(ok = bar_wait(full(s3), phase, p.gave_up) && bar_wait(full(s1), ph1, p.gave_up))) break;
+                fence_after();
+                run(da(s3), db(s1));
+                run(da(s1), db(s3));
+                mma_commit<CG>(empty(s3));
+                if (!(ok = bar_wait(full(s2), ph2, p.gave_up))) break;
+                fence_after();
+                run(da(s2), db(s2));
+                run(da(s1), db(s2));
+                run(da(s2), db(s1));
+                mma_commit<CG>(empty(s2));
+                run(da(s1), db(s1));
+                mma_commit<CG>(empty(s1));
+                s = next(s2);
+                phase = ph2 ^ (s < s2);
+              }
+            }
+            mma_commit<CG>(acc_full(buf));
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1;
+          }
         }
       }
     }
@@ -691,7 +702,7 @@ bool make_job(Job& j, CUtensorMap* a, CUtensorMap* b, const Product& p, const Ep
   j.m = p.m;
   j.n = p.n;
   j.k_blocks = k_blocks_of(p);
-  j.per_split = (j.k_blocks + splits - 1) / splits;
+  j.per_split = piece_of(p, splits);
   j.splits = (j.k_blocks + j.per_split - 1) / j.per_split;
   j.part_stride = j.splits > 1 ? p.m * p.n : 0;
   j.m_tiles = int((p.m + 128 * CG - 1) / (128 * CG));
@@ -706,7 +717,7 @@ bool make_job(Job& j, CUtensorMap* a, CUtensorMap* b, const Product& p, const Ep
 
 // products[0 .. count): one forward product, or one or two of the backward's.
 template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT>
-gsb_status launch(const Product* products, const Epilogue* e, int count, int splits, cudaStream_t st) {
+gsb_status launch(const Product* products, const Epilogue* e, int count, const int* splits, cudaStream_t st) {
   using S = Shape<CG, BN, PLANES>;
   auto* kernel = mma_kernel<KIND, CG, BN, BWD, PLANES, O, ACT>;
   int dev = 0;
@@ -722,10 +733,11 @@ gsb_status launch(const Product* products, const Epilogue* e, int count, int spl
   }
   Args<1 + BWD> a{};
   int64_t units = 0;
-  const bool swap = count == 2 && k_blocks_of(products[1]) > k_blocks_of(products[0]);  // the longer first
+  // the product of the longer pieces first
+  const bool swap = count == 2 && piece_of(products[1], splits[1]) > piece_of(products[0], splits[0]);
   for (int i = 0; i < count; ++i) {
     const int from = swap ? 1 - i : i;
-    if (!make_job<KIND, CG, BN, PLANES>(a.job[i], &a.a[i], &a.b[i], products[from], e[from], splits))
+    if (!make_job<KIND, CG, BN, PLANES>(a.job[i], &a.a[i], &a.b[i], products[from], e[from], splits[from]))
       return GSB_ERR_CUDA;
     units += a.job[i].units;
   }
@@ -762,7 +774,7 @@ gsb_status launch(const Product* products, const Epilogue* e, int count, int spl
 }
 
 template <int KIND, int CG, int BN, int PLANES, typename O>
-gsb_status launch_fwd(const Product& p, const Epilogue& e, int splits, cudaStream_t st) {
+gsb_status launch_fwd(const Product& p, const Epilogue& e, const int* splits, cudaStream_t st) {
   switch (e.act) {
     case GSB_ACT_RELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_RELU>(&p, &e, 1, splits, st);
     case GSB_ACT_GELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_GELU>(&p, &e, 1, splits, st);

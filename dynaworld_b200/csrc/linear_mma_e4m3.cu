@@ -4,7 +4,7 @@
 namespace gsb {
 
 template <int BN>
-static gsb_status of_width(const Product& p, const Epilogue& e, int splits, cudaStream_t st) {
+static gsb_status of_width(const Product& p, const Epilogue& e, const int* splits, cudaStream_t st) {
   switch (p.out_dtype) {
     case GSB_F32: return mma::launch_fwd<1, 2, BN, 1, float>(p, e, splits, st);
     case GSB_BF16: return mma::launch_fwd<1, 2, BN, 1, bf16>(p, e, splits, st);
@@ -12,7 +12,7 @@ static gsb_status of_width(const Product& p, const Epilogue& e, int splits, cuda
   }
 }
 
-gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int, int bn, int splits, cudaStream_t st) {
+gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int, int bn, const int* splits, cudaStream_t st) {
   return bn == 256 ? of_width<256>(*p, *e, splits, st) : of_width<128>(*p, *e, splits, st);
 }
 

@@ -121,28 +121,34 @@ inline int k_blocks_of(const Product& p) {
   return int((p.k + per - 1) / per);
 }
 
+// Blocks of K of one of its `splits` pieces, and how many pieces that makes.
+inline int piece_of(const Product& p, int splits) { return (k_blocks_of(p) + splits - 1) / splits; }
+inline int pieces_of(const Product& p, int splits) {
+  const int per = piece_of(p, splits);
+  return (k_blocks_of(p) + per - 1) / per;
+}
+
 // How the tensor-core kernel walks a product: tiles of 256 x bn, each in `splits` pieces along K whose
 // float sums a second kernel adds (in order) and finishes.
 struct Plan {
   int bn;
-  int splits;
-  float cost;  // estimated, in blocks of K of a 256 x 256 tile
+  int splits[2];  // of the launch's one or two products
+  float cost;     // estimated, in blocks of K of a 256 x 256 tile
 };
 Plan plan_product(const Product& p);
-// The backward's two products in one launch (no splits).
-Plan plan_pair(const Product& p, const Product& q);
-size_t partial_bytes(const Product& p, const Plan& plan);
+// The backward's two products in one launch.
+Plan plan_pair(const Product (&p)[2]);
+size_t partial_bytes(const Product* p, int count, const Plan& plan);
 
 // The products (linear_mma.cu).  The operands' rows (and parts) start on 16-byte boundaries; `part` is
 // partial_bytes long.
-gsb_status mma_product(const Product& p, const Epilogue& e, const Plan& plan, void* part, cudaStream_t st);
-gsb_status mma_pair(const Product (&p)[2], const Epilogue (&e)[2], const Plan& plan, cudaStream_t st);
+gsb_status mma_products(const Product* p, const Epilogue* e, int count, const Plan& plan, void* part, cudaStream_t st);
 // By operand type: products[0 .. count) of one launch, count 2 only with b_mn.  out_dtype F32 beside
 // 16-bit operands writes sums (no epilogue).
-gsb_status mma_launch_bf16(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
-gsb_status mma_launch_f16(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
-gsb_status mma_launch_f32(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
-gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int count, int bn, int splits, cudaStream_t st);
+gsb_status mma_launch_bf16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
+gsb_status mma_launch_f16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
+gsb_status mma_launch_f32(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
+gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 // 1 once a bounded wait of a token-side kernel gave up on the current device.
 gsb_status gave_up_status(int* gave_up);
 
