@@ -47,30 +47,30 @@ gsb_status gave_up_status(int* gave_up) {
 
 // ---- plans ------------------------------------------------------------------------------------
 //
-// Costs in units of one 64-element block of K of a 256 x 256 tile (about 0.27 us).  A 256 x 128
-// tile's block costs 0.9 of that (8192 x 4096 x 4096 bf16: 351 us in 128-wide tiles, 195 in 256-wide
-// ones), a float block (six products) 6.
-// A launch ends with one exposed epilogue (about 2 us, half of it for 128 columns); pieces along K
+// Costs in units of one 64-element block of K of a 256 x 256 tile (about 0.27 us).
+// A launch ends with one exposed epilogue (about 2 us, less for narrower tiles); pieces along K
 // cost a second kernel (about 4 us) and their sums' way through L2.
-constexpr float kBlock128 = 0.9f, kBlockF32 = 6.0f, kTail256 = 8.0f, kTail128 = 4.0f, kReduce = 14.0f;
+constexpr float kReduce = 14.0f;
 constexpr float kPartialPerMB = 1.0f;  // written and read once
 
 struct Walk {
   int bn;
+  int rows;     // of a tile
   float block, tail;
 };
 
-static int walks_of(int dtype, Walk (&w)[2]) {
-  if (dtype == GSB_F32) {
-    w[0] = {256, kBlockF32, kTail256};
-    return 1;
-  }
-  w[0] = {256, 1.0f, kTail256};
-  w[1] = {128, kBlock128, kTail128};
-  return 2;
-}
+// What a block of K of each tile costs.  An MMA takes about 128 cycles whether its B has 64 columns or
+// 256 (A's 128 rows have to be read for each; 8192 x 4096 x 4096 bf16 took 195 us in 256-wide tiles
+// and 351 us in 128-wide ones), so narrow tiles only serve to fill the GPU and to end sooner.
+static const Walk kWalks[3] = {{256, 256, 1.0f, 8.0f}, {128, 128, 0.95f, 4.0f}, {64, 128, 0.9f, 2.5f}};
+constexpr float kFloatBlock = 6.0f;  // six products
 
-static int64_t tiles_of(const Product& p, int bn) { return ((p.m + 255) / 256) * ((p.n + bn - 1) / bn); }
+static float block_cost(const Product& p, const Walk& w) { return p.dtype == GSB_F32 ? kFloatBlock * w.block : w.block; }
+static int64_t workers_of(const Walk& w) { return w.rows == 256 ? sm_count() / 2 : sm_count(); }
+
+static int64_t tiles_of(const Product& p, const Walk& w) {
+  return ((p.m + w.rows - 1) / w.rows) * ((p.n + w.bn - 1) / w.bn);
+}
 
 // The second kernel and its sums' traffic.
 static float reduce_cost(const Product& p, int splits) {
@@ -82,17 +82,14 @@ static bool may_split(const Product& p, int splits, int64_t tiles, int64_t clust
 }
 
 Plan plan_product(const Product& p) {
-  const int64_t clusters = sm_count() / 2;
   Plan best{0, {1, 1}, 0.0f};
-  Walk walks[2];
-  const int n = walks_of(p.dtype, walks);
-  for (int i = 0; i < n; ++i) {
-    const int64_t tiles = tiles_of(p, walks[i].bn);
-    for (int s = 1; s <= 16 && may_split(p, s, tiles, clusters); s *= 2) {
-      const int64_t rounds = (tiles * s + clusters - 1) / clusters;
-      float cost = float(rounds) * float(piece_of(p, s)) * walks[i].block + walks[i].tail;
+  for (const Walk& w : kWalks) {
+    const int64_t workers = workers_of(w), tiles = tiles_of(p, w);
+    for (int s = 1; s <= 16 && may_split(p, s, tiles, workers); s *= 2) {
+      const int64_t rounds = (tiles * s + workers - 1) / workers;
+      float cost = float(rounds) * float(piece_of(p, s)) * block_cost(p, w) + w.tail;
       if (s > 1) cost += reduce_cost(p, s);
-      if (best.bn == 0 || cost < best.cost) best = {walks[i].bn, {s, 1}, cost};
+      if (best.bn == 0 || cost < best.cost) best = {w.bn, {s, 1}, cost};
     }
   }
   return best;
@@ -106,22 +103,19 @@ static bool leaves_sums(const Product* p, int count, const Plan& plan, int i) {
 }
 
 Plan plan_pair(const Product (&p)[2]) {
-  const int64_t clusters = sm_count() / 2;
   Plan best{0, {1, 1}, 0.0f};
-  Walk walks[2];
-  const int n = walks_of(p[0].dtype, walks);
-  for (int i = 0; i < n; ++i) {
-    const int64_t t0 = tiles_of(p[0], walks[i].bn), t1 = tiles_of(p[1], walks[i].bn);
-    for (int s0 = 1; s0 <= 16 && may_split(p[0], s0, t0, clusters); s0 *= 2)
-      for (int s1 = 1; s1 <= 16 && may_split(p[1], s1, t1, clusters); s1 *= 2) {
-        const Plan plan{walks[i].bn, {s0, s1}, 0.0f};
-        const float a = float(piece_of(p[0], s0)) * walks[i].block, b = float(piece_of(p[1], s1)) * walks[i].block;
-        const float all = (float(t0 * s0) * a + float(t1 * s1) * b) / float(clusters);
+  for (const Walk& w : kWalks) {
+    const int64_t workers = workers_of(w), t0 = tiles_of(p[0], w), t1 = tiles_of(p[1], w);
+    for (int s0 = 1; s0 <= 16 && may_split(p[0], s0, t0, workers); s0 *= 2)
+      for (int s1 = 1; s1 <= 16 && may_split(p[1], s1, t1, workers); s1 *= 2) {
+        const Plan plan{w.bn, {s0, s1}, 0.0f};
+        const float a = float(piece_of(p[0], s0)) * block_cost(p[0], w), b = float(piece_of(p[1], s1)) * block_cost(p[1], w);
+        const float all = (float(t0 * s0) * a + float(t1 * s1) * b) / float(workers);
         // an even share, at least the longer piece, and half of the shorter one lost at the end
-        float cost = std::max(all + 0.5f * std::min(a, b), std::max(a, b)) + walks[i].tail;
+        float cost = std::max(all + 0.5f * std::min(a, b), std::max(a, b)) + w.tail;
         for (int k = 0; k < 2; ++k)
           if (leaves_sums(p, 2, plan, k)) cost += reduce_cost(p[k], plan.splits[k]);
-        if (best.bn == 0 || cost < best.cost) best = {plan.bn, {s0, s1}, cost};
+        if (best.bn == 0 || cost < best.cost) best = {w.bn, {s0, s1}, cost};
       }
   }
   return best;

@@ -1,7 +1,7 @@
 // Matrix product on the fifth-generation tensor cores (sm_100a): D = A B^T in float.
 //
 // Persistent kernel, one CTA per SM; CG = 2 pairs the CTAs of a cluster on one 256 x BN tile, so
-// that each loads half of B.  Warp roles of a CTA (384 threads):
+// that each loads half of B, CG = 1 gives each a 128 x BN tile.  Warp roles of a CTA (384 threads):
 //   warp 0      loads: TMA copies of 128-byte wide boxes (swizzled) into a ring of slots
 //   warp 1      issues tcgen05.mma, accumulators in TMEM (two buffers: the next tile's products
 //               run while this tile's epilogue reads)
@@ -162,18 +162,6 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int plane, uint32_t bar) {
   if constexpr (CG == 1)
@@ -246,6 +234,14 @@ __device__ __forceinline__ int stage_at(int r, int q) { return r * 32 + ((q ^ (r
 // that global accesses are 16 bytes per lane: V values, 32 / V lanes per row, kSteps rows per lane.
 // The residual and bias of the next block are loaded while this one is finished: a block takes
 // about 600 cycles, the residual's way from HBM more.
+constexpr int kAnyAct = -1;  // the activation is chosen at run time
+
+template <int ACT, int V>
+__device__ __forceinline__ void activate(const Job& p, float (&z)[V]) {
+  if constexpr (ACT == kAnyAct) apply_act<V>(p.e.act, z);
+  else apply_value<ACT, V>(z);
+}
+
 template <typename O, int ACT>
 struct Rows {
   static constexpr int V = 16 / int(sizeof(O));
@@ -253,9 +249,18 @@ struct Rows {
   static constexpr int kAtOnce = 32 / kPerRow;  // rows in one access of the warp
   static constexpr int kSteps = 32 / kAtOnce;
   using Z = typename PreactOf<O>::type;
+  // What a block's epilogue reads from global memory.  Aligned: kSteps x 16 bytes of the residual and V
+  // values of the bias; else a column per lane: its 32 rows of the residual, one value of the bias.
   struct Ahead {
-    uint4 res[kSteps];
-    uint4 bias;
+    union {
+      uint4 res[kSteps];
+      O col[32];
+    };
+    union {
+      uint4 bias;
+      O bias1;
+    };
+    __device__ __forceinline__ Ahead() {}
   };
   int row0, col;  // this lane's first row and column within the block
   int steps;      // its rows inside the matrix
@@ -277,8 +282,21 @@ struct Rows {
   }
 
   __device__ __forceinline__ void prefetch(const Job& p, int64_t j0, Ahead& a) const {
+    if (!p.e.vec) {
+      const int64_t j = j0 + (threadIdx.x & 31);
+      if (j >= p.n) return;
+      if (p.e.bias) a.bias1 = static_cast<const O*>(p.e.bias)[j];
+      if (p.e.res) {
+        const int64_t i0 = i - row0;
+        const O* r = static_cast<const O*>(p.e.res) + i0 * p.e.res_stride + j;
+#pragma unroll
+        for (int q = 0; q < 32; ++q)
+          if (i0 + q < p.m) a.col[q] = r[q * p.e.res_stride];
+      }
+      return;
+    }
     const int64_t j = j0 + col;
-    const bool in = p.e.vec && j < p.n;
+    const bool in = j < p.n;
     if (p.e.bias && in) a.bias = __ldg(reinterpret_cast<const uint4*>(static_cast<const O*>(p.e.bias) + j));
     if (p.e.res) {
       const O* r = static_cast<const O*>(p.e.res) + i * p.e.res_stride + j;
@@ -344,7 +362,7 @@ struct Rows {
                 *reinterpret_cast<Vec<Z, V>*>(keep + (s0 + h) * kAtOnce * p.n) =
                     kept_of<V>(static_cast<Z*>(nullptr), reinterpret_cast<const float(&)[V]>(z[h * V]));
           }
-          apply_value<ACT, 2 * V>(z);
+          activate<ACT, 2 * V>(p, z);
           if (p.e.res) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -360,34 +378,36 @@ struct Rows {
         }
       }
     } else {
-      // rows that start anywhere: a lane per column, eight rows' loads in flight
+      // rows that start anywhere: a lane per column
       const int64_t j = j0 + lane;
       if (j < p.n) {
-        const float b = p.e.bias ? to_f32(static_cast<const O*>(p.e.bias)[j]) : 0.0f;
+        const float b = p.e.bias ? to_f32(a.bias1) : 0.0f;
         const float cs = p.e.row_scale ? p.e.col_scale[j] : 1.0f;
+        O* out = static_cast<O*>(p.e.out) + plane + i0 * p.e.out_stride + j;
+        Z* keep = static_cast<Z*>(p.e.preact) + i0 * p.n + j;
+        const int rows = int(min(int64_t(32), p.m - i0));
+#pragma unroll
         for (int r0 = 0; r0 < 32; r0 += 8) {
-          const int rows = int(min(int64_t(8), p.m - i0 - r0));
-          float z[8], add[8];
+          float z[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             z[r] = stage[stage_at(r0 + r, lane >> 2) + (lane & 3)];
-            add[r] = 0.0f;
-            if (r < rows) {
-              if (p.e.row_scale) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
-              if (p.e.res) add[r] = to_f32(static_cast<const O*>(p.e.res)[(i0 + r0 + r) * p.e.res_stride + j]);
-            }
+            if (p.e.row_scale && r0 + r < rows) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
             z[r] += b;
           }
           if (p.e.preact) {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-              if (r < rows)
-                static_cast<Z*>(p.e.preact)[(i0 + r0 + r) * p.n + j] = as_preact(static_cast<Z*>(nullptr), z[r]);
+              if (r0 + r < rows) keep[(r0 + r) * p.n] = as_preact(static_cast<Z*>(nullptr), z[r]);
           }
-                    apply_value<ACT, 8>(z);
+          activate<ACT, 8>(p, z);
+          if (p.e.res) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) z[r] += to_f32(a.col[r0 + r]);
+          }
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (r < rows) static_cast<O*>(p.e.out)[plane + (i0 + r0 + r) * p.e.out_stride + j] = from_f32<O>(z[r] + add[r]);
+            if (r0 + r < rows) out[(r0 + r) * p.e.out_stride] = from_f32<O>(z[r]);
         }
       }
     }
@@ -498,6 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       } else {
+        constexpr int kAtOnce = kHalfCols < 64 ? kHalfCols : 64;  // columns on their way from TMEM
         float sum[kHalfCols];
 #pragma unroll
         for (int u = 0; u < kHalfCols; ++u) sum[u] = 0.0f;
@@ -507,16 +528,14 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
           fence_after();
           const uint32_t acc = tmem + lanes + buf * S::kAccCols + half * kHalfCols;
 #pragma unroll
-          for (int c = 0; c < kHalfCols; c += 64) {
-            uint32_t v[32], w2[32];
-            tmem_start32(acc + c, v);
-            tmem_start32(acc + c + 32, w2);
-            tmem_wait32(v);
-            tmem_wait32(w2);
+          for (int c = 0; c < kHalfCols; c += kAtOnce) {
+            uint32_t v[kAtOnce / 32][32];
 #pragma unroll
-            for (int q = 0; q < 32; ++q) sum[c + q] += __uint_as_float(v[q]);
+            for (int h = 0; h < kAtOnce / 32; ++h) tmem_start32(acc + c + 32 * h, v[h]);
 #pragma unroll
-            for (int q = 0; q < 32; ++q) sum[c + 32 + q] += __uint_as_float(w2[q]);
+            for (int h = 0; h < kAtOnce / 32; ++h) tmem_wait32(v[h]);
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) sum[c + q] += __uint_as_float(v[q / 32][q % 32]);
           }
           release(buf);
           buf ^= 1;
@@ -773,15 +792,27 @@ gsb_status launch(const Product* products, const Epilogue* e, int count, const i
   return launch_status();
 }
 
-template <int KIND, int CG, int BN, int PLANES, typename O>
-gsb_status launch_fwd(const Product& p, const Epilogue& e, const int* splits, cudaStream_t st) {
+// By tile: 256 is 256 x 256 over a pair of CTAs, 128 and 64 are 128 rows by that many columns on one
+// CTA (fewer of them are worth an instance per activation).
+template <int KIND, int PLANES, typename O>
+gsb_status launch_fwd(const Product& p, const Epilogue& e, int bn, const int* splits, cudaStream_t st) {
+  if (bn == 128) return launch<KIND, 1, 128, false, PLANES, O, kAnyAct>(&p, &e, 1, splits, st);
+  if (bn == 64) return launch<KIND, 1, 64, false, PLANES, O, kAnyAct>(&p, &e, 1, splits, st);
   switch (e.act) {
-    case GSB_ACT_RELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_RELU>(&p, &e, 1, splits, st);
-    case GSB_ACT_GELU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_GELU>(&p, &e, 1, splits, st);
-    case GSB_ACT_GELU_TANH: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_GELU_TANH>(&p, &e, 1, splits, st);
-    case GSB_ACT_SILU: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_SILU>(&p, &e, 1, splits, st);
-    default: return launch<KIND, CG, BN, false, PLANES, O, GSB_ACT_NONE>(&p, &e, 1, splits, st);
+    case GSB_ACT_RELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_RELU>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU_TANH: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU_TANH>(&p, &e, 1, splits, st);
+    case GSB_ACT_SILU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_SILU>(&p, &e, 1, splits, st);
+    default: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_NONE>(&p, &e, 1, splits, st);
   }
+}
+
+// One product without an epilogue (BWD: one or two).
+template <int KIND, bool BWD, int PLANES, typename O>
+gsb_status launch_plain(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st) {
+  if (bn == 128) return launch<KIND, 1, 128, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
+  if (bn == 64) return launch<KIND, 1, 64, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
+  return launch<KIND, 2, 256, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
 }
 
 }  // namespace mma

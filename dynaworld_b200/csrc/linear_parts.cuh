@@ -128,7 +128,7 @@ inline int pieces_of(const Product& p, int splits) {
   return (k_blocks_of(p) + per - 1) / per;
 }
 
-// How the tensor-core kernel walks a product: tiles of 256 x bn, each in `splits` pieces along K whose
+// How the tensor-core kernel walks a product: tiles of 256 x 256 (bn 256) or 128 x bn, each in `splits` pieces along K whose
 // float sums a second kernel adds (in order) and finishes.
 struct Plan {
   int bn;
@@ -145,6 +145,7 @@ size_t partial_bytes(const Product* p, int count, const Plan& plan);
 gsb_status mma_products(const Product* p, const Epilogue* e, int count, const Plan& plan, void* part, cudaStream_t st);
 // By operand type: products[0 .. count) of one launch, count 2 only with b_mn.  out_dtype F32 beside
 // 16-bit operands writes sums (no epilogue).
+gsb_status mma_launch_sums16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 gsb_status mma_launch_bf16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 gsb_status mma_launch_f16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 gsb_status mma_launch_f32(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
