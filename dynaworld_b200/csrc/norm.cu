@@ -424,7 +424,7 @@ gsb_status bwd_of_type(const NormArgs& a, void* dw, cudaStream_t st) {
 gsb_status check_norm(const gsb_norm* n) {
   if (!n) return GSB_ERR_ARG;
   if (n->dtype != GSB_F32 && n->dtype != GSB_BF16 && n->dtype != GSB_F16) return GSB_ERR_ARG;
-  if (n->rows < 0 || n->rows > 0x7fffffff || n->dim <= 0) return GSB_ERR_SHAPE;
+  if (n->rows < 0 || n->rows > 0x7fffffff || n->dim < 1 || n->dim > (1 << 24)) return GSB_ERR_SHAPE;
   if (n->rows > 0 && !n->x) return GSB_ERR_ARG;
   return GSB_OK;
 }

@@ -381,7 +381,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
 
 int check_norm(const char* what, const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
   const int code = check_input(what, x);
-  TORCH_CHECK_VALUE(x.size(-1) <= INT32_MAX, what, ": rows of ", x.size(-1), " values are too long");
+  TORCH_CHECK_VALUE(x.size(-1) <= (1 << 24), what, ": rows of ", x.size(-1), " values are too long");
   if (weight) check_like(what, "weight", *weight, {x.size(-1)}, x.scalar_type(), x);
   if (residual) check_like(what, "residual", *residual, x.sizes(), x.scalar_type(), x);
   TORCH_CHECK_VALUE(eps >= 0.0, what, ": eps must not be negative, got ", eps);

@@ -392,7 +392,8 @@ GSB_API gsb_status gsb_splats2d_preprocess_bwd(const gsb_splats2d* splats, const
 #define GSB_E4M3 3 /* 8-bit codes: a value is code * scale of its row */
 
 /* Rows [rows, dim] of `dtype` (F32, BF16 or F16).  Strides count elements between rows; a row's
-   elements are adjacent.  Outputs are contiguous.  0 <= rows <= 2^31 - 1. */
+   elements are adjacent.  Outputs are contiguous.  0 <= rows <= 2^31 - 1,
+   1 <= dim <= 2^24. */
 typedef struct gsb_norm {
   int64_t rows;
   int32_t dim;

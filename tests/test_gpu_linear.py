@@ -117,7 +117,9 @@ def check(x, w, b, r, dy, act, grads=True):
 # one token, few tokens, tile edges and one past them, odd widths, long sums, widths below a vector
 SHAPES = [(1, 1, 1), (1, 64, 128), (1, 1000, 77), (2, 515, 24), (8, 256, 513), (9, 64, 40), (16, 2048, 96),
           (63, 100, 300), (64, 64, 64), (127, 129, 255), (128, 128, 256), (129, 136, 264), (300, 771, 1285),
-          (513, 72, 56), (1025, 512, 130), (2500, 40, 3), (5, 4096, 16), (257, 1037, 9), (700, 520, 1032)]
+          (513, 72, 56), (1025, 512, 130), (2500, 40, 3), (5, 4096, 16), (257, 1037, 9), (700, 520, 1032),
+          # backward products in pieces along a long K: both, aligned; one of them much smaller
+          (4100, 264, 520), (20000, 64, 72)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -364,6 +366,86 @@ def test_two_captured_graphs_replayed_together(m, t):
     for got, ref in zip(outs, refs):
         for a, b in zip(got, ref):
             assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    """Outputs, kept pre-activations and dz of more than 2^31 values: the last rows equal those of a call
+    on them alone (the same sums in the same order), forward and backward."""
+    m, k, n, tail = 530_000, 64, 4104, 1000
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(m, k, generator=g, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(n, k, generator=g, device=DEV) / 8).bfloat16()
+    b = torch.randn(n, generator=g, device=DEV, dtype=torch.bfloat16)
+    y = linear(x, w, b, activation="gelu")
+    dy = torch.empty_like(y).fill_(0.25)
+    dy[-tail:] = torch.randn(tail, n, generator=g, device=DEV, dtype=torch.bfloat16)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    part = x.detach()[-tail:].clone().requires_grad_(True)
+    y2 = linear(part, w, b, activation="gelu")
+    (dx2,) = torch.autograd.grad(y2, part, dy[-tail:])
+    assert torch.equal(y[-tail:], y2)
+    X, W = part.detach().double(), w.double()
+    ref = act64(X @ W.T + b.double(), "gelu")[0]
+    bound = ref.abs() * half(torch.bfloat16) * 1.001 + 1.13 * (k + 2) * U * (X.abs() @ W.abs().T + b.double().abs())
+    within(y2, ref, bound + ref.abs() * 2.0 ** -20 + 2.0 ** -22)
+    # dx's plan may cut K differently for the two sizes: the sums' own bound, on equal dz
+    mag = dy[-tail:].double().abs() * 1.13 @ W.abs()
+    within(dx[-tail:], dx2.double(), dx2.double().abs() * 2 * half(torch.bfloat16) + 2 * (n + 2) * U * mag)
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+def test_first_call_of_a_process_is_captured(t):
+    """Nothing that a first call sets up is refused by a capturing stream (a process of its own)."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = f"""
+import torch
+from dynaworld_b200.linear import linear, linear_fp8
+from dynaworld_b200.norm import quantize_rows_fp8, rms_norm
+t = torch.{t}
+g = torch.Generator(device="cuda").manual_seed(0)
+x = torch.randn(5000, 512, generator=g, device="cuda").to(t).requires_grad_(True)
+w = (torch.randn(320, 512, generator=g, device="cuda") / 22).to(t).requires_grad_(True)
+n = torch.ones(512, device="cuda", dtype=t)
+
+def step():
+    y = rms_norm(x, n)
+    z = linear(y, w, activation="gelu")
+    a, b = quantize_rows_fp8(y.detach()), quantize_rows_fp8(w.detach())
+    return [z.detach(), *torch.autograd.grad(z.float().sum(), [x, w]), linear_fp8(*a, *b, dtype=t),
+            linear(x[:3].detach(), w.detach())]
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, step()))
+print("equal")
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=240)
+    assert run.returncode == 0 and "equal" in run.stdout, run.stderr[-2000:]
+
+
+def test_backward_captured_beside_a_live_eager_graph():
+    """Capturing .backward() while an eager graph of the same leaf lives: torch refuses it with an
+    exception (the leaf's accumulation belongs to the eager stream), the process and the eager graph
+    live on; without the eager graph it is captured."""
+    x, w, b, r, dy = make(40, 64, 48, torch.float32)
+    leaf = w.clone().requires_grad_(True)
+    eager = linear(x, leaf).sum()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(graph):
+            linear(2 * x, leaf).sum().backward()
+    torch.cuda.synchronize()
+    leaf.grad = None
+    eager.backward()
+    ref = leaf.grad.clone()
+    within(ref, torch.ones_like(dy).double().T @ x.double(), 42 * U * x.double().abs().sum(0).expand(48, 64))
 
 
 def test_no_wait_gave_up():

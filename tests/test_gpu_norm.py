@@ -276,6 +276,28 @@ def test_other_stream_and_captured_graph():
     assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1) and torch.equal(h1, h2)
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values: the last rows equal those of a call on them alone."""
+    rows, dim, tail = 1_060_000, 2048, 500
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(rows, dim, generator=g, device=DEV, dtype=torch.bfloat16)
+    w = torch.randn(dim, generator=g, device=DEV, dtype=torch.bfloat16)
+    leaf = x.requires_grad_(True)
+    y, h = rms_norm(leaf, w, residual=x.detach())
+    dy = torch.full_like(y, 0.5)
+    (dx,) = torch.autograd.grad([y, h], leaf, [dy, dy])
+    part = x.detach()[-tail:].clone().requires_grad_(True)
+    y2, h2 = rms_norm(part, w, residual=part.detach())
+    (dx2,) = torch.autograd.grad([y2, h2], part, [dy[-tail:], dy[-tail:]])
+    bound = 2 * half(torch.bfloat16) + 300 * U  # one rounding either side; the sums' orders may differ
+    for a, b in ((y, y2), (h, h2), (dx, dx2)):
+        within(a[-tail:].detach(), b.detach().double(), b.detach().double().abs() * bound + 1e-5)
+    del dx, dy, y, h
+    q, s = quantize_rows_fp8(x.detach())
+    q2, s2 = quantize_rows_fp8(part.detach())
+    assert torch.equal(q[-tail:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[-tail:], s2)
+
+
 def test_refusals_on_the_gpu():
     x = torch.zeros(2, 8, device=DEV, requires_grad=True)
     w = torch.ones(8, device=DEV)

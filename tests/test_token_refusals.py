@@ -47,6 +47,8 @@ F = torch.zeros
     (RuntimeError, "CUDA devices only", lambda: rms_norm_fp8(F(2, 4), F(4))),
     (ValueError, "at least one element", lambda: quantize_rows_fp8(F(2, 0))),
     (RuntimeError, "CUDA devices only", lambda: quantize_rows_fp8(F(2, 4))),
+    (ValueError, "values are too long", lambda: quantize_rows_fp8(F(1).expand(1, (1 << 24) + 1))),
+    (ValueError, "larger than 2\\^24", lambda: linear(F(2, 1), F(1, 1).expand((1 << 24) + 1, 1))),
 ])
 def test_refused(error, match, call):
     with pytest.raises(error, match=match):
@@ -74,7 +76,7 @@ def test_entry_points_refuse_before_a_launch(lib):
     assert lib.gsb_quantize_rows_fp8(b, None, 256, None) == 7
     assert lib.gsb_rms_norm_bwd(b, 256, 256, 8, None, 0, 256, None, 256, 16, None) == 2
     assert lib.gsb_rms_norm_bwd(b, None, 256, 8, None, 0, 256, None, 256, 1 << 20, None) == 7
-    for field, bad, status in (("dim", 0, 1), ("rows", -1, 1), ("rows", 1 << 31, 1), ("dtype", _lib.E4M3, 7),
+    for field, bad, status in (("dim", 0, 1), ("dim", (1 << 24) + 1, 1), ("rows", -1, 1), ("rows", 1 << 31, 1), ("dtype", _lib.E4M3, 7),
                                ("eps", -1.0, 7), ("weight", None, 7), ("x", None, 7)):
         keep = getattr(n, field)
         setattr(n, field, bad)
