@@ -7,7 +7,8 @@ namespace gsb {
 
 namespace {
 
-constexpr int64_t kFewRows = 8;
+constexpr int64_t kFewRows = 8;  // float or unaligned rows: up to these without the tensor cores
+constexpr int64_t kFewMma = 1;  // rows from which the warp-wide MMA pays (2,048 x 8,192 e4m3, 2 rows: 6.0 us, 8.4 without)
 
 // ---- few rows: bound by the weights' bytes ----------------------------------------------------
 // A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
@@ -518,6 +519,7 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   const int b = elem_bytes(p->out_dtype);
   e.vec = e.vec && vec_ok(p->bias, 0, b, 16) && vec_ok(preact, 0, b, 16) &&
           (!p->residual || vec_ok(p->residual, p->residual_stride, b, 16));
+  if (p->m > kFewMma && few_rows_mma(*p, e, st)) return launch_status();
   if (p->m <= kFewRows) {
     switch (p->dtype) {
       case GSB_F32: few_rows<float, float>(*p, e, st); break;

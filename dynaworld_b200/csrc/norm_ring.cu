@@ -318,7 +318,7 @@ bool fwd_of(const NormArgs& a, cudaStream_t st) {
   };
   if (nv <= 64) return go(ring_fwd_kernel<T, 2, 32, 512, MODE>, 16, 512);
   if (nv <= 128) return go(ring_fwd_kernel<T, 4, 32, 512, MODE>, 16, 512);
-  if (nv <= 256) return go(ring_fwd_kernel<T, 8, 32, 256, MODE>, 8, 256);
+  if (nv <= 256) return go(ring_fwd_kernel<T, 8, 32, 384, MODE>, 12, 384);
   if (nv <= 512) return go(ring_fwd_kernel<T, 2, 256, 256, MODE>, 1, 256);
   if (nv <= 1024) return go(ring_fwd_kernel<T, 4, 256, 256, MODE>, 1, 256);
   return go(ring_fwd_kernel<T, 8, 256, 256, MODE>, 1, 256);
