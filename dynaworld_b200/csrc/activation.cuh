@@ -105,10 +105,11 @@ __device__ __forceinline__ F2 act_slope(F2 z) {
   } else if constexpr (ACT == GSB_ACT_GELU) {
     F2 minus, gauss;
     const F2 tail = normal_tail(z, minus, gauss);
-    float z0, z1, t0, t1;
+    // Phi(z) = 1/2 + (1/2 - Phi(-|z|)) with the sign of z
+    float z0, z1, h0, h1;
     z.get(z0, z1);
-    tail.get(t0, t1);
-    const F2 cdf(z0 < 0.0f ? t0 : 1.0f - t0, z1 < 0.0f ? t1 : 1.0f - t1);
+    fma2(tail, F2(-1.0f), F2(0.5f)).get(h0, h1);
+    const F2 cdf = add2(F2(copysignf(h0, z0), copysignf(h1, z1)), F2(0.5f));
     return fma2(mul2(z, F2(kInvSqrt2Pi)), gauss, cdf);
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
     const F2 zz = mul2(z, z);

@@ -242,25 +242,18 @@ __device__ __forceinline__ void activate(const Job& p, float (&z)[V]) {
   else apply_value<ACT, V>(z);
 }
 
-template <typename O, int ACT>
+// VEC: the output's rows (and the residual's, bias, kept sums) allow accesses of 16 bytes.
+// SCALED: e4m3 operands with their rows' scales.
+template <typename O, int ACT, bool VEC, bool SCALED>
 struct Rows {
   static constexpr int V = 16 / int(sizeof(O));
   static constexpr int kPerRow = 32 / V;
   static constexpr int kAtOnce = 32 / kPerRow;  // rows in one access of the warp
   static constexpr int kSteps = 32 / kAtOnce;
   using Z = typename PreactOf<O>::type;
-  // What a block's epilogue reads from global memory.  Aligned: kSteps x 16 bytes of the residual and V
-  // values of the bias; else a column per lane: its 32 rows of the residual, one value of the bias.
-  struct Ahead {
-    union {
-      uint4 res[kSteps];
-      O col[32];
-    };
-    union {
-      uint4 bias;
-      O bias1;
-    };
-    __device__ __forceinline__ Ahead() {}
+  struct Ahead {  // what the next block reads, of aligned rows
+    uint4 res[kSteps];
+    uint4 bias;
   };
   int row0, col;  // this lane's first row and column within the block
   int steps;      // its rows inside the matrix
@@ -275,26 +268,14 @@ struct Rows {
     col = (lane % kPerRow) * V;
     i = i0 + row0;
     steps = int(max(int64_t(0), min(int64_t(kSteps), (p.m - i + kAtOnce - 1) / kAtOnce)));
-    if (p.e.row_scale) {
+    if (SCALED && p.e.row_scale) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) rs[s] = s < steps ? p.e.row_scale[i + s * kAtOnce] : 0.0f;
     }
   }
 
   __device__ __forceinline__ void prefetch(const Job& p, int64_t j0, Ahead& a) const {
-    if (!p.e.vec) {
-      const int64_t j = j0 + (threadIdx.x & 31);
-      if (j >= p.n) return;
-      if (p.e.bias) a.bias1 = static_cast<const O*>(p.e.bias)[j];
-      if (p.e.res) {
-        const int64_t i0 = i - row0;
-        const O* r = static_cast<const O*>(p.e.res) + i0 * p.e.res_stride + j;
-#pragma unroll
-        for (int q = 0; q < 32; ++q)
-          if (i0 + q < p.m) a.col[q] = r[q * p.e.res_stride];
-      }
-      return;
-    }
+    if constexpr (!VEC) return;
     const int64_t j = j0 + col;
     const bool in = j < p.n;
     if (p.e.bias && in) a.bias = __ldg(reinterpret_cast<const uint4*>(static_cast<const O*>(p.e.bias) + j));
@@ -319,7 +300,7 @@ struct Rows {
   // ... and from there to the output.
   __device__ __forceinline__ void emit(const Job& p, const float* stage, int64_t i0, int64_t j0, const Ahead& a) const {
     const int lane = threadIdx.x & 31;
-    if (p.e.vec) {
+    if constexpr (VEC) {
       const int64_t j = j0 + col;
       if (j < p.n) {
         float bias[V], cs[V];
@@ -328,7 +309,7 @@ struct Rows {
 #pragma unroll
           for (int u = 0; u < V; ++u) bias[u] = to_f32(b.v[u]);
         }
-        if (p.e.row_scale) {
+        if (SCALED && p.e.row_scale) {
 #pragma unroll
           for (int u = 0; u < V; ++u) cs[u] = p.e.col_scale[j + u];
         }
@@ -347,7 +328,7 @@ struct Rows {
               float* to = z + h * V + v;
               to[0] = q.x, to[1] = q.y, to[2] = q.z, to[3] = q.w;
             }
-          if (p.e.row_scale) {
+          if (SCALED && p.e.row_scale) {
 #pragma unroll
             for (int v = 0; v < 2 * V; ++v) z[v] *= rs[s0 + v / V] * cs[v % V];
           }
@@ -378,11 +359,18 @@ struct Rows {
         }
       }
     } else {
-      // rows that start anywhere: a lane per column
+      // rows that start anywhere: a lane per column, the residual's 32 rows asked for at once
       const int64_t j = j0 + lane;
       if (j < p.n) {
-        const float b = p.e.bias ? to_f32(a.bias1) : 0.0f;
-        const float cs = p.e.row_scale ? p.e.col_scale[j] : 1.0f;
+        O add[32];
+        if (p.e.res) {
+          const O* r = static_cast<const O*>(p.e.res) + i0 * p.e.res_stride + j;
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (i0 + q < p.m) add[q] = r[q * p.e.res_stride];
+        }
+        const float b = p.e.bias ? to_f32(static_cast<const O*>(p.e.bias)[j]) : 0.0f;
+        const float cs = SCALED && p.e.row_scale ? p.e.col_scale[j] : 1.0f;
         O* out = static_cast<O*>(p.e.out) + plane + i0 * p.e.out_stride + j;
         Z* keep = static_cast<Z*>(p.e.preact) + i0 * p.n + j;
         const int rows = int(min(int64_t(32), p.m - i0));
@@ -392,7 +380,7 @@ struct Rows {
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             z[r] = stage[stage_at(r0 + r, lane >> 2) + (lane & 3)];
-            if (p.e.row_scale && r0 + r < rows) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
+            if (SCALED && p.e.row_scale && r0 + r < rows) z[r] *= p.e.row_scale[i0 + r0 + r] * cs;
             z[r] += b;
           }
           if (p.e.preact) {
@@ -403,7 +391,7 @@ struct Rows {
           activate<ACT, 8>(p, z);
           if (p.e.res) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) z[r] += to_f32(a.col[r0 + r]);
+            for (int r = 0; r < 8; ++r) z[r] += to_f32(add[r0 + r]);
           }
 #pragma unroll
           for (int r = 0; r < 8; ++r)
@@ -431,7 +419,7 @@ struct Shape {
 };
 
 // KIND 0: 16-bit operands, 1: e4m3.  BWD: up to two products, B MN-major; else one, both K-major.
-template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT>
+template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<1 + BWD> p) {
   using S = Shape<CG, BN, PLANES>;
   constexpr int kElems = KIND == 1 ? 128 : 64;  // k per block
@@ -479,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     bool ok = true;
     int buf = 0;
     uint32_t acc_phase = 0;
-    Rows<O, ACT> rows;
-    typename Rows<O, ACT>::Ahead ahead;
+    Rows<O, ACT, VEC, KIND == 1> rows;
+    typename Rows<O, ACT, VEC, KIND == 1>::Ahead ahead;
     for (int64_t i = 0; p.unit(cluster, clusters, i, which, u); ++i) {
       const Job& job = p.job[which];
       int64_t mt, nt;
@@ -503,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         tmem_start32(acc, v);
 #pragma unroll 1
         for (int c = 0; c < kHalfCols; c += 32) {
-          const typename Rows<O, ACT>::Ahead now = ahead;
+          const typename Rows<O, ACT, VEC, KIND == 1>::Ahead now = ahead;
           if (c + 32 < kHalfCols) rows.prefetch(job, j0 + c + 32, ahead);
           tmem_wait32(v);
           if (!ok) {
@@ -735,10 +723,10 @@ bool make_job(Job& j, CUtensorMap* a, CUtensorMap* b, const Product& p, const Ep
 }
 
 // products[0 .. count): one forward product, or one or two of the backward's.
-template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT>
+template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT, bool VEC>
 gsb_status launch(const Product* products, const Epilogue* e, int count, const int* splits, cudaStream_t st) {
   using S = Shape<CG, BN, PLANES>;
-  auto* kernel = mma_kernel<KIND, CG, BN, BWD, PLANES, O, ACT>;
+  auto* kernel = mma_kernel<KIND, CG, BN, BWD, PLANES, O, ACT, VEC>;
   int dev = 0;
   (void)cudaGetDevice(&dev);
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel has its shared memory
@@ -793,26 +781,35 @@ gsb_status launch(const Product* products, const Epilogue* e, int count, const i
 }
 
 // By tile: 256 is 256 x 256 over a pair of CTAs, 128 and 64 are 128 rows by that many columns on one
-// CTA (fewer of them are worth an instance per activation).
-template <int KIND, int PLANES, typename O>
-gsb_status launch_fwd(const Product& p, const Epilogue& e, int bn, const int* splits, cudaStream_t st) {
-  if (bn == 128) return launch<KIND, 1, 128, false, PLANES, O, kAnyAct>(&p, &e, 1, splits, st);
-  if (bn == 64) return launch<KIND, 1, 64, false, PLANES, O, kAnyAct>(&p, &e, 1, splits, st);
-  switch (e.act) {
-    case GSB_ACT_RELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_RELU>(&p, &e, 1, splits, st);
-    case GSB_ACT_GELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU>(&p, &e, 1, splits, st);
-    case GSB_ACT_GELU_TANH: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU_TANH>(&p, &e, 1, splits, st);
-    case GSB_ACT_SILU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_SILU>(&p, &e, 1, splits, st);
-    default: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_NONE>(&p, &e, 1, splits, st);
-  }
+// CTA.
+template <int KIND, bool BWD, int PLANES, typename O, int ACT, bool VEC>
+gsb_status launch_tile(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st) {
+  if (bn == 128) return launch<KIND, 1, 128, BWD, PLANES, O, ACT, VEC>(p, e, count, splits, st);
+  if (bn == 64) return launch<KIND, 1, 64, BWD, PLANES, O, ACT, VEC>(p, e, count, splits, st);
+  return launch<KIND, 2, 256, BWD, PLANES, O, ACT, VEC>(p, e, count, splits, st);
 }
 
 // One product without an epilogue (BWD: one or two).
 template <int KIND, bool BWD, int PLANES, typename O>
 gsb_status launch_plain(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st) {
-  if (bn == 128) return launch<KIND, 1, 128, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
-  if (bn == 64) return launch<KIND, 1, 64, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
-  return launch<KIND, 2, 256, BWD, PLANES, O, GSB_ACT_NONE>(p, e, count, splits, st);
+  if (e[0].vec && e[count - 1].vec)
+    return launch_tile<KIND, BWD, PLANES, O, GSB_ACT_NONE, true>(p, e, count, bn, splits, st);
+  return launch_tile<KIND, BWD, PLANES, O, GSB_ACT_NONE, false>(p, e, count, bn, splits, st);
+}
+
+// The forward.  Large aligned outputs have an instance per activation, the others choose at run time.
+template <int KIND, int PLANES, typename O>
+gsb_status launch_fwd(const Product& p, const Epilogue& e, int bn, const int* splits, cudaStream_t st) {
+  if (!e.vec) return launch_tile<KIND, false, PLANES, O, kAnyAct, false>(&p, &e, 1, bn, splits, st);
+  if (bn == 128) return launch<KIND, 1, 128, false, PLANES, O, kAnyAct, true>(&p, &e, 1, splits, st);
+  if (bn == 64) return launch<KIND, 1, 64, false, PLANES, O, kAnyAct, true>(&p, &e, 1, splits, st);
+  switch (e.act) {
+    case GSB_ACT_RELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_RELU, true>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU, true>(&p, &e, 1, splits, st);
+    case GSB_ACT_GELU_TANH: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_GELU_TANH, true>(&p, &e, 1, splits, st);
+    case GSB_ACT_SILU: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_SILU, true>(&p, &e, 1, splits, st);
+    default: return launch<KIND, 2, 256, false, PLANES, O, GSB_ACT_NONE, true>(&p, &e, 1, splits, st);
+  }
 }
 
 }  // namespace mma

@@ -6,9 +6,8 @@ namespace gsb {
 gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int, int bn, const int* splits, cudaStream_t st) {
   switch (p->out_dtype) {
     case GSB_F32:  // the last layers' raw outputs, and sums: not worth an instance per activation
-      if (bn == 128) return mma::launch<1, 1, 128, false, 1, float, mma::kAnyAct>(p, e, 1, splits, st);
-      if (bn == 64) return mma::launch<1, 1, 64, false, 1, float, mma::kAnyAct>(p, e, 1, splits, st);
-      return mma::launch<1, 2, 256, false, 1, float, mma::kAnyAct>(p, e, 1, splits, st);
+      if (e->vec) return mma::launch_tile<1, false, 1, float, mma::kAnyAct, true>(p, e, 1, bn, splits, st);
+      return mma::launch_tile<1, false, 1, float, mma::kAnyAct, false>(p, e, 1, bn, splits, st);
     case GSB_BF16: return mma::launch_fwd<1, 1, bf16>(*p, *e, bn, splits, st);
     default: return mma::launch_fwd<1, 1, f16>(*p, *e, bn, splits, st);
   }
