@@ -24,6 +24,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "async_copy.cuh"
 #include "linear_parts.cuh"
@@ -215,7 +216,7 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn) {
 
 // Descriptor advance per MMA (16 k of 16-bit, 32 of 8-bit values): 32 bytes along a K-major row,
 // two 8-k groups MN-major; in units of 16 bytes.
-__device__ __forceinline__ uint32_t desc_step(bool mn) { return mn ? 2048 / 16 : 32 / 16; }
+__host__ __device__ constexpr uint32_t desc_step(bool mn) { return mn ? 2048 / 16 : 32 / 16; }
 
 __device__ __forceinline__ void tile_of(const Job& p, int64_t t, int64_t& mt, int64_t& nt) {
   const int64_t per = int64_t(p.group) * p.n_tiles;
@@ -423,6 +424,7 @@ template <int KIND, int CG, int BN, bool BWD, int PLANES, typename O, int ACT, b
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<1 + BWD> p) {
   using S = Shape<CG, BN, PLANES>;
   constexpr int kElems = KIND == 1 ? 128 : 64;  // k per block
+  constexpr int JOBS = 1 + BWD;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   uint8_t* smem = raw + (base - smem_addr(raw));
@@ -551,38 +553,41 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         uint32_t phase = 0;
         for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
           const Job& job = p.job[which];
-          const CUtensorMap* map_a = &p.a[which];
-          const CUtensorMap* map_b = &p.b[which];
-          const bool a_mn = BWD && job.a_mn;
+          const CUtensorMap* map_a = which ? &p.a[JOBS - 1] : &p.a[0];
+          const CUtensorMap* map_b = which ? &p.b[JOBS - 1] : &p.b[0];
           int64_t mt, nt;
           tile_of(job, u / job.splits, mt, nt);
           const int i0 = int((mt * CG + rank) * 128);
           const int j0 = int(nt * BN + rank * S::kBRows);
           const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
-          for (int kb = kb0; ok && kb < kb1; ++kb) {
-            const int k0 = kb * kElems;
+          const auto walk = [&](auto mn) {
+            for (int kb = kb0; ok && kb < kb1; ++kb) {
+              const int k0 = kb * kElems;
 #pragma unroll
-            for (int q = 0; q < PLANES; ++q) {
-              const int plane = PLANES == 1 ? 0 : (q == 0 ? 2 : q - 1);  // parts 3, 1, 2
-              if (!(ok = bar_wait(empty(s), phase ^ 1, p.gave_up))) break;
-              const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
-              if (rank == 0) bar_expect(full(s), CG * S::kSlot);
-              const uint32_t a = base + s * S::kSlot, b = a + kABytes;
-              if (a_mn) {
+              for (int q = 0; q < PLANES; ++q) {
+                const int plane = PLANES == 1 ? 0 : (q == 0 ? 2 : q - 1);  // parts 3, 1, 2
+                if (!(ok = bar_wait(empty(s), phase ^ 1, p.gave_up))) break;
+                const uint32_t bar = CG == 1 ? full(s) : map_to_rank(full(s), 0);
+                if (rank == 0) bar_expect(full(s), CG * S::kSlot);
+                const uint32_t a = base + s * S::kSlot, b = a + kABytes;
+                if constexpr (decltype(mn)::value) {
 #pragma unroll
-                for (int v = 0; v < 2; ++v) tma_load<CG>(a + v * 8192, map_a, i0 + 64 * v, k0, plane, bar);
-              } else {
-                tma_load<CG>(a, map_a, k0, i0, plane, bar);
+                  for (int v = 0; v < 2; ++v) tma_load<CG>(a + v * 8192, map_a, i0 + 64 * v, k0, plane, bar);
+                } else {
+                  tma_load<CG>(a, map_a, k0, i0, plane, bar);
+                }
+                if constexpr (BWD) {
+#pragma unroll
+                  for (int v = 0; v < S::kBRows / 64; ++v) tma_load<CG>(b + v * 8192, map_b, j0 + 64 * v, k0, plane, bar);
+                } else {
+                  tma_load<CG>(b, map_b, k0, j0, plane, bar);
+                }
+                if (++s == S::kSlots) s = 0, phase ^= 1;
               }
-              if constexpr (BWD) {
-#pragma unroll
-                for (int v = 0; v < S::kBRows / 64; ++v) tma_load<CG>(b + v * 8192, map_b, j0 + 64 * v, k0, plane, bar);
-              } else {
-                tma_load<CG>(b, map_b, k0, j0, plane, bar);
-              }
-              if (++s == S::kSlots) s = 0, phase ^= 1;
             }
-          }
+          };
+          if (BWD && job.a_mn) walk(std::true_type{});
+          else walk(std::false_type{});
         }
         // every slot released: no arrival of a commit comes after the CTA's end
         for (int q = 0; ok && q < S::kSlots; ++q) {
@@ -599,61 +604,66 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         const auto next = [&](int x) { return x + 1 == S::kSlots ? 0 : x + 1; };
         for (int64_t i = 0; ok && p.unit(cluster, clusters, i, which, u); ++i) {
           const Job& job = p.job[which];
-          const bool a_mn = BWD && job.a_mn;
-          const uint32_t idesc = job.idesc, a_step = desc_step(a_mn), b_step = desc_step(BWD);
+          const uint32_t idesc = job.idesc;
           const int kb0 = int(u % job.splits) * job.per_split, kb1 = min(job.k_blocks, kb0 + job.per_split);
-          for (int kb = kb0; ok && kb < kb1;) {
-            if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
-            fence_after();
-            const uint32_t acc = tmem + buf * S::kAccCols;
-            const int stop = PLANES == 1 ? kb1 : kb + 1;
-            uint32_t more = 0;
-            for (; kb < stop; ++kb) {
-              if constexpr (PLANES == 1) {
-                if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
-                fence_after();
-                const uint64_t a = smem_desc(base + s * S::kSlot, a_mn);
-                const uint64_t b = smem_desc(base + s * S::kSlot + kABytes, BWD);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                  mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
-                  more = 1;
-                }
-                mma_commit<CG>(empty(s));
-                if (++s == S::kSlots) s = 0, phase ^= 1;
-              } else {
-                const int s3 = s, s1 = next(s3), s2 = next(s1);
-                const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
-                const auto da = [&](int q) { return smem_desc(base + q * S::kSlot, a_mn); };
-                const auto db = [&](int q) { return smem_desc(base + q * S::kSlot + kABytes, BWD); };
-                const auto run = [&](uint64_t a, uint64_t b) {
+          const auto walk = [&](auto mn) {
+            constexpr bool a_mn = decltype(mn)::value;
+            constexpr uint32_t a_step = desc_step(a_mn), b_step = desc_step(BWD);
+            for (int kb = kb0; ok && kb < kb1;) {
+              if (!(ok = bar_wait(acc_empty(buf), acc_phase ^ 1, p.gave_up))) break;
+              fence_after();
+              const uint32_t acc = tmem + buf * S::kAccCols;
+              const int stop = PLANES == 1 ? kb1 : kb + 1;
+              uint32_t more = 0;
+              for (; kb < stop; ++kb) {
+                if constexpr (PLANES == 1) {
+                  if (!(ok = bar_wait(full(s), phase, p.gave_up))) break;
+                  fence_after();
+                  const uint64_t a = smem_desc(base + s * S::kSlot, a_mn);
+                  const uint64_t b = smem_desc(base + s * S::kSlot + kABytes, BWD);
 #pragma unroll
                   for (int v = 0; v < 4; ++v) {
                     mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
                     more = 1;
                   }
-                };
-                if (!(ok = bar_wait(full(s3), phase, p.gave_up) && bar_wait(full(s1), ph1, p.gave_up))) break;
-                fence_after();
-                run(da(s3), db(s1));
-                run(da(s1), db(s3));
-                mma_commit<CG>(empty(s3));
-                if (!(ok = bar_wait(full(s2), ph2, p.gave_up))) break;
-                fence_after();
-                run(da(s2), db(s2));
-                run(da(s1), db(s2));
-                run(da(s2), db(s1));
-                mma_commit<CG>(empty(s2));
-                run(da(s1), db(s1));
-                mma_commit<CG>(empty(s1));
-                s = next(s2);
-                phase = ph2 ^ (s < s2);
+                  mma_commit<CG>(empty(s));
+                  if (++s == S::kSlots) s = 0, phase ^= 1;
+                } else {
+                  const int s3 = s, s1 = next(s3), s2 = next(s1);
+                  const uint32_t ph1 = phase ^ (s1 < s3), ph2 = ph1 ^ (s2 < s1);
+                  const auto da = [&](int q) { return smem_desc(base + q * S::kSlot, a_mn); };
+                  const auto db = [&](int q) { return smem_desc(base + q * S::kSlot + kABytes, BWD); };
+                  const auto run = [&](uint64_t a, uint64_t b) {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                      mma_issue<KIND, CG>(acc, a + v * a_step, b + v * b_step, idesc, more);
+                      more = 1;
+                    }
+                  };
+                  if (!(ok = bar_wait(full(s3), phase, p.gave_up) && bar_wait(full(s1), ph1, p.gave_up))) break;
+                  fence_after();
+                  run(da(s3), db(s1));
+                  run(da(s1), db(s3));
+                  mma_commit<CG>(empty(s3));
+                  if (!(ok = bar_wait(full(s2), ph2, p.gave_up))) break;
+                  fence_after();
+                  run(da(s2), db(s2));
+                  run(da(s1), db(s2));
+                  run(da(s2), db(s1));
+                  mma_commit<CG>(empty(s2));
+                  run(da(s1), db(s1));
+                  mma_commit<CG>(empty(s1));
+                  s = next(s2);
+                  phase = ph2 ^ (s < s2);
+                }
               }
+              mma_commit<CG>(acc_full(buf));
+              buf ^= 1;
+              if (buf == 0) acc_phase ^= 1;
             }
-            mma_commit<CG>(acc_full(buf));
-            buf ^= 1;
-            if (buf == 0) acc_phase ^= 1;
-          }
+          };
+          if (BWD && job.a_mn) walk(std::true_type{});
+          else walk(std::false_type{});
         }
       }
     }
