@@ -30,7 +30,7 @@ __device__ __forceinline__ float fast_rcp(float x) {
 // Two floats in one register pair: the FMA pipe takes both in one instruction (sm_100).
 struct F2 {
   unsigned long long v;
-  __device__ __forceinline__ F2() = default;
+  F2() = default;
   __device__ __forceinline__ explicit F2(float both) : F2(both, both) {}
   __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
   __device__ __forceinline__ void get(float& lo, float& hi) const {
@@ -129,12 +129,13 @@ __device__ __forceinline__ F2 act_slope(F2 z) {
 // V values at once.
 template <int ACT, int V>
 __device__ __forceinline__ void apply_value(float (&z)[V]) {
-  if constexpr (ACT == GSB_ACT_NONE) return;
+  if constexpr (ACT != GSB_ACT_NONE) {
 #pragma unroll
-  for (int u = 0; u < V; u += 2) {
-    float unused;
-    if (u + 1 < V) act_value<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
-    else act_value<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
+    for (int u = 0; u < V; u += 2) {
+      float unused;
+      if (u + 1 < V) act_value<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
+      else act_value<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
+    }
   }
 }
 template <int ACT, int V>

@@ -10,8 +10,9 @@ namespace {
 constexpr int64_t kFewRows = 8;  // float or unaligned rows: up to these without the tensor cores
 constexpr int64_t kFewMma = 1;  // rows from which the warp-wide MMA pays (2,048 x 8,192 e4m3, 2 rows: 6.0 us, 8.4 without)
 
-// ---- few rows: bound by the weights' bytes ----------------------------------------------------
-// A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
+// ---- one row; float or unaligned rows up to kFewRows -------------------------------------------
+// Bound by the weights' bytes (1,024 x 4,096 bf16: 3.3 us, a launch and the way to HBM and back being
+// 2.5 of them).  A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
 // that the weights are read once; the tokens come from L1.  Float operands stay float.
 template <typename T, typename O, int V, int ROWS, int C>
 __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, int m,
@@ -63,9 +64,11 @@ void few_rows_v(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
     note_launch();
   };
   if (p.m == 1) return run(few_rows_kernel<T, O, V, 1, 2>, 2);
-  if (p.m == 2) return run(few_rows_kernel<T, O, V, 2, 2>, 2);
-  if (p.m <= 4) return run(few_rows_kernel<T, O, V, 4, 4>, 4);
-  return run(few_rows_kernel<T, O, V, 8, 4>, 4);
+  if constexpr (V == 1 || sizeof(T) == 4) {  // more aligned rows of the other types: linear_few.cu
+    if (p.m == 2) return run(few_rows_kernel<T, O, V, 2, 2>, 2);
+    if (p.m <= 4) return run(few_rows_kernel<T, O, V, 4, 4>, 4);
+    run(few_rows_kernel<T, O, V, 8, 4>, 4);
+  }
 }
 
 template <typename T, typename O>

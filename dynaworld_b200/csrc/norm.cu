@@ -7,11 +7,12 @@
 //   e4m3: top = max(max |y|, 1e-30), scale = top / 448, code = e4m3(y (448 / top))
 //
 // All of it is bound by HBM: a row is read once, kept in registers as float, reduced, and written.
-// A row belongs to one warp while 32 lanes x 4 accesses of 16 bytes hold it (1,024 16-bit values:
-// no barrier between rows, the loads of eight rows of a block overlap), to a block of 256 threads
-// above that, and above what 256 threads hold in registers it is walked twice (the second walk
-// finds it in L2).  Blocks walk rows with a grid stride so that the weight, and in the backward the
-// weight gradient's partial sums, stay in registers over all rows of a block.
+// Many rows of up to 256 16-byte accesses go through norm_ring.cu.  Here: few rows, rows that start
+// anywhere (one value per access) and wider ones.  A row belongs to one warp while 32 lanes x 4
+// accesses hold it, to a block of 256 threads above that, and above what those hold in registers it is
+// walked twice (the second walk finds it in L2).  Blocks walk rows with a grid stride so that the
+// weight, and in the backward the weight gradient's partial sums, stay in registers over all rows of a
+// block.  8,192 x 2,048 floats quantised: 13.2 us (6.4 TB/s); one row of 1,024: 3 us, a launch.
 #include "norm_parts.cuh"
 
 #include <type_traits>

@@ -2,9 +2,10 @@
 // asynchronous copies (cp.async.bulk of whole rows, one barrier per slot).
 //
 // The kernels of norm.cu load a row, wait, reduce, store; with 92 registers a thread only 16 warps
-// fit an SM and their loads pause while they reduce (norm of 16,384 x 1,024 bf16 values with a
-// residual: 32.5 us, 4.1 TB/s; e4m3 norm of 65,536 x 2,048: 234 us, 4.0 TB/s).  Here up to 200 KB of
-// rows are on their way to each SM whatever the warps do.
+// fit an SM and their loads pause while they reduce.  Here a warp owns a row and up to 200 KB of rows
+// are on their way to each SM whatever the warps do.  Norm of 16,384 x 1,024 bf16 values with a
+// residual: 32.5 -> 20.1 us (6.7 TB/s), its backward 37 -> 34 us though it reads a fifth more
+// (4.9 TB/s); e4m3 norm of 65,536 x 2,048: 234 -> 146 us (6.4 TB/s).
 #include "async_copy.cuh"
 #include "norm_parts.cuh"
 
@@ -18,10 +19,10 @@ constexpr int kBudget = 200 * 1024;  // bytes of row slots per block
 constexpr int kMaxSlots = 6;
 constexpr int kBarBytes = 1024;      // barriers at the front of the shared memory: 16 groups x 6 slots
 
-// A group's walk over its rows.  Slot s holds `streams` rows of `bytes` bytes one after the other.
-template <int GROUP, int THREADS>
+// A warp's walk over its rows.  Slot s holds `streams` rows of `bytes` bytes one after the other.
+template <int THREADS>
 struct Ring {
-  static constexpr int kGroups = THREADS / GROUP;
+  static constexpr int kGroups = THREADS / 32;
   uint32_t bars, data;
   const uint8_t* smem;
   int slots, streams;
@@ -30,7 +31,7 @@ struct Ring {
   bool ok;
 
   __device__ __forceinline__ void init(uint8_t* raw, int slots_, int streams_, uint32_t bytes_, int* flag) {
-    const int g = threadIdx.x / GROUP;
+    const int g = threadIdx.x / 32;
     slots = slots_;
     streams = streams_;
     bytes = bytes_;
@@ -39,7 +40,7 @@ struct Ring {
     bars = smem_addr(raw) + g * kMaxSlots * 8;
     smem = raw + kBarBytes + size_t(g) * slots * streams * bytes;
     data = smem_addr(smem);
-    if (threadIdx.x % GROUP == 0)
+    if (threadIdx.x % 32 == 0)
       for (int s = 0; s < slots; ++s) bar_init(bars + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
@@ -58,10 +59,6 @@ struct Ring {
   __device__ __forceinline__ const Vec<T, V>* row(int s, int q) const {
     return reinterpret_cast<const Vec<T, V>*>(smem + (s * streams + q) * size_t(bytes));
   }
-  __device__ __forceinline__ void all_read() const {
-    if constexpr (GROUP == 32) __syncwarp();
-    else __syncthreads();
-  }
 };
 
 struct RingArgs {
@@ -70,13 +67,13 @@ struct RingArgs {
   int* gave_up;
 };
 
-template <typename T, int PV, int GROUP, int THREADS, int MODE>
+template <typename T, int PV, int THREADS, int MODE>
 __global__ void __launch_bounds__(THREADS, 1) ring_fwd_kernel(const __grid_constant__ RingArgs ra) {
   constexpr int V = 16 / sizeof(T);
   const NormArgs& a = ra.a;
-  __shared__ float red[THREADS / 32];
   extern __shared__ __align__(128) uint8_t raw[];
-  using R = Ring<GROUP, THREADS>;
+  using R = Ring<THREADS>;
+  constexpr int GROUP = 32;
   const int t = threadIdx.x % GROUP, g = threadIdx.x / GROUP;
   const int nv = a.dim / V;
   const bool has_res = MODE != kQuantize && a.res;
@@ -123,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_fwd_kernel(const __grid_const
         for (int e = 0; e < V; ++e) h[j][e] = 0.0f;
       }
     }
-    ring.all_read();
+    __syncwarp();  // every lane has read the slot
     if (t == 0 && ring.ok && row + ra.slots * step < a.rows) fetch(row + ra.slots * step, s);
     if (++s == ra.slots) s = 0, parity ^= 1;
     if constexpr (MODE != kQuantize) {
@@ -137,7 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_fwd_kernel(const __grid_const
       for (int j = 0; j < PV; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) ss = fmaf(h[j][e], h[j][e], ss);
-      ss = group_sum<GROUP>(ss, red);
+      ss = warp_sum(ss);
       const float rstd = 1.0f / sqrtf(ss * a.inv_dim + a.eps);
       if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
@@ -158,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_fwd_kernel(const __grid_const
 #pragma unroll
           for (int e = 0; e < V; ++e) top = max(top, abs_bits(h[j][e]));
         }
-      top = group_max<GROUP>(top, red);
+      top = __reduce_max_sync(0xffffffffu, top);
       const float most = __uint_as_float(top);
       const float inv = kE4M3Max / most;
       if (t == 0) a.scale[row] = most / kE4M3Max;
@@ -172,13 +169,13 @@ __global__ void __launch_bounds__(THREADS, 1) ring_fwd_kernel(const __grid_const
   if (!ring.ok) let_copies_land();
 }
 
-template <typename T, int PV, int GROUP, int THREADS>
+template <typename T, int PV, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) ring_bwd_kernel(const __grid_constant__ RingArgs ra) {
   constexpr int V = 16 / sizeof(T);
   const NormArgs& a = ra.a;
-  __shared__ float red[THREADS / 32];
   extern __shared__ __align__(128) uint8_t raw[];
-  using R = Ring<GROUP, THREADS>;
+  using R = Ring<THREADS>;
+  constexpr int GROUP = 32;
   const int t = threadIdx.x % GROUP, g = threadIdx.x / GROUP;
   const int nv = a.dim / V;
   const int q_res = 2, q_ds = a.res ? 3 : 2;
@@ -229,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_bwd_kernel(const __grid_const
         }
       }
     }
-    ring.all_read();
+    __syncwarp();  // every lane has read the slot
     if (t == 0 && ring.ok && row + ra.slots * step < a.rows) fetch(row + ra.slots * step, s);
     if (++s == ra.slots) s = 0, parity ^= 1;
     float dot = 0.0f;
@@ -243,7 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_bwd_kernel(const __grid_const
           acc[j][e] = fmaf(gh, rstd, acc[j][e]);
         }
       }
-    dot = group_sum<GROUP>(dot, red);
+    dot = warp_sum(dot);
     const float c = rstd * rstd * (dot * a.inv_dim);
 #pragma unroll
     for (int j = 0; j < PV; ++j) {
@@ -262,14 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) ring_bwd_kernel(const __grid_const
   if (!ring.ok) let_copies_land();
   // the block's column sums, its groups added in order; the slots are free once every row is read
   float* part = a.dw_part + int64_t(blockIdx.x) * a.dim;
-  if constexpr (R::kGroups == 1) {
-#pragma unroll
-    for (int j = 0; j < PV; ++j)
-      if (j * GROUP + t < nv) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) part[(j * GROUP + t) * V + e] = acc[j][e];
-      }
-  } else {
+  {
     __syncthreads();
     float* s_dw = reinterpret_cast<float*>(raw + kBarBytes);
 #pragma unroll
@@ -316,12 +306,9 @@ bool fwd_of(const NormArgs& a, cudaStream_t st) {
     const int64_t blocks = std::min<int64_t>(sm_count(), (a.rows + groups - 1) / groups);
     return slots >= 2 && start(kernel, a, groups, threads, streams, E, slots, int(blocks), st);
   };
-  if (nv <= 64) return go(ring_fwd_kernel<T, 2, 32, 512, MODE>, 16, 512);
-  if (nv <= 128) return go(ring_fwd_kernel<T, 4, 32, 512, MODE>, 16, 512);
-  if (nv <= 256) return go(ring_fwd_kernel<T, 8, 32, 384, MODE>, 12, 384);
-  if (nv <= 512) return go(ring_fwd_kernel<T, 2, 256, 256, MODE>, 1, 256);
-  if (nv <= 1024) return go(ring_fwd_kernel<T, 4, 256, 256, MODE>, 1, 256);
-  return go(ring_fwd_kernel<T, 8, 256, 256, MODE>, 1, 256);
+  if (nv <= 64) return go(ring_fwd_kernel<T, 2, 512, MODE>, 16, 512);
+  if (nv <= 128) return go(ring_fwd_kernel<T, 4, 512, MODE>, 16, 512);
+  return go(ring_fwd_kernel<T, 8, 384, MODE>, 12, 384);  // eight warps with a slot more: 172 us instead of 146
 }
 
 template <typename T>
@@ -334,18 +321,16 @@ bool bwd_of(const NormArgs& a, int* parts, cudaStream_t st) {
     *parts = int(blocks);
     return slots >= 2 && start(kernel, a, groups, 256, streams, E, slots, int(blocks), st);
   };
-  if (nv <= 64) return go(ring_bwd_kernel<T, 2, 32, 256>, 8);
-  if (nv <= 128) return go(ring_bwd_kernel<T, 4, 32, 256>, 8);
-  if (nv <= 256) return go(ring_bwd_kernel<T, 1, 256, 256>, 1);
-  if (nv <= 512) return go(ring_bwd_kernel<T, 2, 256, 256>, 1);
-  return go(ring_bwd_kernel<T, 4, 256, 256>, 1);
+  if (nv <= 64) return go(ring_bwd_kernel<T, 2, 256>, 8);
+  return go(ring_bwd_kernel<T, 4, 256>, 8);
 }
 
-// A ring pays once every group walks a few rows (below that the register kernels' single round is
-// shorter) and a row is worth a copy of its own.
+// A ring pays once every warp walks a few rows (below that the register kernels' single round is
+// shorter), a row is worth a copy of its own and a warp's registers hold it (a block per row, with one
+// ring per SM, took 31 us for the 13 us of norm.cu's blocks: 8,192 x 2,048 floats quantised).
 bool worth_it(const NormArgs& a, int elem, int most_vectors) {
   const int nv = a.dim * elem / 16;
-  return a.dim * elem >= 512 && nv <= most_vectors && a.rows >= int64_t(sm_count()) * (nv <= 256 ? 32 : 4);
+  return a.dim * elem >= 512 && nv <= most_vectors && a.rows >= int64_t(sm_count()) * 32;
 }
 
 }  // namespace
