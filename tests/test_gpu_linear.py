@@ -119,7 +119,9 @@ SHAPES = [(1, 1, 1), (1, 64, 128), (1, 1000, 77), (2, 515, 24), (8, 256, 513), (
           (63, 100, 300), (64, 64, 64), (127, 129, 255), (128, 128, 256), (129, 136, 264), (300, 771, 1285),
           (513, 72, 56), (1025, 512, 130), (2500, 40, 3), (5, 4096, 16), (257, 1037, 9), (700, 520, 1032),
           # backward products in pieces along a long K: both, aligned; one of them much smaller
-          (4100, 264, 520), (20000, 64, 72)]
+          (4100, 264, 520), (20000, 64, 72),
+          # a few aligned rows: one and two blocks of 16, columns past a block of 32, a ragged last step of K
+          (13, 96, 4741), (2, 208, 4800), (24, 128, 520), (31, 2064, 33), (17, 48, 4744)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -323,6 +325,40 @@ def test_refusals_on_the_gpu():
 
 
 # ---- streams and graphs ----
+
+
+def test_calls_at_once_from_threads():
+    """Four threads on streams of their own, forward and backward at the same time: every result is that of
+    the call alone."""
+    import threading
+
+    cases = [make(m, 264, 520, t, seed=m) for m, t in ((700, torch.bfloat16), (20, torch.float16),
+                                                       (600, torch.float32), (1, torch.bfloat16))]
+
+    def step(case):
+        x, w, b, r, dy = case
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        y = linear(leaves[0], leaves[1], leaves[2], activation="gelu_tanh", residual=r)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    refs = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step(cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, refs[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.parametrize("t", TYPES)
