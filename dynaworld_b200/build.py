@@ -54,7 +54,7 @@ def torch_command(out: Path) -> list[str]:
     return [shutil.which("g++") or "g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden", f"-I{INCLUDE}",
             *(a for p in include for a in ("-isystem", p)), str(CSRC / TORCH_SOURCE), "-o", str(out),
             *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-            "-ltorch_python"]
+            "-ltorch_cuda", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:

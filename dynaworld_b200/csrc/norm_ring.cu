@@ -280,14 +280,20 @@ __global__ void __launch_bounds__(THREADS, 1) ring_bwd_kernel(const __grid_const
 
 template <typename K>
 bool start(K kernel, const NormArgs& a, int groups, int threads, int streams, int elem, int slots, int blocks,
-           cudaStream_t st) {
+           std::atomic<uint64_t>& ready, cudaStream_t st) {
   RingArgs ra{a, slots, gave_up_flag()};
   if (!ra.gave_up) return false;
-  const size_t bytes = kBarBytes + size_t(groups) * slots * streams * a.dim * elem;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return false;
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBarBytes + kBudget) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    ready.fetch_or(bit, std::memory_order_relaxed);
   }
+  const size_t bytes = kBarBytes + size_t(groups) * slots * streams * a.dim * elem;
   kernel<<<blocks, threads, bytes, st>>>(ra);
   note_launch();
   return true;
@@ -301,28 +307,31 @@ template <typename T, int MODE>
 bool fwd_of(const NormArgs& a, cudaStream_t st) {
   constexpr int E = sizeof(T), V = 16 / E;
   const int nv = a.dim / V, row = a.dim * E, streams = MODE != kQuantize && a.res ? 2 : 1;
-  const auto go = [&](auto kernel, int groups, int threads) {
+  // per instance: the devices whose copy of the kernel has its shared memory
+  const auto go = [&](auto kernel, int groups, int threads, std::atomic<uint64_t>& ready) {
     const int slots = slots_of(groups, streams, row);
     const int64_t blocks = std::min<int64_t>(sm_count(), (a.rows + groups - 1) / groups);
-    return slots >= 2 && start(kernel, a, groups, threads, streams, E, slots, int(blocks), st);
+    return slots >= 2 && start(kernel, a, groups, threads, streams, E, slots, int(blocks), ready, st);
   };
-  if (nv <= 64) return go(ring_fwd_kernel<T, 2, 512, MODE>, 16, 512);
-  if (nv <= 128) return go(ring_fwd_kernel<T, 4, 512, MODE>, 16, 512);
-  return go(ring_fwd_kernel<T, 8, 384, MODE>, 12, 384);  // eight warps with a slot more: 172 us instead of 146
+  static std::atomic<uint64_t> ready[3];
+  if (nv <= 64) return go(ring_fwd_kernel<T, 2, 512, MODE>, 16, 512, ready[0]);
+  if (nv <= 128) return go(ring_fwd_kernel<T, 4, 512, MODE>, 16, 512, ready[1]);
+  return go(ring_fwd_kernel<T, 8, 384, MODE>, 12, 384, ready[2]);  // eight warps with a slot more: 172 us instead of 146
 }
 
 template <typename T>
 bool bwd_of(const NormArgs& a, int* parts, cudaStream_t st) {
   constexpr int E = sizeof(T), V = 16 / E;
   const int nv = a.dim / V, row = a.dim * E, streams = 2 + (a.res != nullptr) + (a.dsum != nullptr);
-  const auto go = [&](auto kernel, int groups) {
+  const auto go = [&](auto kernel, int groups, std::atomic<uint64_t>& ready) {
     const int slots = slots_of(groups, streams, row);
     const int64_t blocks = std::min<int64_t>(sm_count(), (a.rows + groups - 1) / groups);
     *parts = int(blocks);
-    return slots >= 2 && start(kernel, a, groups, 256, streams, E, slots, int(blocks), st);
+    return slots >= 2 && start(kernel, a, groups, 256, streams, E, slots, int(blocks), ready, st);
   };
-  if (nv <= 64) return go(ring_bwd_kernel<T, 2, 256>, 8);
-  return go(ring_bwd_kernel<T, 4, 256>, 8);
+  static std::atomic<uint64_t> ready[2];
+  if (nv <= 64) return go(ring_bwd_kernel<T, 2, 256>, 8, ready[0]);
+  return go(ring_bwd_kernel<T, 4, 256>, 8, ready[1]);
 }
 
 // A ring pays once every warp walks a few rows (below that the register kernels' single round is

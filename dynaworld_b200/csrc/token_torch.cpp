@@ -6,6 +6,7 @@
 // These operators take microseconds, and one product of a single token spent 3 us on the GPU and
 // 12.5 on the host that way, a norm with its gradients 107, most of it in the Python halves of the
 // autograd engine.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -141,8 +142,10 @@ OptTensor rows_of(const OptTensor& t, int64_t width) {
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* address(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 
+// A new tensor on like's device, past the dispatcher: half the time of at::empty, and a call makes
+// one to three.
 Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
-  return at::empty(shape, like.options().dtype(type));
+  return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
 }
 Tensor workspace(const Tensor& like, size_t bytes) {
   return bytes ? empty(like, {int64_t(bytes)}, at::kByte) : Tensor();
