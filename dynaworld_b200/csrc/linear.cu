@@ -7,12 +7,21 @@ namespace gsb {
 
 namespace {
 
-constexpr int64_t kFewRows = 8;  // float or unaligned rows: up to these without the tensor cores
-constexpr int64_t kFewMma = 1;  // rows from which the warp-wide MMA pays (2,048 x 8,192 e4m3, 2 rows: 6.0 us, 8.4 without)
+// Which kernels serve a forward: the weights walked row by row without the tensor cores (one row; float
+// or unaligned rows, up to 64 while the weights stay in L2 between eight rows and the next), the
+// warp-wide MMA, or tcgen05 tiles.  1,024 x 1,024 float, 16 rows: 6.0 us, 17 on tiles; 64 rows: 12.8.
+enum class Path { kWalk, kFewMma, kTiles };
+Path path_of(const gsb_linear& p) {
+  if (few_rows_mma_serves(p)) return Path::kFewMma;
+  const int b = elem_bytes(p.dtype);
+  const bool aligned = p.dtype != GSB_F32 && p.k % (16 / b) == 0 && vec_ok(p.x, p.x_stride, b, 16) &&
+                       vec_ok(p.weight, p.weight_stride, b, 16);
+  const int64_t most = aligned ? 1 : int64_t(p.n) * p.k * b <= (8 << 20) ? 64 : 8;
+  return p.m <= most ? Path::kWalk : Path::kTiles;
+}
 
-// ---- one row; float or unaligned rows up to kFewRows -------------------------------------------
-// Bound by the weights' bytes (1,024 x 4,096 bf16: 3.3 us, a launch and the way to HBM and back being
-// 2.5 of them).  A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
+// ---- one row; a few float or unaligned rows ------------------------------------------------------
+// Bound by the weights' bytes (1,024 x 4,096 bf16: 3.0 us, most of it a launch and the way to HBM and back).  A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
 // that the weights are read once; the tokens come from L1.  Float operands stay float.
 template <typename T, typename O, int V, int ROWS, int C>
 __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, int m,
@@ -20,6 +29,9 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_str
   const int lane = threadIdx.x & 31;
   const int j0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * C;
   if (j0 >= n) return;
+  const int r0 = blockIdx.y * ROWS;  // float rows beyond ROWS: the weights come from L2 for each ROWS more
+  x += int64_t(r0) * x_stride;
+  m -= r0;
   float acc[ROWS][C];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
@@ -43,22 +55,23 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_str
         for (int u = 0; u < V; ++u) acc[r][c] = fmaf(xv[u], wv[c][u], acc[r][c]);
     }
   }
+  // lane r C + c keeps that sum, so that the lanes finish theirs together
+  float z[1] = {0.0f};
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const float s = warp_sum(acc[r][c]);
-      if (lane == r * C + c && r < m && j0 + c < n) {
-        float z[1] = {s};
-        finish<O, 1>(e, n, r, j0 + c, z);
-      }
+      if (lane == r * C + c) z[0] = s;
     }
+  const int r = lane / C, c = lane % C;
+  if (r < ROWS && r < m && j0 + c < n) finish<O, 1>(e, n, r0 + r, j0 + c, z);
 }
 
 template <typename T, typename O, int V>
 void few_rows_v(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
   const auto run = [&](auto kernel, int cols) {
-    kernel<<<(p.n + 4 * cols - 1) / (4 * cols), 128, 0, st>>>(static_cast<const T*>(p.x), p.x_stride,
+    kernel<<<dim3((p.n + 4 * cols - 1) / (4 * cols), unsigned((p.m + 7) / 8)), 128, 0, st>>>(static_cast<const T*>(p.x), p.x_stride,
                                                               static_cast<const T*>(p.weight), p.weight_stride,
                                                               int(p.m), p.n, p.k, e);
     note_launch();
@@ -382,7 +395,7 @@ Product dw_shape(const gsb_linear& p) {
 FwdSpace fwd_space(const gsb_linear& p, void* ws, size_t cap) {
   Carver c(ws, cap);
   FwdSpace s{};
-  if (p.m > kFewRows) {
+  if (path_of(p) == Path::kTiles) {
     if (!fits_tma(p.x, p.x_stride, p.dtype)) s.x = c.take<char>(copy_bytes(p.m, p.k, p.dtype));
     if (!fits_tma(p.weight, p.weight_stride, p.dtype)) s.w = c.take<char>(copy_bytes(p.n, p.k, p.dtype));
     const Product q = fwd_shape(p);
@@ -522,8 +535,12 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   const int b = elem_bytes(p->out_dtype);
   e.vec = e.vec && vec_ok(p->bias, 0, b, 16) && vec_ok(preact, 0, b, 16) &&
           (!p->residual || vec_ok(p->residual, p->residual_stride, b, 16));
-  if (p->m > kFewMma && few_rows_mma(*p, e, st)) return launch_status();
-  if (p->m <= kFewRows) {
+  const Path path = path_of(*p);
+  if (path == Path::kFewMma) {
+    few_rows_mma(*p, e, st);
+    return launch_status();
+  }
+  if (path == Path::kWalk) {
     switch (p->dtype) {
       case GSB_F32: few_rows<float, float>(*p, e, st); break;
       case GSB_BF16: few_rows<bf16, bf16>(*p, e, st); break;

@@ -139,14 +139,18 @@ void launch(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
 
 }  // namespace
 
-bool few_rows_mma(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
+bool few_rows_mma_serves(const gsb_linear& p) {
   const int b = elem_bytes(p.dtype);
-  // 17 to 32 rows: their values' way through L1 outweighs the weights' once those are large
-  // (1,024 x 1,024 bf16: 3.7 us here, 9.3 on tcgen05 tiles; 2,048 x 8,192: 16.0 and 14.8)
-  const int64_t most = int64_t(p.n) * p.k * b <= (8 << 20) ? 32 : 16;
-  if (p.dtype == GSB_F32 || p.m > most || p.k % (16 / b) != 0 || !vec_ok(p.x, p.x_stride, b, 16) ||
+  if (p.dtype == GSB_F32 || p.k % (16 / b) != 0 || !vec_ok(p.x, p.x_stride, b, 16) ||
       !vec_ok(p.weight, p.weight_stride, b, 16))
     return false;
+  // from 2 rows (2,048 x 8,192 e4m3: 6.0 us, 8.4 one row after the other); 17 to 32 rows: their values'
+  // way through L1 outweighs the weights' once those are large (1,024 x 1,024 bf16: 3.7 us here, 9.3 on
+  // tcgen05 tiles; 2,048 x 8,192: 16.0 and 14.8)
+  return p.m >= 2 && p.m <= (int64_t(p.n) * p.k * b <= (8 << 20) ? 32 : 16);
+}
+
+void few_rows_mma(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
   switch (p.dtype) {
     case GSB_BF16: launch<bf16, bf16>(p, e, st); break;
     case GSB_F16: launch<f16, f16>(p, e, st); break;
@@ -155,7 +159,6 @@ bool few_rows_mma(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
       else if (p.out_dtype == GSB_BF16) launch<e4m3, bf16>(p, e, st);
       else launch<e4m3, f16>(p, e, st);
   }
-  return true;
 }
 
 }  // namespace gsb

@@ -121,8 +121,9 @@ inline int k_blocks_of(const Product& p) {
   return int((p.k + per - 1) / per);
 }
 
-// Up to 32 aligned rows of 16-bit or e4m3 values (linear_few.cu); false where it does not apply.
-bool few_rows_mma(const gsb_linear& p, const Epilogue& e, cudaStream_t st);
+// 2 to 32 aligned rows of 16-bit or e4m3 values (linear_few.cu).
+bool few_rows_mma_serves(const gsb_linear& p);
+void few_rows_mma(const gsb_linear& p, const Epilogue& e, cudaStream_t st);
 
 // Blocks of K of one of its `splits` pieces, and how many pieces that makes.
 inline int piece_of(const Product& p, int splits) { return (k_blocks_of(p) + splits - 1) / splits; }
