@@ -21,7 +21,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libgsb200.so"
 SOURCES = ["abi.cu", "preprocess.cu", "sort.cu", "bin.cu", "raster.cu", "loss.cu", "splat2d.cu",
-           "norm.cu", "norm_ring.cu", "linear.cu", "linear_few.cu", "linear_mma.cu", "linear_mma_bf16.cu", "linear_mma_f16.cu", "linear_mma_sums.cu",
+           "norm.cu", "norm_ring.cu", "linear.cu", "linear_few.cu", "linear_mma.cu", "linear_mma_bf16.cu",
+           "linear_mma_f16.cu", "linear_mma_sums.cu",
            "linear_mma_f32.cu", "linear_mma_e4m3.cu"]
 TORCH_SOURCE = "token_torch.cpp"  # the token-side operators' torch binding (host code, no CUDA compiler)
 TORCH_LIB = PKG / "_token_torch.so"

@@ -21,8 +21,9 @@ Path path_of(const gsb_linear& p) {
 }
 
 // ---- one row; a few float or unaligned rows ------------------------------------------------------
-// Bound by the weights' bytes (1,024 x 4,096 bf16: 3.0 us, most of it a launch and the way to HBM and back).  A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at once, so
-// that the weights are read once; the tokens come from L1.  Float operands stay float.
+// Bound by the weights' bytes (1,024 x 4,096 bf16: 3.0 us, most of it a launch and the way to HBM and
+// back).  A warp owns C columns and walks their weight rows in 16-byte accesses, all ROWS tokens at
+// once, so that the weights are read once; the tokens come from L1.  Float operands stay float.
 template <typename T, typename O, int V, int ROWS, int C>
 __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, int m,
                                                        int n, int k, Epilogue e) {
@@ -71,9 +72,9 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const T* x, int64_t x_str
 template <typename T, typename O, int V>
 void few_rows_v(const gsb_linear& p, const Epilogue& e, cudaStream_t st) {
   const auto run = [&](auto kernel, int cols) {
-    kernel<<<dim3((p.n + 4 * cols - 1) / (4 * cols), unsigned((p.m + 7) / 8)), 128, 0, st>>>(static_cast<const T*>(p.x), p.x_stride,
-                                                              static_cast<const T*>(p.weight), p.weight_stride,
-                                                              int(p.m), p.n, p.k, e);
+    const dim3 grid((p.n + 4 * cols - 1) / (4 * cols), unsigned((p.m + 7) / 8));
+    kernel<<<grid, 128, 0, st>>>(static_cast<const T*>(p.x), p.x_stride, static_cast<const T*>(p.weight), p.weight_stride,
+                                 int(p.m), p.n, p.k, e);
     note_launch();
   };
   if (p.m == 1) return run(few_rows_kernel<T, O, V, 1, 2>, 2);
@@ -341,7 +342,8 @@ template <typename T, int ACT>
 void launch_dz(const DzJob& d, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   // z and dz are this library's own, aligned whenever n is a multiple of V
-  if (d.n % V == 0 && vec_ok(d.dy, d.dy_stride, sizeof(T), V * sizeof(T)) && vec_ok(d.z, 0, 1, 16)) launch_dz_v<T, ACT, V>(d, st);
+  if (d.n % V == 0 && vec_ok(d.dy, d.dy_stride, sizeof(T), V * sizeof(T)) && vec_ok(d.z, 0, 1, 16))
+    launch_dz_v<T, ACT, V>(d, st);
   else launch_dz_v<T, ACT, 1>(d, st);
 }
 

@@ -392,7 +392,8 @@ template <typename T>
 gsb_status bwd_of_type(const NormArgs& a, void* dw, cudaStream_t st) {
   constexpr int E = sizeof(T);
   const bool ok = a.dim % (16 / E) == 0 && vec_ok(a.x, a.x_stride, E, 16) && vec_ok(a.dy, a.dy_stride, E, 16) &&
-                  (!a.res || vec_ok(a.res, a.res_stride, E, 16)) && (!a.dsum || vec_ok(a.dsum, a.dsum_stride, E, 16)) && vec_ok(a.w, 0, E, 16) && vec_ok(a.dx, 0, E, 16);
+                  (!a.res || vec_ok(a.res, a.res_stride, E, 16)) && (!a.dsum || vec_ok(a.dsum, a.dsum_stride, E, 16)) &&
+                  vec_ok(a.w, 0, E, 16) && vec_ok(a.dx, 0, E, 16);
   const int code = sizeof(T) == 4 ? GSB_F32 : std::is_same<T, bf16>::value ? GSB_BF16 : GSB_F16;
   const Split s = split_of(a.dim, E, ok);
   int parts;
@@ -481,7 +482,8 @@ gsb_status quantize_rows_fp8(const gsb_norm* n, void* codes, float* scales, cuda
 
 size_t rms_norm_bwd_workspace(const gsb_norm* n) {
   if (check_norm(n) != GSB_OK) return 0;
-  const size_t parts = std::max<size_t>(kWideParts, bwd_blocks(n->rows, 1));  // at least one per SM: the ring's too
+  // as many rows of sums as any of the kernels leaves (the ring: one per SM)
+  const size_t parts = std::max<size_t>(kWideParts, bwd_blocks(n->rows, 1));
   return align_up(parts * size_t(n->dim) * 4);
 }
 
