@@ -25,9 +25,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     in x, weight, bias and residual.  With an activation the forward keeps x weight^T + bias for the
     backward (float beside float32 operands, else float16), and the backward rounds
     dy act'(z) to the operands' type before its two products.  The same inputs give the same bits.
-    Rows may lie apart (any row stride); other layouts are copied.  float32 operands of more than 8
-    rows are multiplied as sums of three bfloat16 parts, as exactly as float32 sums are; an infinity
-    among them may give NaN."""
+    Rows may lie apart (any row stride); other layouts are copied.  float32 products of more than 8
+    rows (64 with at most 8 MB of weights), and the backward's, take their operands as sums of three
+    bfloat16 parts, as exact as float32 sums; an infinity among them may give NaN."""
     return _token.ext().linear(x, weight, bias, residual, activation, _token.traced())
 
 
