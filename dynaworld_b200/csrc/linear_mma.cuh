@@ -245,6 +245,11 @@ __device__ __forceinline__ int stage_at(int r, int q) { return r * 32 + ((q ^ (r
 // about 600 cycles, the residual's way from HBM more.
 constexpr int kAnyAct = -1;  // the activation is chosen at run time
 
+template <int ACT>
+__device__ __forceinline__ bool is_relu(const Job& p) {
+  return (ACT == kAnyAct ? p.e.act : ACT) == GSB_ACT_RELU;
+}
+
 template <int ACT, int V>
 __device__ __forceinline__ void activate(const Job& p, float (&z)[V]) {
   if constexpr (ACT == kAnyAct) apply_act<V>(p.e.act, z);
@@ -350,7 +355,7 @@ struct Rows {
             for (int h = 0; h < 2; ++h)
               if (s0 + h < steps)
                 *reinterpret_cast<Vec<Z, V>*>(keep + (s0 + h) * kAtOnce * p.n) =
-                    kept_of<V>(static_cast<Z*>(nullptr), reinterpret_cast<const float(&)[V]>(z[h * V]));
+                    kept_of<V>(static_cast<Z*>(nullptr), reinterpret_cast<const float(&)[V]>(z[h * V]), is_relu<ACT>(p));
           }
           activate<ACT, 2 * V>(p, z);
           if (p.e.res) {
@@ -395,7 +400,7 @@ struct Rows {
           if (p.e.preact) {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-              if (r0 + r < rows) keep[(r0 + r) * p.n] = as_preact(static_cast<Z*>(nullptr), z[r]);
+              if (r0 + r < rows) keep[(r0 + r) * p.n] = as_preact(static_cast<Z*>(nullptr), z[r], is_relu<ACT>(p));
           }
           activate<ACT, 8>(p, z);
           if (p.e.res) {

@@ -41,9 +41,15 @@ struct Product {
 
 // The pre-activation kept for the backward: float beside float operands, else fp16 saturated at
 // its largest value.  fp16 and not bf16: its 11 bits keep the slope's error (at most 2^-11 |z|
-// act'') an eighth of the rounding that dz gets, and beyond +-65504 every slope is constant.
-__device__ __forceinline__ float as_preact(float*, float z) { return z; }
-__device__ __forceinline__ f16 as_preact(f16*, float z) {
+// act'') an eighth of the rounding that dz gets, and beyond +-65504 every slope is constant.  ReLU's
+// slope jumps at 0 however small z is: there a z that would round to 0 from above is kept as the least
+// fp16 (bf16 operands reach z = 1e-38, and their gradients would be lost).
+constexpr float kLeastHalf = 5.9604644775390625e-08f;  // 2^-24
+__device__ __forceinline__ float on_its_side(float z) { return z > 0.0f ? fmaxf(z, kLeastHalf) : z; }
+
+__device__ __forceinline__ float as_preact(float*, float z, bool) { return z; }
+__device__ __forceinline__ f16 as_preact(f16*, float z, bool relu) {
+  if (relu) z = on_its_side(z);
   uint16_t h;
   asm("cvt.rn.satfinite.f16.f32 %0, %1;" : "=h"(h) : "f"(z));
   return __ushort_as_half(h);
@@ -65,25 +71,25 @@ __device__ __forceinline__ void apply_act(int act, float (&z)[V]) {
   }
 }
 
-// z as it is kept.
+// z as it is kept; relu: for ReLU's backward.
 template <int V>
-__device__ __forceinline__ Vec<float, V> kept_of(float*, const float (&z)[V]) {
+__device__ __forceinline__ Vec<float, V> kept_of(float*, const float (&z)[V], bool) {
   Vec<float, V> k;
 #pragma unroll
   for (int u = 0; u < V; ++u) k.v[u] = z[u];
   return k;
 }
 template <int V>
-__device__ __forceinline__ Vec<f16, V> kept_of(f16*, const float (&z)[V]) {
+__device__ __forceinline__ Vec<f16, V> kept_of(f16*, const float (&z)[V], bool relu) {
   Vec<f16, V> k;
   if constexpr (V == 1) {
-    k.v[0] = as_preact(static_cast<f16*>(nullptr), z[0]);
+    k.v[0] = as_preact(static_cast<f16*>(nullptr), z[0], relu);
   } else {
 #pragma unroll
-    for (int u = 0; u < V; u += 2)
-      asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;"
-          : "=r"(*reinterpret_cast<uint32_t*>(&k.v[u]))
-          : "f"(z[u + 1]), "f"(z[u]));
+    for (int u = 0; u < V; u += 2) {
+      const float lo = relu ? on_its_side(z[u]) : z[u], hi = relu ? on_its_side(z[u + 1]) : z[u + 1];
+      asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(*reinterpret_cast<uint32_t*>(&k.v[u])) : "f"(hi), "f"(lo));
+    }
   }
   return k;
 }
@@ -104,7 +110,8 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t n, int64_t i, 
     for (int u = 0; u < V; ++u) z[u] += b[u];
   }
   if (e.preact) {
-    *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) = kept_of<V>(static_cast<Z*>(nullptr), z);
+    *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) =
+        kept_of<V>(static_cast<Z*>(nullptr), z, e.act == GSB_ACT_RELU);
   }
   apply_act<V>(e.act, z);
   if (e.res) {

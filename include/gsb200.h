@@ -460,7 +460,8 @@ typedef struct gsb_linear {
 
 GSB_API size_t gsb_linear_fwd_workspace(const gsb_linear* linear);
 /* preact (or NULL) [m,n] keeps z = x weight^T + bias for the backward: float for F32 operands, fp16
-   saturated at its largest value for 16-bit ones (every activation is flat or linear there). */
+   saturated at its largest value for 16-bit ones (every activation is flat or linear there) and, for
+   RELU, not below its least positive value where z > 0. */
 GSB_API gsb_status gsb_linear_fwd(const gsb_linear* linear, void* y, void* preact, void* workspace,
                                   size_t workspace_bytes, void* stream);
 GSB_API size_t gsb_linear_bwd_workspace(const gsb_linear* linear, const void* dy,

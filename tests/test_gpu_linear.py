@@ -240,6 +240,30 @@ def test_saturated_preactivations(t):
         assert bool((g[:70].float() == 32 * float(w[0, 0])).all())
 
 
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 40), (3, 64, 40), (5, 65, 41), (300, 64, 264), (129, 65, 131),
+                                   (200, 2048, 64)])
+def test_relu_of_small_preactivations(m, k, n, t):
+    """Every |z| is far below fp16's least value: ReLU's slope is still 1 wherever z > 0, on every path (one
+    row, few rows, tiles, rows off 16 bytes, pieces).  Only within the sum's own error of 0 is it open."""
+    x, w, _, _, dy = make(m, k, n, torch.float32, seed=m + k)
+    s = 2.0 ** -15 if t == torch.float16 else 2.0 ** -30
+    x, w, dy = (s * x).to(t), (s * math.sqrt(k) * w).to(t), dy.to(t)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, torch.zeros(n, dtype=t, device=DEV))]
+    dx, dw, db = torch.autograd.grad(linear(*leaves, activation="relu"), leaves, dy)
+    X, W, G = x.double(), w.double(), dy.double()
+    z = X @ W.T
+    dz = torch.where(z > 0, G, 0.0)
+    err = torch.where(z.abs() <= (k + 2) * U * (X.abs() @ W.abs().T), G.abs(), 0.0)
+    whole = dz.abs() + err
+    ref = dz @ W
+    within(dx, ref, ref.abs() * half(t) + err @ W.abs() + (n + 2) * U * (whole @ W.abs()) + tiny(t), "dx")
+    ref = dz.T @ X
+    within(dw, ref, ref.abs() * half(t) + err.T @ X.abs() + (m + 2) * U * (whole.T @ X.abs()) + tiny(t), "dw")
+    ref = dz.sum(0)
+    within(db, ref, ref.abs() * half(t) + err.sum(0) + (m + 2) * U * whole.sum(0) + tiny(t), "db")
+
+
 def test_same_bits_every_run():
     for t in TYPES:
         x, w, b, r, dy = make(3000, 136, 72, t)
