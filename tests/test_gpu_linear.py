@@ -295,6 +295,38 @@ def test_gradient_against_differences():
             assert abs(float((f(plus) - f(minus)) / (2 * step)) - float(got[i][idx])) < 2e-5
 
 
+# products that are cut into pieces along K: small outputs of long sums, aligned and not
+LONG = [(300, 4096, 1024), (64, 4096, 512), (100, 4100, 515), (40, 8192, 264)]
+
+
+def pieces_of(dtype, m, k, n):
+    """Bytes of the forward's float sums of pieces: its workspace, where the operands are read in place."""
+    import ctypes
+
+    p = _lib.Linear(m=m, n=n, k=k, dtype=dtype, out_dtype=dtype if dtype != _lib.E4M3 else _lib.BF16, x=256,
+                    x_stride=k, weight=256, weight_stride=k, x_scale=256, weight_scale=256)
+    return _lib.lib().gsb_linear_fwd_workspace(ctypes.byref(p)) // (4 * m * n)
+
+
+def test_long_sums_are_cut():
+    """What the tests below are about: every aligned shape of LONG runs in pieces, in every type that is
+    read in place."""
+    for m, k, n in LONG:
+        for dtype in (_lib.BF16, _lib.F16, _lib.E4M3):
+            if k % (16 if dtype == _lib.E4M3 else 8) == 0:
+                assert pieces_of(dtype, m, k, n) >= 2, (m, k, n, dtype)
+    assert pieces_of(_lib.BF16, 8192, 1024, 4096) == 0
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,k,n", LONG)
+def test_long_sums_and_gradients(m, k, n, act, t):
+    x, w, b, r, dy = make(m, k, n, t, seed=m)
+    check(x, w, b, r, dy, act)
+    check(x, w, None, None, dy, act)
+
+
 # ---- 8-bit operands ----
 
 
@@ -313,6 +345,26 @@ def test_fp8(m, k, n, t):
     ref = act64(z, act)[0] + r.double()
     within(y, ref, ref.abs() * half(t) * 1.001 + 1.13 * (k + 4) * U * mag + z.abs() * 2.0 ** -20 + 2.0 ** -24 +
            r.double().abs() * U + tiny(t))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,k,n", LONG)
+def test_fp8_long_sums(m, k, n, act, t):
+    x, w, b, r, _ = make(m, k, n, torch.float32, seed=m + k)
+    b, r = b.to(t), r.to(t)
+    xq, xs = quantize_rows_fp8(x)
+    wq, ws = quantize_rows_fp8(w)
+    X, W = xq.double() * xs.double()[:, None], wq.double() * ws.double()[:, None]
+    z, mag = X @ W.T, X.abs() @ W.abs().T
+    for bias, res in ((b, r), (None, None)):
+        y = linear_fp8(xq, xs, wq, ws, bias, activation=act, residual=res, dtype=t)
+        zb, mb, rd = z, mag, torch.zeros_like(z)
+        if bias is not None:
+            zb, mb, rd = z + b.double(), mag + b.double().abs(), r.double()
+        ref = act64(zb, act)[0] + rd
+        within(y, ref, ref.abs() * half(t) * 1.001 + 1.13 * (k + 4) * U * mb + zb.abs() * 2.0 ** -20 + 2.0 ** -24 +
+               rd.abs() * U + tiny(t))
 
 
 def test_fp8_strides_and_dimensions():
