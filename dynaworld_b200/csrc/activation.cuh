@@ -86,9 +86,11 @@ __device__ __forceinline__ F2 act_value(F2 z) {
   if constexpr (ACT == GSB_ACT_RELU) {
     return each(z, [](float x) { return x < 0.0f ? 0.0f : x; });
   } else if constexpr (ACT == GSB_ACT_GELU) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|), whose second term is 0 from z = 15 on: there |z| ends at 1e4, so
+    // that +infinity does not meet that 0 (-infinity does: NaN, as z Phi(z) is)
     F2 minus, gauss;
-    const F2 tail = normal_tail(z, minus, gauss);
-    return fma2(minus, tail, each(z, [](float x) { return fmaxf(x, 0.0f); }));  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const F2 tail = normal_tail(each(z, [](float x) { return fminf(x, 1e4f); }), minus, gauss);
+    return fma2(minus, tail, each(z, [](float x) { return fmaxf(x, 0.0f); }));
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
     return mul2(z, sigmoid_of(gelu_tanh_arg(z, mul2(z, z))));
   } else if constexpr (ACT == GSB_ACT_SILU) {

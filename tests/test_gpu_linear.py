@@ -216,6 +216,33 @@ def test_nonfinite_rows_stay_in_their_row(m, t):
     assert torch.equal(y2[keep], y[keep])
 
 
+def same_kind(got, ref):
+    """Equal, or both NaN."""
+    return bool(((got == ref) | (got.isnan() & ref.isnan())).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,k", [(1, 64), (4, 64), (4, 65), (130, 64), (130, 65), (64, 4096)])
+def test_infinite_preactivations(m, k, act, t):
+    """z of +infinity and -infinity (float and bf16: finite operands whose products overflow) give what the
+    formula gives, on every path."""
+    x, w = torch.zeros(m, k, dtype=t, device=DEV), torch.zeros(512, k, dtype=t, device=DEV)
+    x[:, 0], x[:, 1] = (math.inf if t == torch.float16 else 3e38), 1
+    w[:, 0], w[:, 1] = 1, 0.5
+    w[::2, 0], w[1::2, 0] = 4, -4
+    ref = act64(torch.tensor([math.inf, -math.inf], dtype=torch.float64), act)[0].to(DEV, t)
+    y = linear(x, w, activation=act)
+    assert float(ref[0]) == math.inf
+    assert same_kind(y, ref.repeat(256).expand(m, 512)), y[0, :2]
+    if t == torch.float32:
+        return
+    q, s = torch.ones(m, k, device=DEV).to(E4M3), torch.full((m,), 2e38, device=DEV)
+    q2 = w.float().clamp(-1, 1).to(E4M3)
+    y = linear_fp8(q, s, q2, torch.full((512,), 2e38, device=DEV), activation=act, dtype=t)
+    assert same_kind(y, ref.repeat(256).expand(m, 512)), y[0, :2]
+
+
 def test_large_values_in_float32():
     """Values near the type's largest, whose bf16 rounding would overflow."""
     x = torch.full((130, 64), 0.0, device=DEV)
