@@ -7,6 +7,7 @@
 // 12.5 on the host that way, a norm with its gradients 107, most of it in the Python halves of the
 // autograd engine.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -121,6 +122,17 @@ void check_device(const char* what, const Tensor& x) {
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
+
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+
+// Forward-mode derivatives have no formula here: a dual tensor (which need not require a gradient) would
+// lose its tangent silently.
+template <typename... T>
+void refuse_tangent(const char* what, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && (has_tangent(t) || ...)), what,
+                              " has no forward-mode derivative; unpack its dual tensors or use reverse mode.");
+}
 
 template <typename... T>
 void refuse_grad(const char* what, const T&... t) {
@@ -268,6 +280,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
   const int code = check_input("linear", x);
   const int act = activation_code(activation);
   const int64_t n = check_shapes("linear", x, weight, bias, residual, x.scalar_type());
+  refuse_tangent("linear", x, weight, bias, residual);
   check_device("linear", x);
   const Tensor x2 = rows_of(x, x.size(-1)), w2 = rows_of(weight, weight.size(1));
   const OptTensor r2 = rows_of(residual, n), b = bias ? OptTensor(bias->contiguous()) : std::nullopt;
@@ -297,6 +310,7 @@ Tensor linear_fp8(const Tensor& x, const Tensor& x_scale, const Tensor& weight, 
   const int64_t n = check_shapes(what, x, weight, bias, residual, type);
   check_like(what, "x_scale", x_scale, x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
   check_like(what, "weight_scale", weight_scale, {n}, at::kFloat, x);
+  refuse_tangent(what, x_scale, weight_scale, bias, residual);
   check_device(what, x);
   refuse_grad(what, x_scale, weight_scale, bias, residual);
   const Tensor x2 = rows_of(x, x.size(-1)), w2 = rows_of(weight, weight.size(1));
@@ -388,6 +402,7 @@ int check_norm(const char* what, const Tensor& x, const OptTensor& weight, const
   if (weight) check_like(what, "weight", *weight, {x.size(-1)}, x.scalar_type(), x);
   if (residual) check_like(what, "residual", *residual, x.sizes(), x.scalar_type(), x);
   TORCH_CHECK_VALUE(eps >= 0.0, what, ": eps must not be negative, got ", eps);
+  refuse_tangent(what, x, weight, residual);
   check_device(what, x);
   return code;
 }

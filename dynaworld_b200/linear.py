@@ -22,7 +22,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     "gelu", "gelu_tanh" (its tanh form) or "silu".
 
     Sums, bias, activation and residual are formed in float and rounded once.  Differentiable once
-    in x, weight, bias and residual.  With an activation the forward keeps x weight^T + bias for the
+    in x, weight, bias and residual (reverse mode; tangents of forward mode are refused).  With an activation the forward keeps x weight^T + bias for the
     backward (float beside float32 operands, else float16), and the backward rounds
     dy act'(z) to the operands' type before its two products.  The same inputs give the same bits.
     Rows may lie apart (any row stride); other layouts are copied.  float32 products of more than 8

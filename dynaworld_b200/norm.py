@@ -19,7 +19,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
     x and residual [..., D], weight [D], all float32, bfloat16 or float16 of one type.  Returns y,
     or with a residual the pair (y, h): h is the new residual stream.  The sum, the statistics and
     the product are formed in float; y and h are rounded once.  Differentiable in x, weight and
-    residual (once; the backward forms h again from x and residual); the weight gradient is the same
+    residual (once, in reverse mode; the backward forms h again from x and residual); the weight gradient is the same
     on every run."""
     return _token.ext().rms_norm(x, weight, residual, eps, _token.traced())
 

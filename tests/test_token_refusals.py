@@ -55,6 +55,36 @@ def test_refused(error, match, call):
         call()
 
 
+def test_dual_tensors_are_refused():
+    """A tangent in any argument raises (its derivative would be lost), with and without reverse mode beside
+    it; without one, or with forward mode off, the call goes on to the check of the device."""
+    import torch.autograd.forward_ad as fwd
+
+    q = F(2, 4, dtype=E4M3)
+    with fwd.dual_level():
+        d24, d34, d3, d23, d4, d2 = (fwd.make_dual(F(*s), torch.ones(*s)) for s in ((2, 4), (3, 4), (3,), (2, 3), (4,), (2,)))
+        for call in (lambda: linear(d24, F(3, 4)), lambda: linear(F(2, 4), d34), lambda: linear(F(2, 4), F(3, 4), d3),
+                     lambda: linear(F(2, 4), F(3, 4), residual=d23),
+                     lambda: linear(d24, F(3, 4).requires_grad_(True)),
+                     lambda: linear_fp8(q, d2, F(3, 4, dtype=E4M3), F(3)),
+                     lambda: linear_fp8(q, F(2), F(3, 4, dtype=E4M3), d3),
+                     lambda: linear_fp8(q, F(2), F(3, 4, dtype=E4M3), F(3), d3, dtype=torch.float32),
+                     lambda: linear_fp8(q, F(2), F(3, 4, dtype=E4M3), F(3), residual=d23, dtype=torch.float32),
+                     lambda: rms_norm(d24, F(4)), lambda: rms_norm(F(2, 4), d4),
+                     lambda: rms_norm(F(2, 4), F(4), residual=d24), lambda: rms_norm_fp8(d24, F(4)),
+                     lambda: rms_norm_fp8(F(2, 4), d4), lambda: quantize_rows_fp8(d24)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA devices only"):
+            linear(fwd.unpack_dual(d24).primal, F(3, 4))
+        with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA devices only"):
+            linear(d24, F(3, 4))
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        linear(F(2, 4), F(3, 4))
+
+
 @pytest.fixture(scope="module")
 def lib():
     build.build()
