@@ -38,7 +38,8 @@ int* gave_up_flag() {
 }
 
 gsb_status gave_up_status(int* gave_up) {
-  if (cudaMemcpyFromSymbol(gave_up, g_gave_up, sizeof(int)) != cudaSuccess) {
+  // every stream: the copy waits for the legacy default stream only, and torch's are non-blocking ones
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(gave_up, g_gave_up, sizeof(int)) != cudaSuccess) {
     (void)cudaGetLastError();
     return GSB_ERR_CUDA;
   }

@@ -476,7 +476,7 @@ GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, 
 
 /* GSB_ERR_TIMEOUT once a bounded device-side wait of a token-side operator gave up on the current device
    since the library was loaded (the outputs of that call hold NaN where it happened), else GSB_OK.
-   Waits for the device's queued work. */
+   Waits for the device's queued work on every stream (not allowed while a stream is captured). */
 GSB_API gsb_status gsb_token_status(void);
 
 /* ---- utility: the library's radix sort on its own (tests, benchmarks) --------------------- */

@@ -591,3 +591,15 @@ def test_no_wait_gave_up():
     x, w, b, r, dy = make(300, 264, 144, torch.bfloat16)
     linear(x, w, b)
     assert _lib.lib().gsb_token_status() == _lib.GSB_OK
+
+
+def test_status_waits_for_every_stream():
+    """The status of work that is still queued on a non-blocking stream is not given before that work ends."""
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # about 0.2 s
+        done.record()
+    assert not done.query()
+    assert _lib.lib().gsb_token_status() == _lib.GSB_OK
+    assert done.query()
