@@ -164,6 +164,7 @@ SIGNATURES = {
     "gsb_linear_fwd": (C.c_int, [P(Linear), vp, vp, vp, C.c_size_t, vp]),
     "gsb_linear_bwd_workspace": (C.c_size_t, [P(Linear), vp, C.c_int64]),
     "gsb_token_status": (C.c_int, []),
+    "gsb_debug_token_timeout": (C.c_int, [C.c_uint32, vp]),
     "gsb_linear_bwd": (C.c_int, [P(Linear), vp, vp, C.c_int64, vp, vp, vp, vp, C.c_size_t, vp]),
     "gsb_radix_sort_workspace": (C.c_size_t, [C.c_uint32, C.c_int, C.c_int]),
     "gsb_radix_sort": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),

@@ -627,4 +627,8 @@ GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, 
 
 GSB_API gsb_status gsb_token_status(void) { return token_status(); }
 
+GSB_API gsb_status gsb_debug_token_timeout(uint32_t limit_us, void* stream) {
+  return token_timeout_probe(limit_us, as_stream(stream));
+}
+
 }  // extern "C"

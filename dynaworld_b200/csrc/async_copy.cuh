@@ -36,11 +36,11 @@ __device__ __forceinline__ uint64_t now_ns() {
 }
 
 // Bounded wait; false when it gave up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* gave_up) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* gave_up, uint64_t limit_ns = kWaitNs) {
   for (int i = 0; i < 256; ++i)
     if (bar_try(bar, parity)) return true;
   const uint64_t t0 = now_ns();
-  while (now_ns() - t0 < kWaitNs) {
+  while (now_ns() - t0 < limit_ns) {
     for (int i = 0; i < 64; ++i)
       if (bar_try(bar, parity)) return true;
   }

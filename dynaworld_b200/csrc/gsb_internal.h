@@ -173,6 +173,7 @@ size_t linear_fwd_workspace(const gsb_linear* p);
 gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size_t ws_bytes, cudaStream_t st);
 size_t linear_bwd_workspace(const gsb_linear* p, const void* dy, int64_t dy_stride);
 gsb_status token_status();
+gsb_status token_timeout_probe(uint32_t limit_us, cudaStream_t st);
 gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, int64_t dy_stride, void* dx,
                       void* dweight, void* dbias, void* ws, size_t ws_bytes, cudaStream_t st);
 

@@ -43,7 +43,26 @@ gsb_status gave_up_status(int* gave_up) {
     (void)cudaGetLastError();
     return GSB_ERR_CUDA;
   }
+  const int none = 0;  // reported once
+  if (*gave_up && cudaMemcpyToSymbol(g_gave_up, &none, sizeof(int)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return GSB_ERR_CUDA;
+  }
   return GSB_OK;
+}
+
+// One thread waits, as the kernels do, on a barrier that nothing completes.
+static __global__ void timeout_probe_kernel(uint64_t limit_ns, int* gave_up) {
+  __shared__ __align__(8) uint64_t bar;
+  bar_init(smem_addr(&bar), 1);
+  (void)bar_wait(smem_addr(&bar), 0, gave_up, limit_ns);
+}
+
+gsb_status token_timeout_probe(uint32_t limit_us, cudaStream_t st) {
+  int* flag = gave_up_flag();
+  if (!flag) return GSB_ERR_CUDA;
+  timeout_probe_kernel<<<1, 1, 0, st>>>(uint64_t(std::min<uint32_t>(limit_us, 1000000)) * 1000, flag);
+  return launch_status();
 }
 
 // ---- plans ------------------------------------------------------------------------------------

@@ -161,7 +161,7 @@ gsb_status mma_launch_bf16(const Product* p, const Epilogue* e, int count, int b
 gsb_status mma_launch_f16(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 gsb_status mma_launch_f32(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
 gsb_status mma_launch_e4m3(const Product* p, const Epilogue* e, int count, int bn, const int* splits, cudaStream_t st);
-// 1 once a bounded wait of a token-side kernel gave up on the current device.
+// 1 when a bounded wait of a token-side kernel gave up on the current device since this last gave 1.
 gsb_status gave_up_status(int* gave_up);
 
 }  // namespace gsb

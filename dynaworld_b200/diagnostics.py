@@ -18,6 +18,9 @@ the work the raster kernels did, and nothing is recomputed.
 Collecting keeps references to two device tensors per render call (no copies, no kernels); the
 summary runs torch reductions on them and reads back one scalar per statistic.
 
+Token-side operators (linear, rms_norm and their 8-bit forms) do not read a status back from the
+GPU; ``check_token_status`` asks for it where a program waits anyway, or where NaN has to be explained.
+
 NVTX: with ``nvtx(True)`` (or GSB200_NVTX=1 in the environment) every C-ABI stage of the render
 (depth_order, preprocess_fwd, bin, raster_fwd, loss, raster_bwd, preprocess_bwd, ...) is a named
 NVTX range "gsb:<stage>" on the host timeline, for Nsight Systems.
@@ -31,7 +34,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import render
+from . import _lib, render
 
 SELECTED_KEYS = ("total_overlap_keys", "duplication_factor", "p95_tiles_per_splat", "max_tiles_per_splat",
                  "large_splat_count", "p95_splats_per_tile", "max_splats_per_tile")
@@ -59,6 +62,14 @@ class FrameLists:
     def per_tile_counts(self, view: int) -> torch.Tensor:
         r = self.ranges.view(self.n_views, self.n_tiles, 2)[view].to(torch.int64)
         return r[:, 1] - r[:, 0]
+
+
+def check_token_status(device: torch.device | str | int | None = None) -> None:
+    """Waits for the work queued on ``device`` (the current one) and raises GsbError (GSB_ERR_TIMEOUT)
+    if a bounded wait inside a token-side operator gave up since the last time this raised; that call's
+    outputs hold NaN.  Not to be called while a stream is captured."""
+    with torch.cuda.device(device):
+        _lib.check("gsb_token_status", _lib.lib().gsb_token_status())
 
 
 @contextlib.contextmanager

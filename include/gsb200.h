@@ -474,10 +474,14 @@ GSB_API gsb_status gsb_linear_bwd(const gsb_linear* linear, const void* preact, 
                                   int64_t dy_stride, void* dx, void* dweight, void* dbias,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
-/* GSB_ERR_TIMEOUT once a bounded device-side wait of a token-side operator gave up on the current device
-   since the library was loaded (the outputs of that call hold NaN where it happened), else GSB_OK.
-   Waits for the device's queued work on every stream (not allowed while a stream is captured). */
+/* GSB_ERR_TIMEOUT when a bounded device-side wait of a token-side operator gave up on the current device
+   (the outputs of that call hold NaN where it happened), else GSB_OK.  A timeout is reported once: the
+   next call speaks of what ran after this one.  Waits for the device's queued work on every stream (not
+   allowed while a stream is captured). */
 GSB_API gsb_status gsb_token_status(void);
+/* Test hook for it: a kernel of one thread waits, as the operators do, on a barrier that nothing
+   completes, and gives up after limit_us microseconds (at most 1,000,000). */
+GSB_API gsb_status gsb_debug_token_timeout(uint32_t limit_us, void* stream);
 
 /* ---- utility: the library's radix sort on its own (tests, benchmarks) --------------------- */
 GSB_API size_t gsb_radix_sort_workspace(uint32_t n, int key_bytes, int with_values);

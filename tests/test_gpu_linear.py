@@ -603,3 +603,20 @@ def test_status_waits_for_every_stream():
     assert not done.query()
     assert _lib.lib().gsb_token_status() == _lib.GSB_OK
     assert done.query()
+
+
+def test_a_wait_that_gives_up_is_reported_once():
+    """A wait on a barrier that nothing completes gives up after 1 ms: the status reports it once, on the
+    device it happened, and the context goes on."""
+    from dynaworld_b200 import diagnostics
+
+    diagnostics.check_token_status()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        _lib.check("gsb_debug_token_timeout",
+                   _lib.lib().gsb_debug_token_timeout(1000, torch.cuda.current_stream().cuda_stream))
+    with pytest.raises(_lib.GsbError, match="TIMEOUT"):
+        diagnostics.check_token_status(DEV)
+    diagnostics.check_token_status()
+    x, w, b, r, dy = make(300, 264, 144, torch.bfloat16)
+    check(x, w, b, r, dy, "gelu")
+    diagnostics.check_token_status(torch.device(DEV))
