@@ -126,10 +126,18 @@ class TokenHeads:
         return replace(self, **parts, blocks=blocks, norm_weight=norm)
 
 
+def _walk(module):
+    """The module and what it holds, in order: one that stands in several places each time."""
+    yield module
+    for child in module._modules.values():
+        if child is not None:
+            yield from _walk(child)
+
+
 def _layers_of(mlp, name: str, activations: set) -> tuple[Layer, ...]:
     nn = torch.nn
     layers, between = [], None
-    for m in mlp.modules():
+    for m in _walk(mlp):
         if isinstance(m, nn.Linear):
             if layers and between is None:
                 raise ValueError(f"the {name} head has two linear layers with no activation between them")

@@ -28,6 +28,16 @@ def test_reads_the_module(act, name):
     assert h.rot[1].weight is m.rot_head[2].weight and h.rot[1].bias is m.rot_head[2].bias
 
 
+def test_reads_shared_modules_at_every_place():
+    """One activation object between all layers, and one layer used twice."""
+    act, mid = nn.GELU(), nn.Linear(8, 8)
+    m = Heads(rgb=nn.Sequential(nn.Linear(8, 8), act, nn.Linear(8, 8), act, nn.Linear(8, 12)),
+              xyz=nn.Sequential(nn.Sequential(mid, nn.GELU()), mid, act, nn.Linear(8, 12)))
+    h = TokenHeads.from_heads(m)
+    assert all(layer.weight is m.rgb_head[i].weight for layer, i in zip(h.rgb, (0, 2, 4))) and len(h.rgb) == 3
+    assert len(h.xyz) == 3 and h.xyz[0].weight is h.xyz[1].weight is mid.weight
+
+
 @pytest.mark.parametrize("match, make", [
     ("no activation between", lambda: Heads(rgb=nn.Sequential(nn.Linear(8, 8), nn.Linear(8, 12)))),
     ("starts with an activation", lambda: Heads(rgb=nn.Sequential(nn.GELU(), nn.Linear(8, 12)))),
