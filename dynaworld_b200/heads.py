@@ -16,6 +16,7 @@ from __future__ import annotations
 from dataclasses import dataclass, replace
 
 import torch
+import torch.nn.functional as F
 
 from . import _lib
 from .linear import linear, linear_fp8
@@ -102,7 +103,8 @@ class TokenHeads:
     def from_heads(cls, heads, *, norm_weight=None, blocks=(), eps: float = 1e-6) -> "TokenHeads":
         """Reads a GaussianParameterHeads-like module: its five ``*_head`` MLPs (torch.nn.Linear layers
         with one kind of activation between them) and its activation constants.  The parameters are
-        shared, not copied."""
+        shared, not copied.  An MLP class with a forward of its own is run once on four rows and refused
+        where that differs from its layers one after the other."""
         activations = set()
         parts = {name: _layers_of(getattr(heads, f"{name}_head"), name, activations) for name in HEAD_CHANNELS}
         if len(activations) > 1:
@@ -134,33 +136,62 @@ def _walk(module):
             yield from _walk(child)
 
 
+def _plain(m, kind) -> bool:
+    """Whether m computes what torch's class does (no forward of its own)."""
+    return isinstance(m, kind) and type(m).forward is kind.forward
+
+
 def _layers_of(mlp, name: str, activations: set) -> tuple[Layer, ...]:
     nn = torch.nn
-    layers, between = [], None
+    layers, between, acts, own_forward = [], None, [], False
     for m in _walk(mlp):
-        if isinstance(m, nn.Linear):
+        if m._forward_hooks or m._forward_pre_hooks:
+            raise ValueError(f"the {name} head holds a {type(m).__name__} with forward hooks, which would not run here")
+        if _plain(m, nn.Linear) and not m._modules:
             if layers and between is None:
                 raise ValueError(f"the {name} head has two linear layers with no activation between them")
             if between is not None and not layers:
                 raise ValueError(f"the {name} head starts with an activation")
             layers.append(Layer(m.weight, m.bias))
             if between is not None:
-                activations.add(between)
+                acts.append(between)
             between = None
-        elif isinstance(m, (nn.GELU, nn.SiLU, nn.ReLU)):
+        elif _plain(m, nn.GELU) or _plain(m, nn.SiLU) or _plain(m, nn.ReLU):
             if between is not None:
                 raise ValueError(f"the {name} head has two activations in a row")
             if isinstance(m, nn.GELU):
                 between = "gelu" if m.approximate == "none" else "gelu_tanh"
             else:
                 between = "silu" if isinstance(m, nn.SiLU) else "relu"
-        elif not isinstance(m, (nn.Identity, nn.Dropout)) and not list(m.children()):
+        elif isinstance(m, nn.Dropout):
+            if m.training and m.p > 0:
+                raise ValueError(f"the {name} head holds an active dropout, which has no kernel here")
+        elif m._modules and not isinstance(m, nn.Linear):
+            if next(m.parameters(recurse=False), None) is not None or next(m.buffers(recurse=False), None) is not None:
+                raise ValueError(f"the {name} head holds a {type(m).__name__} with parameters of its own")
+            own_forward |= not _plain(m, nn.Sequential)
+        elif not isinstance(m, nn.Identity):
             raise ValueError(f"the {name} head holds a {type(m).__name__}, which has no kernel here")
-        elif isinstance(m, nn.Dropout) and m.training and m.p > 0:
-            raise ValueError(f"the {name} head holds an active dropout, which has no kernel here")
     if not layers or between is not None:
         raise ValueError(f"the {name} head must end in a linear layer")
+    if own_forward and not _is_chain(mlp, layers, acts):
+        raise ValueError(f"the {name} head ({type(mlp).__name__}) computes something else than its layers one after "
+                         "the other")
+    activations.update(acts)
     return tuple(layers)
+
+
+@torch.no_grad()
+def _is_chain(mlp, layers, acts) -> bool:
+    """Whether a module with a forward of its own gives on a few rows what its layers give one after the
+    other (a skip, a scale or another order does not show in what it holds)."""
+    fn = {"gelu": F.gelu, "gelu_tanh": lambda v: F.gelu(v, approximate="tanh"), "silu": F.silu, "relu": F.relu}
+    w = layers[0].weight
+    x = (2 * torch.sin(torch.arange(1.0, 4 * w.shape[1] + 1))).view(1, 4, w.shape[1]).to(w)
+    got, ref = mlp(x), F.linear(x, w, layers[0].bias)
+    for act, layer in zip(acts, layers[1:]):
+        ref = F.linear(fn[act](ref), layer.weight, layer.bias)
+    return got.shape == ref.shape and float((got - ref).norm()) <= 64 * torch.finfo(w.dtype).eps * float(ref.norm())
 
 
 def _mlp(x, layers, activation):

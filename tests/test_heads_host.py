@@ -54,6 +54,61 @@ def test_refused_modules(match, make):
         TokenHeads.from_heads(make())
 
 
+class Wrapped(nn.Module):
+    """An MLP class of its own around the layers; `how` is what its forward makes of them."""
+
+    def __init__(self, how, *layers):
+        super().__init__()
+        self.net, self.how = nn.Sequential(*layers), how
+
+    def forward(self, x):
+        return self.how(self.net, x)
+
+
+class Scaled(nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class Gated(Wrapped):
+    def __init__(self, *args):
+        super().__init__(*args)
+        self.gate = nn.Parameter(torch.zeros(12))
+
+
+def layers(first=8):
+    return nn.Linear(first, 8), nn.GELU(), nn.Linear(8, 12)
+
+
+def hooked():
+    m = nn.Sequential(*layers())
+    m[0].register_forward_hook(lambda mod, args, out: 2 * out)
+    return m
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_reads_a_class_that_runs_its_layers(dtype):
+    m = Heads(rgb=Wrapped(lambda net, x: net(x), *layers()), xyz=Wrapped(lambda net, x: net(x) + 0, nn.Linear(8, 12))).to(dtype)
+    h = TokenHeads.from_heads(m)
+    assert h.rgb[1].weight is m.rgb_head.net[2].weight and len(h.xyz) == 1
+
+
+@pytest.mark.parametrize("match, make", [
+    ("something else", lambda: Wrapped(lambda net, x: 0.5 * net(x), *layers())),
+    ("something else", lambda: Wrapped(lambda net, x: net(x) + x[..., :1], *layers())),
+    ("something else", lambda: Wrapped(lambda net, x: net(torch.tanh(x)), *layers())),
+    ("something else", lambda: Wrapped(lambda net, x: net(x)[..., :6], *layers())),
+    ("something else", lambda: nn.Sequential(Wrapped(lambda net, x: net(x) + x, nn.Linear(8, 8)), nn.GELU(), nn.Linear(8, 12))),
+    ("parameters of its own", lambda: Gated(lambda net, x: net(x), *layers())),
+    ("holds a Scaled", lambda: nn.Sequential(nn.Linear(8, 8), nn.GELU(), Scaled(8, 12))),
+    ("forward hooks", hooked),
+    ("which has no kernel", lambda: nn.utils.parametrizations.weight_norm(nn.Linear(8, 12))),
+])
+def test_refuses_what_is_no_chain(match, make):
+    with pytest.raises(ValueError, match=match):
+        TokenHeads.from_heads(Heads(rgb=make()))
+
+
 def test_refused_arguments():
     layers = {n: (Layer(torch.zeros(c, 8)),) for n, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1),
                                                          ("rgb", 3))}
