@@ -109,6 +109,9 @@ class TokenHeads:
         parts = {name: _layers_of(getattr(heads, f"{name}_head"), name, activations) for name in HEAD_CHANNELS}
         if len(activations) > 1:
             raise ValueError(f"the head MLPs use different activations: {sorted(activations)}")
+        if blocks and not activations:
+            raise ValueError("the feed-forward blocks take the head MLPs' activation, and these heads have none: build "
+                             "TokenHeads with the activation named")
         return cls(**parts, head=HeadActivation.from_heads(heads), activation=next(iter(activations), "none"),
                    norm_weight=norm_weight, blocks=tuple(blocks), eps=eps)
 

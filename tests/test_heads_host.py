@@ -109,6 +109,17 @@ def test_refuses_what_is_no_chain(match, make):
         TokenHeads.from_heads(Heads(rgb=make()))
 
 
+def test_blocks_need_an_activation_to_take():
+    """Heads of one layer have no activation between layers: the blocks would run without any."""
+    single = {n: nn.Linear(8, c) for n, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1), ("rgb", 3))}
+    block = FeedForward(torch.ones(8), Layer(torch.zeros(16, 8)), Layer(torch.zeros(8, 16)))
+    with pytest.raises(ValueError, match="activation named"):
+        TokenHeads.from_heads(Heads(**single), blocks=(block,))
+    h = TokenHeads.from_heads(Heads(**single))
+    named = TokenHeads(h.xyz, h.scale, h.rot, h.opacity, h.rgb, head=h.head, activation="silu", blocks=(block,))
+    assert named.activation == "silu" and h.activation == "none"
+
+
 def test_refused_arguments():
     layers = {n: (Layer(torch.zeros(c, 8)),) for n, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1),
                                                          ("rgb", 3))}
