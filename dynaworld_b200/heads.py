@@ -249,7 +249,8 @@ def head_outputs(tokens: torch.Tensor, heads: TokenHeads, *, residual: torch.Ten
         elif add is not None:
             h = h + add
         outs = [_mlp(h, getattr(heads, n), heads.activation) for n in HEAD_CHANNELS]
-    return tuple(o.reshape(h.shape[0], -1, c) for o, c in zip(outs, HEAD_CHANNELS.values()))
+    sets, count = tokens.shape[0], tokens.shape[1] * heads.gaussians_per_token
+    return tuple(o.reshape(sets, count, c) for o, c in zip(outs, HEAD_CHANNELS.values()))
 
 
 def render_b200_tokens(tokens: torch.Tensor, heads: TokenHeads, *, residual: torch.Tensor | None = None, **render):

@@ -186,3 +186,18 @@ def test_stages_are_traced():
         render.STAGE_EVENTS = None
     assert names.count("rms_norm") == names.count("rms_norm_bwd") == 2
     assert names.count("linear") == names.count("linear_bwd") == 12
+
+
+@pytest.mark.parametrize("sets,tokens", [(0, 5), (2, 0), (0, 0)])
+def test_no_tokens(sets, tokens):
+    """Empty batches keep their shapes, forward and backward and in 8 bits."""
+    heads = make(torch.float32)
+    t = torch.zeros(sets, tokens, 72, device=DEV, requires_grad=True)
+    outs = head_outputs(t, heads, residual=torch.zeros_like(t))
+    for o, c in zip(outs, HEAD_CHANNELS.values()):
+        assert o.shape == (sets, tokens * 4, c)
+    sum(o.sum() for o in outs).backward()
+    assert t.grad.shape == t.shape and bool((heads.xyz[0].weight.grad == 0).all())
+    with torch.no_grad():
+        for o, c in zip(head_outputs(t, heads.quantized()), HEAD_CHANNELS.values()):
+            assert o.shape == (sets, tokens * 4, c)
