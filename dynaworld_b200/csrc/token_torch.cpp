@@ -145,11 +145,15 @@ void refuse_grad(const char* what, const T&... t) {
 Tensor rows_of(const Tensor& t, int64_t width) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, width});
   if ((r.stride(1) != 1 && width > 1) || (r.stride(0) < 1 && r.size(0) > 1)) r = r.contiguous();
-  return r;
+  return r.is_neg() ? r.resolve_neg() : r;  // a view may stand for the negative of what its memory holds
 }
 OptTensor rows_of(const OptTensor& t, int64_t width) {
   return t ? OptTensor(rows_of(*t, width)) : std::nullopt;
 }
+
+// [n] with adjacent elements.
+Tensor line_of(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
+OptTensor line_of(const OptTensor& t) { return t ? OptTensor(line_of(*t)) : std::nullopt; }
 
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* address(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
@@ -283,7 +287,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
   refuse_tangent("linear", x, weight, bias, residual);
   check_device("linear", x);
   const Tensor x2 = rows_of(x, x.size(-1)), w2 = rows_of(weight, weight.size(1));
-  const OptTensor r2 = rows_of(residual, n), b = bias ? OptTensor(bias->contiguous()) : std::nullopt;
+  const OptTensor r2 = rows_of(residual, n), b = line_of(bias);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual))) {
     const Tensor y = LinearNode::apply(x2, w2, b, r2, int64_t(act), int64_t(code), traced);
@@ -314,8 +318,8 @@ Tensor linear_fp8(const Tensor& x, const Tensor& x_scale, const Tensor& weight, 
   check_device(what, x);
   refuse_grad(what, x_scale, weight_scale, bias, residual);
   const Tensor x2 = rows_of(x, x.size(-1)), w2 = rows_of(weight, weight.size(1));
-  const OptTensor r2 = rows_of(residual, n), b = bias ? OptTensor(bias->contiguous()) : std::nullopt;
-  const Tensor xs = x_scale.contiguous(), ws = weight_scale.contiguous();
+  const OptTensor r2 = rows_of(residual, n), b = line_of(bias);
+  const Tensor xs = line_of(x_scale), ws = line_of(weight_scale);
   gsb_linear p = linear_spec(x2, w2, b, r2, act, GSB_E4M3, out_code);
   p.x_scale = static_cast<const float*>(address(xs));
   p.weight_scale = static_cast<const float*>(address(ws));
@@ -410,7 +414,7 @@ int check_norm(const char* what, const Tensor& x, const OptTensor& weight, const
 py::object rms_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, bool traced) {
   const int code = check_norm("rms_norm", x, weight, residual, eps);
   const int64_t dim = x.size(-1);
-  const Tensor x2 = rows_of(x, dim), w = weight.contiguous();
+  const Tensor x2 = rows_of(x, dim), w = line_of(weight);
   const OptTensor r2 = rows_of(residual, dim);
   Tensor y, h;
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(residual))) {
@@ -434,7 +438,7 @@ py::object rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& 
   const int code = check_norm("rms_norm_fp8", x, weight, residual, eps);
   refuse_grad("rms_norm_fp8", x, weight, residual);
   const int64_t dim = x.size(-1);
-  const Tensor x2 = rows_of(x, dim), w = weight.contiguous();
+  const Tensor x2 = rows_of(x, dim), w = line_of(weight);
   const OptTensor r2 = rows_of(residual, dim);
   const Tensor q = empty(x, x.sizes(), at::kFloat8_e4m3fn);
   const Tensor scale = empty(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);

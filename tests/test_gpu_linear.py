@@ -180,6 +180,24 @@ def test_strides_and_leading_dimensions(t):
     assert torch.equal(linear(rep, w, b)[5], linear(rep, w, b)[77])
 
 
+def test_views_that_stand_for_negatives():
+    """The imaginary part of a conjugate is a view of the parts' memory with a sign: operands, bias,
+    residual, gradient and the norm's tensors."""
+    from dynaworld_b200.norm import rms_norm
+
+    x, w, b, r, dy = (torch._neg_view(v) for v in make(20, 16, 24, torch.float32))
+    assert x.is_neg()
+    X, W, B, R, G = (v.clone().resolve_neg() for v in (x, w, b, r, dy))
+    leaf, LEAF = (v.requires_grad_(True) for v in (x.detach(), X.detach()))
+    got, ref = (linear(*v[:3], activation="silu", residual=v[3]) for v in ((leaf, w, b, r), (LEAF, W, B, R)))
+    assert torch.equal(got, ref)
+    assert torch.equal(torch.autograd.grad(got, leaf, dy)[0], torch.autograd.grad(ref, LEAF, G)[0])
+    assert torch.equal(rms_norm(x, w[0], residual=x)[0], rms_norm(X, W[0], residual=X)[0])
+    one = torch.randn(6, 1, dtype=torch.complex64, device=DEV).conj().imag
+    assert one.is_neg() and torch.equal(linear(one, torch.ones(1, 1, device=DEV)), one.clone().resolve_neg())
+    assert all(torch.equal(a.float(), c.float()) for a, c in zip(quantize_rows_fp8(x), quantize_rows_fp8(X)))
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_nothing_to_do(t):
     w = torch.ones(24, 16, dtype=t, device=DEV, requires_grad=True)
