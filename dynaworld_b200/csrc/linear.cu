@@ -505,6 +505,9 @@ gsb_status check_linear(const gsb_linear* p) {
   return GSB_OK;
 }
 
+// Workspaces hold rows that TMA and 16-byte accesses read and write.
+bool aligned16(const void* ws) { return reinterpret_cast<uintptr_t>(ws) % 16 == 0; }
+
 gsb_status check_operands(const gsb_linear* p) {
   if (!p->weight || (p->m > 0 && !p->x)) return GSB_ERR_ARG;
   if (p->dtype == GSB_E4M3 && p->m > 0 && (!p->x_scale || !p->weight_scale)) return GSB_ERR_ARG;
@@ -556,6 +559,7 @@ gsb_status linear_fwd(const gsb_linear* p, void* y, void* preact, void* ws, size
   }
   const FwdSpace s = fwd_space(*p, ws, ws_bytes);
   if (s.bytes && (!ws || ws_bytes < s.bytes)) return GSB_ERR_WORKSPACE;
+  if (s.bytes && !aligned16(ws)) return GSB_ERR_ARG;
   Ready x, w;
   ready_pair(job_of(p->x, p->x_stride, p->m, p->k, p->dtype, s.x),
              job_of(p->weight, p->weight_stride, p->n, p->k, p->dtype, s.w), p->dtype, x, w, st);
@@ -584,6 +588,7 @@ gsb_status linear_bwd(const gsb_linear* p, const void* preact, const void* dy, i
   if (!dy || (p->activation != GSB_ACT_NONE && !preact)) return GSB_ERR_ARG;
   if ((dx && !p->weight) || (dweight && !p->x)) return GSB_ERR_ARG;
   if (!ws || ws_bytes < linear_bwd_workspace(p, dy, dy_stride)) return GSB_ERR_WORKSPACE;
+  if (!aligned16(ws)) return GSB_ERR_ARG;
   return bwd(*p, preact, dy, dy_stride, dx, dweight, dbias, bwd_space(*p, dy, dy_stride, ws, ws_bytes), st);
 }
 

@@ -458,6 +458,7 @@ typedef struct gsb_linear {
   const float* weight_scale;
 } gsb_linear;
 
+/* Workspaces of both directions start on a 16-byte boundary (else GSB_ERR_ARG). */
 GSB_API size_t gsb_linear_fwd_workspace(const gsb_linear* linear);
 /* preact (or NULL) [m,n] keeps z = x weight^T + bias for the backward: float for F32 operands, fp16
    saturated at its largest value for 16-bit ones (every activation is flat or linear there) and, for

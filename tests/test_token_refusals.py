@@ -137,3 +137,18 @@ def test_entry_points_refuse_before_a_launch(lib):
     assert lib.gsb_linear_bwd(b, 256, 256, 8, 256, 256, 256, 256, big, None) == 7  # serving only
     p.m, p.dtype, p.x = 0, _lib.BF16, None
     assert lib.gsb_linear_fwd(b, 256, None, 256, big, None) == 0
+
+
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16, _lib.F16, _lib.E4M3])
+def test_workspaces_off_their_boundary_are_refused(lib, dtype):
+    """Rows in the workspace are read and written 16 bytes at a time: an address that allows no such access
+    gives a status before any kernel."""
+    out = _lib.BF16 if dtype == _lib.E4M3 else dtype
+    p = _lib.Linear(m=300, n=40, k=67, dtype=dtype, out_dtype=out, x=256, x_stride=67, weight=256, weight_stride=67,
+                    x_scale=256, weight_scale=256)
+    b = ctypes.byref(p)
+    assert lib.gsb_linear_fwd_workspace(b) > 0
+    for ws in (264, 260, 257):
+        assert lib.gsb_linear_fwd(b, 256, None, ws, 1 << 30, None) == 7
+        if dtype != _lib.E4M3:
+            assert lib.gsb_linear_bwd(b, None, 256, 40, 256, 256, 256, ws, 1 << 30, None) == 7
