@@ -1,10 +1,12 @@
 // Activations of the matrix product's epilogue and their derivatives, in float.
 //
 // They are evaluated for every value of a tile between two tiles' products, so instructions count:
-// one exponential and one reciprocal each.  The normal distribution function follows Abramowitz
-// and Stegun, Handbook of Mathematical Functions, 7.1.26 (erf within 1.5e-7), whose exponential
-// is the density's own; the tanh form of GELU is z sigmoid(2 u).  With the erff / expf / divide
-// forms the bf16 product of 16384 x 1024 x 4096 with GELU took 218 us and dz 136 us.
+// one exponential and one reciprocal each.  The normal distribution function is the density's own
+// exponential times a polynomial in t = 1 / (1 + c |z|): for 16-bit outputs Abramowitz and Stegun, Handbook
+// of Mathematical Functions, 7.1.26 (erf within 1.5e-7, which in the tail is 5e-5 of the value at z = -3),
+// for float outputs (FINE) three degrees more of the same form.  The tanh form of GELU is z sigmoid(2 u).
+// With the erff / expf / divide forms the bf16 product of 16384 x 1024 x 4096 with GELU took 218 us and dz
+// 136 us.
 #pragma once
 
 #include "gsb200.h"
@@ -61,14 +63,28 @@ __device__ __forceinline__ F2 each(F2 a, F f) {
 __device__ __forceinline__ F2 exp2_2(F2 a) { return each(a, [](float x) { return fast_exp2(x); }); }
 __device__ __forceinline__ F2 rcp_2(F2 a) { return each(a, [](float x) { return fast_rcp(x); }); }
 
-// -|z|, Phi(-|z|) and exp(-z^2 / 2): 7.1.26 with its coefficients halved, its argument |z| / sqrt(2).
+// -|z|, Phi(-|z|) and exp(-z^2 / 2).  7.1.26 with its coefficients halved, its argument |z| / sqrt(2).
+// FINE: minimax fit of Phi(-a) / (t exp(-a^2 / 2)) over a <= 13.5 (where the exponential leaves float's
+// range) by its relative error, 9.4e-8, with the c that a search found best for the degree.
+template <bool FINE>
 __device__ __forceinline__ F2 normal_tail(F2 z, F2& minus, F2& gauss) {
   minus = each(z, [](float x) { return __int_as_float(__float_as_int(x) | 0x80000000); });
-  const F2 t = rcp_2(fma2(F2(-0.3275911f * 0.70710678118654752f), minus, F2(1.0f)));
-  F2 p = fma2(F2(0.5f * 1.061405429f), t, F2(0.5f * -1.453152027f));
-  p = fma2(p, t, F2(0.5f * 1.421413741f));
-  p = fma2(p, t, F2(0.5f * -0.284496736f));
-  p = fma2(p, t, F2(0.5f * 0.254829592f));
+  const F2 t = rcp_2(fma2(F2(FINE ? -0.305f : -0.3275911f * 0.70710678118654752f), minus, F2(1.0f)));
+  F2 p;
+  if constexpr (FINE) {
+    p = fma2(F2(0.0366991855f), t, F2(-0.1529882908f));
+    p = fma2(p, t, F2(0.1857168636f));
+    p = fma2(p, t, F2(-0.0379767906f));
+    p = fma2(p, t, F2(0.1210216580f));
+    p = fma2(p, t, F2(0.1034208725f));
+    p = fma2(p, t, F2(0.1224668160f));
+    p = fma2(p, t, F2(0.1216397327f));
+  } else {
+    p = fma2(F2(0.5f * 1.061405429f), t, F2(0.5f * -1.453152027f));
+    p = fma2(p, t, F2(0.5f * 1.421413741f));
+    p = fma2(p, t, F2(0.5f * -0.284496736f));
+    p = fma2(p, t, F2(0.5f * 0.254829592f));
+  }
   gauss = exp2_2(mul2(mul2(z, z), F2(-0.5f * kLog2E)));
   return mul2(mul2(p, t), gauss);
 }
@@ -81,7 +97,7 @@ __device__ __forceinline__ F2 gelu_tanh_arg(F2 z, F2 zz) {
 }
 
 // ReLU passes a NaN on, as torch does.
-template <int ACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ F2 act_value(F2 z) {
   if constexpr (ACT == GSB_ACT_RELU) {
     return each(z, [](float x) { return x < 0.0f ? 0.0f : x; });
@@ -89,7 +105,7 @@ __device__ __forceinline__ F2 act_value(F2 z) {
     // z Phi(z) = max(z, 0) - |z| Phi(-|z|), whose second term is 0 from z = 15 on: there |z| ends at 1e4, so
     // that +infinity does not meet that 0 (-infinity does: NaN, as z Phi(z) is)
     F2 minus, gauss;
-    const F2 tail = normal_tail(each(z, [](float x) { return fminf(x, 1e4f); }), minus, gauss);
+    const F2 tail = normal_tail<FINE>(each(z, [](float x) { return fminf(x, 1e4f); }), minus, gauss);
     return fma2(minus, tail, each(z, [](float x) { return fmaxf(x, 0.0f); }));
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
     return mul2(z, sigmoid_of(gelu_tanh_arg(z, mul2(z, z))));
@@ -100,18 +116,25 @@ __device__ __forceinline__ F2 act_value(F2 z) {
   }
 }
 
-template <int ACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ F2 act_slope(F2 z) {
   if constexpr (ACT == GSB_ACT_RELU) {
     return each(z, [](float x) { return x <= 0.0f ? 0.0f : 1.0f; });
   } else if constexpr (ACT == GSB_ACT_GELU) {
     F2 minus, gauss;
-    const F2 tail = normal_tail(z, minus, gauss);
-    // Phi(z) = 1/2 + (1/2 - Phi(-|z|)) with the sign of z
+    const F2 tail = normal_tail<FINE>(z, minus, gauss);
     float z0, z1, h0, h1;
     z.get(z0, z1);
-    fma2(tail, F2(-1.0f), F2(0.5f)).get(h0, h1);
-    const F2 cdf = add2(F2(copysignf(h0, z0), copysignf(h1, z1)), F2(0.5f));
+    F2 cdf;
+    if constexpr (FINE) {
+      float t0, t1;
+      tail.get(t0, t1);
+      fma2(tail, F2(-1.0f), F2(1.0f)).get(h0, h1);
+      cdf = F2(z0 < 0.0f ? t0 : h0, z1 < 0.0f ? t1 : h1);
+    } else {  // Phi(z) = 1/2 + (1/2 - Phi(-|z|)) with the sign of z
+      fma2(tail, F2(-1.0f), F2(0.5f)).get(h0, h1);
+      cdf = add2(F2(copysignf(h0, z0), copysignf(h1, z1)), F2(0.5f));
+    }
     return fma2(mul2(z, F2(kInvSqrt2Pi)), gauss, cdf);
   } else if constexpr (ACT == GSB_ACT_GELU_TANH) {
     const F2 zz = mul2(z, z);
@@ -128,25 +151,27 @@ __device__ __forceinline__ F2 act_slope(F2 z) {
   }
 }
 
-// V values at once.
-template <int ACT, int V>
+// V values at once, for outputs of type O.
+template <int ACT, typename O, int V>
 __device__ __forceinline__ void apply_value(float (&z)[V]) {
+  constexpr bool FINE = sizeof(O) == 4;
   if constexpr (ACT != GSB_ACT_NONE) {
 #pragma unroll
     for (int u = 0; u < V; u += 2) {
       float unused;
-      if (u + 1 < V) act_value<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
-      else act_value<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
+      if (u + 1 < V) act_value<ACT, FINE>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
+      else act_value<ACT, FINE>(F2(z[u], 0.0f)).get(z[u], unused);
     }
   }
 }
-template <int ACT, int V>
+template <int ACT, typename O, int V>
 __device__ __forceinline__ void apply_slope(float (&z)[V]) {
+  constexpr bool FINE = sizeof(O) == 4;
 #pragma unroll
   for (int u = 0; u < V; u += 2) {
     float unused;
-    if (u + 1 < V) act_slope<ACT>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
-    else act_slope<ACT>(F2(z[u], 0.0f)).get(z[u], unused);
+    if (u + 1 < V) act_slope<ACT, FINE>(F2(z[u], z[u + 1])).get(z[u], z[u + 1]);
+    else act_slope<ACT, FINE>(F2(z[u], 0.0f)).get(z[u], unused);
   }
 }
 

@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256, 4)
         float slope[V];
 #pragma unroll
         for (int u = 0; u < V; ++u) slope[u] = to_f32(at.v[u]);
-        apply_slope<ACT, V>(slope);
+        apply_slope<ACT, T, V>(slope);
 #pragma unroll
         for (int u = 0; u < V; ++u) v[u] = __fmul_rn(v[u], slope[u]);
       }

@@ -250,10 +250,10 @@ __device__ __forceinline__ bool is_relu(const Job& p) {
   return (ACT == kAnyAct ? p.e.act : ACT) == GSB_ACT_RELU;
 }
 
-template <int ACT, int V>
+template <int ACT, typename O, int V>
 __device__ __forceinline__ void activate(const Job& p, float (&z)[V]) {
-  if constexpr (ACT == kAnyAct) apply_act<V>(p.e.act, z);
-  else apply_value<ACT, V>(z);
+  if constexpr (ACT == kAnyAct) apply_act<O, V>(p.e.act, z);
+  else apply_value<ACT, O, V>(z);
 }
 
 // VEC: the output's rows (and the residual's, bias, kept sums) allow accesses of 16 bytes.
@@ -357,7 +357,7 @@ struct Rows {
                 *reinterpret_cast<Vec<Z, V>*>(keep + (s0 + h) * kAtOnce * p.n) =
                     kept_of<V>(static_cast<Z*>(nullptr), reinterpret_cast<const float(&)[V]>(z[h * V]), is_relu<ACT>(p));
           }
-          activate<ACT, 2 * V>(p, z);
+          activate<ACT, O, 2 * V>(p, z);
           if (p.e.res) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -402,7 +402,7 @@ struct Rows {
             for (int r = 0; r < 8; ++r)
               if (r0 + r < rows) keep[(r0 + r) * p.n] = as_preact(static_cast<Z*>(nullptr), z[r], is_relu<ACT>(p));
           }
-          activate<ACT, 8>(p, z);
+          activate<ACT, O, 8>(p, z);
           if (p.e.res) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) z[r] += to_f32(add[r0 + r]);

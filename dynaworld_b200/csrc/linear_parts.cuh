@@ -60,13 +60,13 @@ struct PreactOf { using type = f16; };
 template <>
 struct PreactOf<float> { using type = float; };
 
-template <int V>
+template <typename O, int V>
 __device__ __forceinline__ void apply_act(int act, float (&z)[V]) {
   switch (act) {
-    case GSB_ACT_RELU: apply_value<GSB_ACT_RELU, V>(z); break;
-    case GSB_ACT_GELU: apply_value<GSB_ACT_GELU, V>(z); break;
-    case GSB_ACT_GELU_TANH: apply_value<GSB_ACT_GELU_TANH, V>(z); break;
-    case GSB_ACT_SILU: apply_value<GSB_ACT_SILU, V>(z); break;
+    case GSB_ACT_RELU: apply_value<GSB_ACT_RELU, O, V>(z); break;
+    case GSB_ACT_GELU: apply_value<GSB_ACT_GELU, O, V>(z); break;
+    case GSB_ACT_GELU_TANH: apply_value<GSB_ACT_GELU_TANH, O, V>(z); break;
+    case GSB_ACT_SILU: apply_value<GSB_ACT_SILU, O, V>(z); break;
     default: break;
   }
 }
@@ -113,7 +113,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t n, int64_t i, 
     *reinterpret_cast<Vec<Z, V>*>(static_cast<Z*>(e.preact) + i * n + j) =
         kept_of<V>(static_cast<Z*>(nullptr), z, e.act == GSB_ACT_RELU);
   }
-  apply_act<V>(e.act, z);
+  apply_act<O, V>(e.act, z);
   if (e.res) {
     float r[V];
     load_f32<O, V>(static_cast<const O*>(e.res) + i * e.res_stride + j, r);

@@ -261,6 +261,24 @@ def test_infinite_preactivations(m, k, act, t):
     assert same_kind(y, ref.repeat(256).expand(m, 512)), y[0, :2]
 
 
+def test_gelu_in_float32():
+    """GELU and its slope over |z| <= 12 to float's accuracy, the tail's relative one included.  Phi(-|z|)
+    and the density carry: the fit (2^-23), 8 steps of the polynomial whose terms' magnitudes are at most
+    1.8 times its value (8 x 1.8 x 2^-24), the reciprocal (2^-23 times t's weight, at most 2.5), the
+    exponential (2^-22) and three products: 2^-19 in all, and the exponent's roundings, z^2 2^-23.  The sums
+    around them round once each (2^-23)."""
+    z = torch.linspace(-12, 12, 40001, device=DEV, dtype=torch.float64).float()[:, None].requires_grad_(True)
+    y = linear(z, torch.ones(1, 1, device=DEV), activation="gelu")  # z itself is exact: one product with 1
+    (slope,) = torch.autograd.grad(y.sum(), z)
+    Z = z.detach().double()
+    ref, ref_slope = act64(Z, "gelu")
+    tail = 0.5 * torch.special.erfc(Z.abs() / math.sqrt(2))
+    gauss = torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi)
+    rel = 2.0 ** -19 + Z * Z * U
+    within(y, ref, Z.abs() * tail * rel + ref.abs() * U + 1e-37, "y")
+    within(slope, ref_slope, (tail + Z.abs() * gauss) * rel + ref_slope.abs() * U + 1e-37, "slope")
+
+
 def test_large_values_in_float32():
     """Values near the type's largest, whose bf16 rounding would overflow."""
     x = torch.full((130, 64), 0.0, device=DEV)
