@@ -261,6 +261,36 @@ def test_infinite_preactivations(m, k, act, t):
     assert same_kind(y, ref.repeat(256).expand(m, 512)), y[0, :2]
 
 
+def bf16_parts(v):
+    """v (float32) as three bf16 values, in 64 bits."""
+    out = []
+    for _ in range(3):
+        out.append(v.bfloat16())
+        v = v - out[-1].float()
+    return [p.double() for p in out]
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 64), (9, 64, 40), (65, 64, 64), (127, 129, 255), (129, 136, 264),
+                                   (300, 771, 1285), (1025, 512, 130), (257, 1037, 9), (700, 520, 1032),
+                                   (4100, 264, 520), (20000, 64, 72), (100, 4100, 512), (300, 4096, 1024)])
+def test_float32_products_are_as_exact_as_float32_sums(m, k, n):
+    """In norm: four steps of float (2^-24) for the split operands, the tensor core's chain over 64 of K and
+    the last rounding, and one more per addition of such a chain's sum, whose roundings add up as their root.
+    Products without the parts' small cross terms are past that bound, so it holds the split to all six."""
+    x, w, _, _, dy = make(m, k, n, torch.float32, seed=m + n)
+    leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+    y = linear(*leaves)
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    for got, a, b in ((y, x, w.T), (dx, dy, w), (dw, dy.T, x)):
+        ref = a.double() @ b.double()
+        bound = 2.0 ** -24 * (4 + math.sqrt(a.shape[1] / 64))
+        assert float((got.double() - ref).norm() / ref.norm()) <= bound
+        if min(got.shape) > 1 and a.shape[1] > 16:
+            (a1, a2, a3), (b1, b2, b3) = bf16_parts(a), bf16_parts(b)
+            for lost in (a1 @ b3 + a3 @ b1, a2 @ b2, a1 @ b3):
+                assert float(lost.norm() / ref.norm()) > bound
+
+
 def test_gelu_in_float32():
     """GELU and its slope over |z| <= 12 to float's accuracy, the tail's relative one included.  Phi(-|z|)
     and the density carry: the fit (2^-23), 8 steps of the polynomial whose terms' magnitudes are at most
