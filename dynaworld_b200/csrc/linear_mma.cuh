@@ -121,8 +121,11 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 // bar: an address in the cluster's shared window.  Relaxed: what the arrival hands over is TMEM that has
-// been read (tcgen05.wait::ld, tcgen05.fence); a release would also wait for the warp's stores of
-// outputs, about a microsecond per tile.
+// been read, and nothing in global or shared memory, which is what a release would order.  TMEM accesses of
+// different threads are ordered by tcgen05's own rules (PTX, tcgen05 memory consistency model): the reads are
+// complete after tcgen05.wait::ld, tcgen05.fence::before_thread_sync orders them before the arrival, and the
+// waiting thread's fence::after_thread_sync orders its next MMA after the wait that saw it.  A release would
+// also wait for the warp's stores of outputs, about a microsecond per tile.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
