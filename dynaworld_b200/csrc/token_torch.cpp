@@ -314,9 +314,9 @@ Tensor linear_fp8(const Tensor& x, const Tensor& x_scale, const Tensor& weight, 
   const int64_t n = check_shapes(what, x, weight, bias, residual, type);
   check_like(what, "x_scale", x_scale, x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
   check_like(what, "weight_scale", weight_scale, {n}, at::kFloat, x);
-  refuse_tangent(what, x_scale, weight_scale, bias, residual);
+  refuse_tangent(what, x, x_scale, weight, weight_scale, bias, residual);
+  refuse_grad(what, x, x_scale, weight, weight_scale, bias, residual);
   check_device(what, x);
-  refuse_grad(what, x_scale, weight_scale, bias, residual);
   const Tensor x2 = rows_of(x, x.size(-1)), w2 = rows_of(weight, weight.size(1));
   const OptTensor r2 = rows_of(residual, n), b = line_of(bias);
   const Tensor xs = line_of(x_scale), ws = line_of(weight_scale);

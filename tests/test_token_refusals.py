@@ -85,6 +85,17 @@ def test_dual_tensors_are_refused():
         linear(F(2, 4), F(3, 4))
 
 
+def test_codes_that_want_gradients_are_refused():
+    """float8 tensors may require gradients like any floating type; the 8-bit product has none to give."""
+    x, w = F(2, 4, dtype=E4M3), F(3, 4, dtype=E4M3)
+    for call in (lambda: linear_fp8(x.clone().requires_grad_(True), F(2), w, F(3)),
+                 lambda: linear_fp8(x, F(2), w.clone().requires_grad_(True), F(3))):
+        with pytest.raises(NotImplementedError, match="not differentiable"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA devices only"):
+            call()
+
+
 @pytest.fixture(scope="module")
 def lib():
     build.build()
