@@ -4,7 +4,8 @@
 // one exponential and one reciprocal each.  The normal distribution function is the density's own
 // exponential times a polynomial in t = 1 / (1 + c |z|): for 16-bit outputs Abramowitz and Stegun, Handbook
 // of Mathematical Functions, 7.1.26 (erf within 1.5e-7, which in the tail is 5e-5 of the value at z = -3),
-// for float outputs (FINE) three degrees more of the same form.  The tanh form of GELU is z sigmoid(2 u).
+// for float outputs (FINE) three degrees more of the same form (4,096 x 512 x 2,560 float with GELU: 64 us
+// with 7.1.26, 66 so).  The tanh form of GELU is z sigmoid(2 u).
 // With the erff / expf / divide forms the bf16 product of 16384 x 1024 x 4096 with GELU took 218 us and dz
 // 136 us.
 #pragma once

@@ -18,7 +18,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
 
     x and residual [..., D], weight [D], all float32, bfloat16 or float16 of one type.  Returns y,
     or with a residual the pair (y, h): h is the new residual stream.  The sum, the statistics and
-    the product are formed in float; y and h are rounded once.  Differentiable in x, weight and
+    the product are formed in float (a row whose squares add up past float's range, 3e38, gives zeros); y
+    and h are rounded once.  Differentiable in x, weight and
     residual (once, in reverse mode; the backward forms h again from x and residual); the weight gradient is the same
     on every run."""
     return _token.ext().rms_norm(x, weight, residual, eps, _token.traced())
