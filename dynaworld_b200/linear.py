@@ -22,14 +22,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     "gelu", "gelu_tanh" (its tanh form) or "silu".
 
     Sums, bias, activation and residual are formed in float and rounded once; on the tensor cores the
-    additions of 16-bit (and e4m3) products truncate, about 2^-25 of the sum for every 16 (32) of k.  Differentiable once
-    in x, weight, bias and residual (reverse mode; tangents of forward mode are refused).  With an activation the forward keeps x weight^T + bias for the
-    backward (float beside float32 operands, else float16), and the backward rounds
-    dy act'(z) to the operands' type before its two products.  The same inputs give the same bits.
-    Rows may lie apart (any row stride); other layouts are copied.  float32 products of more than 8
-    rows (64 with at most 8 MB of weights), and the backward's, take their operands as sums of three
-    bfloat16 parts, as exact as float32 sums; an infinity among them may give NaN.  An infinite sum
-    gives what the activation's formula gives (-infinity: NaN with GELU and SiLU, 0 with ReLU)."""
+    additions of 16-bit (and e4m3) products truncate, about 2^-25 of the sum for every 16 (32) of k.
+    Differentiable once in x, weight, bias and residual (reverse mode; tangents of forward mode are
+    refused).  With an activation the forward keeps x weight^T + bias for the backward (float beside
+    float32 operands, else float16), and the backward rounds dy act'(z) to the operands' type before its
+    two products.  The same inputs give the same bits.  Rows may lie apart (any row stride); other
+    layouts are copied.  float32 products of more than 8 rows (64 with at most 8 MB of weights), and the
+    backward's, take their operands as sums of three bfloat16 parts, as exact as float32 sums; an
+    infinity among them may give NaN.  An infinite sum gives what the activation's formula gives
+    (-infinity: NaN with GELU and SiLU, 0 with ReLU)."""
     return _token.ext().linear(x, weight, bias, residual, activation, _token.traced())
 
 
