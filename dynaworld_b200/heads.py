@@ -13,6 +13,8 @@ layers in front of it run on ``rms_norm`` and ``linear`` too, and for serving on
 """
 from __future__ import annotations
 
+import copy
+import math
 from dataclasses import dataclass, replace
 
 import torch
@@ -177,7 +179,7 @@ def _layers_of(mlp, name: str, activations: set) -> tuple[Layer, ...]:
             raise ValueError(f"the {name} head holds a {type(m).__name__}, which has no kernel here")
     if not layers or between is not None:
         raise ValueError(f"the {name} head must end in a linear layer")
-    if own_forward and not _is_chain(mlp, layers, acts):
+    if own_forward and not _is_chain(mlp, acts):
         raise ValueError(f"the {name} head ({type(mlp).__name__}) computes something else than its layers one after "
                          "the other")
     activations.update(acts)
@@ -185,16 +187,26 @@ def _layers_of(mlp, name: str, activations: set) -> tuple[Layer, ...]:
 
 
 @torch.no_grad()
-def _is_chain(mlp, layers, acts) -> bool:
+def _is_chain(mlp, acts) -> bool:
     """Whether a module with a forward of its own gives on a few rows what its layers give one after the
-    other (a skip, a scale or another order does not show in what it holds)."""
+    other (a skip, a scale or another order does not show in what it holds).  On a copy with values of its
+    own in 64 bits: no rounding and no layer that starts at zero hides a difference."""
     fn = {"gelu": F.gelu, "gelu_tanh": lambda v: F.gelu(v, approximate="tanh"), "silu": F.silu, "relu": F.relu}
+
+    def wave(shape, device, phase):
+        n = torch.arange(1.0, math.prod(shape) + 1, dtype=torch.float64, device=device)
+        return torch.sin(n * n + phase).view(shape)
+
+    mlp = copy.deepcopy(mlp).double()
+    for i, p in enumerate(mlp.parameters()):
+        p.copy_(wave(p.shape, p.device, i))
+    layers = [m for m in _walk(mlp) if isinstance(m, torch.nn.Linear)]
     w = layers[0].weight
-    x = (2 * torch.sin(torch.arange(1.0, 4 * w.shape[1] + 1))).view(1, 4, w.shape[1]).to(w)
-    got, ref = mlp(x), F.linear(x, w, layers[0].bias)
-    for act, layer in zip(acts, layers[1:]):
-        ref = F.linear(fn[act](ref), layer.weight, layer.bias)
-    return got.shape == ref.shape and float((got - ref).norm()) <= 64 * torch.finfo(w.dtype).eps * float(ref.norm())
+    x = 2 * wave((1, 4, w.shape[1]), w.device, 0.5)
+    got, ref = mlp(x), x
+    for act, layer in zip([None, *acts], layers):
+        ref = F.linear(ref if act is None else fn[act](ref), layer.weight, layer.bias)
+    return got.shape == ref.shape and float((got - ref).norm()) <= 1e-9 * float(ref.norm())
 
 
 def _mlp(x, layers, activation):

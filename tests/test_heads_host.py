@@ -109,6 +109,18 @@ def test_refuses_what_is_no_chain(match, make):
         TokenHeads.from_heads(Heads(rgb=make()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [0.5, 1.01])
+def test_refuses_a_scale_that_rounding_or_zeros_would_hide(dtype, scale):
+    m = Heads(rgb=Wrapped(lambda net, x: scale * net(x), *layers())).to(dtype)
+    with pytest.raises(ValueError, match="something else"):
+        TokenHeads.from_heads(m)
+    nn.init.zeros_(m.rgb_head.net[2].weight)  # a head that starts at zero
+    nn.init.zeros_(m.rgb_head.net[2].bias)
+    with pytest.raises(ValueError, match="something else"):
+        TokenHeads.from_heads(m)
+
+
 def test_blocks_need_an_activation_to_take():
     """Heads of one layer have no activation between layers: the blocks would run without any."""
     single = {n: nn.Linear(8, c) for n, c in (("xyz", 3), ("scale", 3), ("rot", 4), ("opacity", 1), ("rgb", 3))}
