@@ -105,7 +105,7 @@ class TokenHeads:
     def from_heads(cls, heads, *, norm_weight=None, blocks=(), eps: float = 1e-6) -> "TokenHeads":
         """Reads a GaussianParameterHeads-like module: its five ``*_head`` MLPs (torch.nn.Linear layers
         with one kind of activation between them) and its activation constants.  The parameters are
-        shared, not copied.  An MLP class with a forward of its own is run once on four rows and refused
+        shared, not copied.  An MLP class with a forward of its own is run once (a copy) on four rows and refused
         where that differs from its layers one after the other."""
         activations = set()
         parts = {name: _layers_of(getattr(heads, f"{name}_head"), name, activations) for name in HEAD_CHANNELS}
