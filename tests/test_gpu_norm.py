@@ -210,6 +210,33 @@ def test_quantised_special_rows(t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim", [256, 520, 1024, 2048])
+def test_special_rows_among_many(dim, t):
+    """Rows that come through the ring of copies: a NaN, an infinity or a row of zeros stays in its row,
+    forward, in 8 bits and backward."""
+    x, r, w, dy, _ = make(9500, dim, t, seed=dim)
+    x[5], r[5] = 0, 0
+    clean = x.clone()
+    x[7, 3], x[4000, 9], x[9499, 0] = float("nan"), float("inf"), float("-inf")
+    bad = torch.tensor([7, 4000, 9499], device=DEV)
+    rest = torch.ones(9500, dtype=torch.bool, device=DEV).index_fill(0, bad, False)
+    for a, b in zip(rms_norm(x, w, residual=r), rms_norm(clean, w, residual=r)):
+        assert torch.equal(a[rest], b[rest]) and bool((a[5] == 0).all())
+    for got, ref in ((rms_norm_fp8(x, w, residual=r), rms_norm_fp8(clean, w, residual=r)),
+                     (quantize_rows_fp8(x), quantize_rows_fp8(clean))):
+        assert torch.equal(got[0].view(torch.uint8)[rest], ref[0].view(torch.uint8)[rest])
+        assert torch.equal(got[1][rest], ref[1][rest])
+        value = got[0].float() * got[1][:, None]
+        assert bool(value[bad].isnan().all()) and bool((value[5] == 0).all())
+    leaf = clean.requires_grad_(True)
+    dirty = dy.clone()
+    dirty[bad] = float("nan")
+    for a, b in zip(torch.autograd.grad(rms_norm(leaf, w, residual=r)[0], leaf, dy),
+                    torch.autograd.grad(rms_norm(leaf, w, residual=r)[0], leaf, dirty)):
+        assert torch.equal(a[rest], b[rest])
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,dim", SHAPES + [(4800, 1024), (5001, 2048), (700, 4096), (601, 16384)])
 @pytest.mark.parametrize("residual", [True, False])
 def test_norm_in_8_bits(rows, dim, t, residual):
