@@ -112,17 +112,19 @@ size_t copy_bytes(int64_t rows, int64_t cols, int dtype) {
 
 // v as a sum of three bf16 values, each the rounding of what the ones before leave: 3 x 8 bits and
 // signs hold all 24 of a float's.  A first part that would round to infinity is truncated
-// instead; infinities and NaN go to the first part alone.
+// instead.  Infinities and NaN go to the third part alone: it meets only the other operand's first part,
+// which is 0 only where that value is, while its second and third are 0 for every value exact in bf16 (and
+// infinity times 0 is NaN).  Two infinities that meet give NaN so.
 struct Parts { bf16 p[3]; };
 __device__ __forceinline__ Parts split3(float v) {
   Parts s;
-  s.p[0] = __float2bfloat16_rn(v);
-  const float top = __bfloat162float(s.p[0]);
   const bool finite = fabsf(v) <= 3.402823466e38f;
-  if (finite && fabsf(top) > 3.402823466e38f) s.p[0] = __float2bfloat16_rz(v);
-  const float rest = finite ? v - __bfloat162float(s.p[0]) : 0.0f;
+  const float f = finite ? v : 0.0f;
+  s.p[0] = __float2bfloat16_rn(f);
+  if (fabsf(__bfloat162float(s.p[0])) > 3.402823466e38f) s.p[0] = __float2bfloat16_rz(f);
+  const float rest = f - __bfloat162float(s.p[0]);
   s.p[1] = __float2bfloat16_rn(rest);
-  s.p[2] = __float2bfloat16_rn(rest - __bfloat162float(s.p[1]));
+  s.p[2] = __float2bfloat16_rn(finite ? rest - __bfloat162float(s.p[1]) : v);
   return s;
 }
 

@@ -28,8 +28,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     float32 operands, else float16), and the backward rounds dy act'(z) to the operands' type before its
     two products.  The same inputs give the same bits.  Rows may lie apart (any row stride); other
     layouts are copied.  float32 products of more than 8 rows (64 with at most 8 MB of weights), and the
-    backward's, take their operands as sums of three bfloat16 parts, as exact as float32 sums; an
-    infinity among them may give NaN.  An infinite sum gives what the activation's formula gives
+    backward's, take their operands as sums of three bfloat16 parts, as exact as float32 sums (two
+    infinities multiplied give NaN there).  An infinite sum gives what the activation's formula gives
     (-infinity: NaN with GELU and SiLU, 0 with ReLU)."""
     return _token.ext().linear(x, weight, bias, residual, activation, _token.traced())
 

@@ -309,6 +309,34 @@ def test_gelu_in_float32():
     within(slope, ref_slope, (tail + Z.abs() * gauss) * rel + ref_slope.abs() * U + 1e-37, "slope")
 
 
+@pytest.mark.parametrize("m,k,n", [(3, 64, 40), (130, 64, 72), (130, 67, 41), (300, 512, 264), (100, 4096, 512)])
+def test_infinities_in_float32(m, k, n):
+    """Infinite operands give what sums of float products give, however many rows there are: an infinity of
+    the factors' sign, NaN where it meets a zero or the other infinity; everything else is untouched."""
+    x, w, _, _, dy = make(m, k, n, torch.float32, seed=m)
+    w[::2] = w[::2].bfloat16().float()  # values whose second and third part are 0
+    w[5, 3] = 0
+    x[1, 3], x[2, 7], x[2, 9], dy[0, 6] = math.inf, -math.inf, math.inf, -math.inf
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    y = linear(*leaves)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    X, W, G = x.detach().double(), w.detach().double(), dy.double()
+
+    def product(a, b):
+        """a b^T with the terms of infinities counted one by one."""
+        fa, fb = a.nan_to_num(0, 0, 0), b.nan_to_num(0, 0, 0)
+        out = fa @ fb.T
+        for c in torch.nonzero(a.isinf().any(0) | b.isinf().any(0)).flatten().tolist():
+            out = out + a[:, c, None] * b[None, :, c] - fa[:, c, None] * fb[None, :, c]
+        return out, (fa.abs() @ fb.abs().T) * ((a.shape[1] + 2) * U)
+
+    for what, v, (ref, bound) in zip(("y", "dx", "dw"), got, (product(X, W), product(G, W.T), product(G.T, X.T))):
+        kind = ~torch.isfinite(ref)
+        assert same_kind(v.double()[kind], ref[kind]), what
+        within(v[~kind], ref[~kind], ref[~kind].abs() * half(torch.float32) + bound[~kind], what)
+        assert 0 < int(kind.sum()) < kind.numel()
+
+
 def test_large_values_in_float32():
     """Values near the type's largest, whose bf16 rounding would overflow."""
     x = torch.full((130, 64), 0.0, device=DEV)
