@@ -180,6 +180,19 @@ def test_strides_and_leading_dimensions(t):
     assert torch.equal(linear(rep, w, b)[5], linear(rep, w, b)[77])
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_rows_that_overlap(m, t):
+    """Windows over one line of values: rows whose distance is less than their length."""
+    line = torch.randn(8 * m + 64, generator=torch.Generator().manual_seed(m)).to(DEV, t)
+    x, w = line.as_strided((m, 64), (8, 1)), line.as_strided((min(m, 40), 64), (8, 1))
+    dy = torch.ones(m, w.shape[0], dtype=t, device=DEV)
+    got, ref = [x.detach().requires_grad_(True), w.detach()], [x.contiguous().requires_grad_(True), w.contiguous()]
+    a, b = (linear(*v, activation="silu") for v in (got, ref))
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, got[0], dy)[0], torch.autograd.grad(b, ref[0], dy)[0])
+
+
 def test_views_that_stand_for_negatives():
     """The imaginary part of a conjugate is a view of the parts' memory with a sign: operands, bias,
     residual, gradient and the norm's tensors."""
