@@ -297,7 +297,7 @@ def test_float32_products_are_as_exact_as_float32_sums(m, k, n):
     for got, a, b in ((y, x, w.T), (dx, dy, w), (dw, dy.T, x)):
         ref = a.double() @ b.double()
         bound = 2.0 ** -24 * (4 + math.sqrt(a.shape[1] / 64))
-        assert float((got.double() - ref).norm() / ref.norm()) <= bound
+        assert float((got.detach().double() - ref).norm() / ref.norm()) <= bound
         if min(got.shape) > 1 and a.shape[1] > 16:
             (a1, a2, a3), (b1, b2, b3) = bf16_parts(a), bf16_parts(b)
             for lost in (a1 @ b3 + a3 @ b1, a2 @ b2, a1 @ b3):
